@@ -1,0 +1,323 @@
+// Embedding lookup with scaling, and its gradient by sorted tokens.
+//
+//   out[i] = scale * table[ids[i] - first],  dtable[v] = scale * sum of dy[i] over ids[i] == first + v
+//
+// Gradient, three launches. (1) One cluster sorts the positions by token (key_sort.cuh) and marks
+// the rows that occur. (2) The sorted positions are cut into windows of equal length, so a token
+// that is everywhere is summed by many blocks: a block adds the rows of its window in order and
+// writes every token that lies wholly in it; the part of a token that runs over the window's
+// edge goes to a 32-bit partial row. The same launch writes zeros to the rows that do not occur.
+// (3) The partial rows of a token are added in order. Every row of dtable is written once, by
+// one block, and every sum has a fixed order.
+// Bound by memory: dy in, dtable out.
+#include "kernels/key_sort.cuh"
+#include "kernels/ops.h"
+
+#include <algorithm>
+
+namespace bccl {
+namespace ops {
+namespace {
+
+constexpr int kThreads = 256;
+
+template <int D, int E>
+__global__ void __launch_bounds__(kThreads) lookup_kernel(const KeySource key, long long n, const Bits<D>* __restrict__ table,
+                                                          long long table_stride, long long h, float scale,
+                                                          Bits<D>* __restrict__ out, long long out_stride) {
+    const long long c = (static_cast<long long>(blockIdx.y) * blockDim.x + threadIdx.x) * E;
+    if (c >= h) return;
+    for (long long i = blockIdx.x; i < n; i += gridDim.x) {
+        const unsigned int row = key(i);
+        Raw<D, E> r = zero_raw<D, E>();
+        if (row < key.bins) r = load_raw<D, E>(table + row * table_stride + c);
+        if (scale == 1.0f) {
+            store_raw_cs<D, E>(out + i * out_stride + c, r);
+        } else {
+            float f[E];
+            unpack<D, E>(r, f);
+#pragma unroll
+            for (int e = 0; e < E; ++e) f[e] = row < key.bins ? f[e] * scale : 0.0f;
+            store_f_cs<D, E>(out + i * out_stride + c, f);
+        }
+    }
+}
+
+// sorted: {row, position} of the n positions, by row; a and b are the buffers between passes
+// (the last pass writes b). present (rows bytes) marks the rows that occur.
+__global__ void __launch_bounds__(1024) position_sort_kernel(const KeySource key, long long n, int bits, int passes,
+                                                             uint2* a, uint2* b, unsigned char* present) {
+    extern __shared__ unsigned int counters[];
+    namespace cg = cooperative_groups;
+    if (present != nullptr) {
+        // Cleared by all blocks; the first pass's cluster barriers come before the last pass marks.
+        const long long threads = static_cast<long long>(gridDim.x) * blockDim.x;
+        const long long me = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
+        for (long long i = me; i < (key.bins + 15) / 16; i += threads)
+            reinterpret_cast<uint4*>(present)[i] = make_uint4(0, 0, 0, 0);
+    }
+    for (int p = 0; p < passes; ++p) {
+        // Buffers alternate so that the last pass writes b.
+        uint2* to = ((passes - 1 - p) & 1) ? a : b;
+        const uint2* from = to == a ? b : a;
+        const bool last = p == passes - 1;
+        sort_pass(
+            counters, n, p * bits, bits,
+            [&](long long i) {
+                return p == 0 ? make_uint2(key(i), static_cast<unsigned int>(i)) : __ldcg(from + i);
+            },
+            [&](unsigned int place, unsigned int k, unsigned int pos) {
+                to[place] = make_uint2(k, pos);
+                if (last && present != nullptr && k < key.bins) present[k] = 1;
+            },
+            [](unsigned int, unsigned int) {});
+    }
+}
+
+template <int OD, int E>
+__device__ __forceinline__ void write_row(Bits<OD>* p, const float (&sum)[E], float scale, bool accumulate) {
+    float f[E];
+    if (accumulate) {
+        // Plain loads: this kernel writes the array they read.
+        if constexpr (E == 1) {
+            f[0] = Ty<OD>::load(*p);
+        } else {
+            constexpr int W = Vec<OD>::E;
+#pragma unroll
+            for (int i = 0; i < E / W; ++i) {
+                float t[W];
+                Vec<OD>::unpack(*(reinterpret_cast<const uint4*>(p) + i), t);
+#pragma unroll
+                for (int e = 0; e < W; ++e) f[i * W + e] = t[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[e] = fmaf(sum[e], scale, f[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[e] = sum[e] * scale;
+    }
+    store_f_cs<OD, E>(p, f);
+}
+
+constexpr int kMaxWindow = 128;
+constexpr int kFlight = 8;  // rows of dy in flight per thread
+
+struct WindowArgs {
+    const uint2* sorted;
+    long long n, rows, h;
+    int window;
+    long long windows;
+    float* partial;  // [windows][2][h]: a token that came from the left; one that goes on to the right
+    const unsigned char* present;
+    float scale;
+    int accumulate;
+};
+
+// blockIdx.x < windows: a window of sorted positions; beyond: rows to clear. blockIdx.y: columns.
+template <int D, int OD, int E>
+__global__ void __launch_bounds__(kThreads) window_kernel(const WindowArgs a, const Bits<D>* __restrict__ dy,
+                                                          long long dy_stride, Bits<OD>* __restrict__ dtable) {
+    __shared__ uint2 item[kMaxWindow + 2];  // the window and its neighbours on either side
+    const long long c = (static_cast<long long>(blockIdx.y) * blockDim.x + threadIdx.x) * E;
+    if (blockIdx.x >= a.windows) {
+        if (c >= a.h) return;
+        float zero[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) zero[e] = 0.0f;
+        for (long long r = blockIdx.x - a.windows; r < a.rows; r += gridDim.x - a.windows)
+            if (__ldg(a.present + r) == 0) store_f_cs<OD, E>(dtable + r * a.h + c, zero);
+        return;
+    }
+    const long long w0 = static_cast<long long>(blockIdx.x) * a.window;
+    const int count = static_cast<int>(a.n - w0 < a.window ? a.n - w0 : a.window);
+    for (int i = threadIdx.x; i < count + 2; i += blockDim.x) {
+        const long long j = w0 + i - 1;
+        item[i] = j >= 0 && j < a.n ? __ldg(a.sorted + j) : make_uint2(0xffffffffu, 0);
+    }
+    __syncthreads();
+    if (c >= a.h) return;
+    const uint2* it = item + 1;
+    float sum[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum[e] = 0.0f;
+    bool from_left = it[-1].x == it[0].x;
+    for (int i0 = 0; i0 < count; i0 += kFlight) {
+        Raw<D, E> r[kFlight];
+#pragma unroll
+        for (int u = 0; u < kFlight; ++u) {
+            r[u] = zero_raw<D, E>();
+            if (i0 + u < count && it[i0 + u].x < a.rows)
+                r[u] = load_raw_cs<D, E>(dy + static_cast<long long>(it[i0 + u].y) * dy_stride + c);
+        }
+#pragma unroll
+        for (int u = 0; u < kFlight; ++u) {
+            const int i = i0 + u;
+            if (i >= count) break;
+            const unsigned int row = it[i].x;
+            if (row >= a.rows) return;  // sorted last: nothing but dropped positions follows
+            float f[E];
+            unpack<D, E>(r[u], f);
+#pragma unroll
+            for (int e = 0; e < E; ++e) sum[e] += f[e];
+            if (it[i + 1].x == row && i + 1 < count) continue;
+            const bool to_right = it[i + 1].x == row;
+            if (from_left || to_right) {
+                float* p = a.partial + (static_cast<long long>(blockIdx.x) * 2 + (from_left ? 0 : 1)) * a.h + c;
+                store_f<kF32, E>(reinterpret_cast<Bits<kF32>*>(p), sum);
+            } else {
+                write_row<OD, E>(dtable + row * a.h + c, sum, a.scale, a.accumulate != 0);
+            }
+            from_left = false;
+#pragma unroll
+            for (int e = 0; e < E; ++e) sum[e] = 0.0f;
+        }
+    }
+}
+
+// The window in which a token begins that runs over its right edge adds the token's partial rows.
+template <int OD, int E>
+__global__ void __launch_bounds__(kThreads) join_kernel(const WindowArgs a, Bits<OD>* __restrict__ dtable) {
+    const long long w = blockIdx.x;
+    const long long end = (w + 1) * a.window;  // windows but the last are full
+    if (end >= a.n) return;
+    const unsigned int row = __ldg(&a.sorted[end - 1].x);
+    if (row >= a.rows || __ldg(&a.sorted[end].x) != row) return;
+    const long long begin = w * a.window;
+    if (begin > 0 && __ldg(&a.sorted[begin - 1].x) == row) return;  // it began in an earlier window
+    // The last window that holds the token: the last whose first position has it.
+    long long lo = w + 1, hi = a.windows;
+    while (hi - lo > 1) {
+        const long long mid = (lo + hi) >> 1;
+        if (__ldg(&a.sorted[mid * a.window].x) == row) lo = mid; else hi = mid;
+    }
+    const long long c = (static_cast<long long>(blockIdx.y) * blockDim.x + threadIdx.x) * E;
+    if (c >= a.h) return;
+    float sum[E];
+    load_f<kF32, E>(reinterpret_cast<const Bits<kF32>*>(a.partial + (w * 2 + 1) * a.h + c), sum);
+#pragma unroll 4
+    for (long long k = w + 1; k <= lo; ++k) {
+        float f[E];
+        load_f<kF32, E>(reinterpret_cast<const Bits<kF32>*>(a.partial + k * 2 * a.h + c), f);
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum[e] += f[e];
+    }
+    write_row<OD, E>(dtable + row * a.h + c, sum, a.scale, a.accumulate != 0);
+}
+
+// Positions per window: long ones make fewer partial rows, short ones more blocks.
+int window_of(long long n) {
+    int w = 16;
+    while (w < kMaxWindow && ceil_div(n, 2 * w) >= 512) w *= 2;
+    return w;
+}
+
+size_t align16(size_t v) { return (v + 15) / 16 * 16; }
+
+}  // namespace
+}  // namespace ops
+
+cudaError_t LaunchEmbeddingForward(const EmbeddingArgs& a, const void* table, long long table_stride, float scale,
+                                   void* out, long long out_stride, int dtype, cudaStream_t stream) {
+    using namespace ops;
+    if (a.n == 0 || a.h == 0) return cudaSuccess;
+    const int size = size_of(dtype);
+    const bool wide = rows16(table, table_stride, a.h, size) && rows16(out, out_stride, a.h, size);
+    const KeySource key{a.ids, a.ids64, a.first, a.rows, 0, 0};
+    return with_type(dtype, [&](auto D) {
+        constexpr int kD = decltype(D)::value, kE = Vec<kD>::E;
+        auto go = [&](auto EE) {
+            constexpr int E = decltype(EE)::value;
+            const int threads = static_cast<int>(std::min<long long>(kThreads, round32(ceil_div(a.h, E))));
+            const dim3 grid(static_cast<unsigned>(std::min<long long>(a.n, 1 << 20)),
+                            static_cast<unsigned>(ceil_div(a.h, static_cast<long long>(threads) * E)));
+            lookup_kernel<kD, E><<<grid, threads, 0, stream>>>(key, a.n, static_cast<const Bits<kD>*>(table),
+                                                               table_stride, a.h, scale, static_cast<Bits<kD>*>(out),
+                                                               out_stride);
+            return cudaGetLastError();
+        };
+        return wide ? go(Int<kE>{}) : go(Int<1>{});
+    });
+}
+
+size_t EmbeddingBackwardWorkspace(long long n, long long rows, long long h) {
+    using namespace ops;
+    const long long windows = ceil_div(n, window_of(n));
+    return 2 * align16(sizeof(uint2) * static_cast<size_t>(n)) + align16(static_cast<size_t>(rows)) +
+           align16(sizeof(float) * 2 * static_cast<size_t>(windows) * static_cast<size_t>(h));
+}
+
+cudaError_t LaunchEmbeddingBackward(const EmbeddingArgs& a, const void* dy, long long dy_stride, void* dtable,
+                                    float scale, long long skip, bool has_skip, bool accumulate, int dtype,
+                                    int out_dtype, void* workspace, cudaStream_t stream) {
+    using namespace ops;
+    if (a.rows == 0 || a.h == 0) return cudaSuccess;
+    if (a.n == 0) {
+        if (accumulate) return cudaSuccess;
+        return cudaMemsetAsync(dtable, 0, static_cast<size_t>(a.rows) * a.h * size_of(out_dtype), stream);
+    }
+    char* ws = static_cast<char*>(workspace);
+    uint2* buf_a = reinterpret_cast<uint2*>(ws);
+    ws += align16(sizeof(uint2) * static_cast<size_t>(a.n));
+    uint2* buf_b = reinterpret_cast<uint2*>(ws);
+    ws += align16(sizeof(uint2) * static_cast<size_t>(a.n));
+    unsigned char* present = reinterpret_cast<unsigned char*>(ws);
+    ws += align16(static_cast<size_t>(a.rows));
+    float* partial = reinterpret_cast<float*>(ws);
+
+    int key_bits = 1;
+    while (key_bits < 31 && (1ll << key_bits) < a.rows + 1) ++key_bits;
+    const int passes = static_cast<int>(ceil_div(key_bits, kSortMaxBits));
+    const int bits = static_cast<int>(ceil_div(key_bits, passes));
+    const KeySource key{a.ids, a.ids64, a.first, a.rows, skip, has_skip ? 1 : 0};
+    cudaError_t e = cudaFuncSetAttribute(position_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(sort_smem(1024, kSortMaxBits)));
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = sort_blocks(a.n);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(sort_blocks(a.n));
+    cfg.blockDim = dim3(1024);
+    cfg.dynamicSmemBytes = sort_smem(1024, bits);
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, position_sort_kernel, key, a.n, bits, passes, buf_a, buf_b,
+                           accumulate ? static_cast<unsigned char*>(nullptr) : present);
+    if (e != cudaSuccess) return e;
+
+    WindowArgs w{};
+    w.sorted = buf_b;
+    w.n = a.n;
+    w.rows = a.rows;
+    w.h = a.h;
+    w.window = window_of(a.n);
+    w.windows = ceil_div(a.n, w.window);
+    w.partial = partial;
+    w.present = present;
+    w.scale = scale;
+    w.accumulate = accumulate ? 1 : 0;
+    const bool wide = rows16(dy, dy_stride, a.h, size_of(dtype)) && rows16(dtable, a.h, a.h, size_of(out_dtype));
+    return with_types(dtype, out_dtype, [&](auto D, auto O) {
+        constexpr int kD = decltype(D)::value, kO = decltype(O)::value, kE = Vec<kD>::E;
+        auto go = [&](auto EE) {
+            constexpr int E = decltype(EE)::value;
+            const int threads = static_cast<int>(std::min<long long>(kThreads, round32(ceil_div(a.h, E))));
+            const unsigned cols = static_cast<unsigned>(ceil_div(a.h, static_cast<long long>(threads) * E));
+            const long long clear =
+                accumulate ? 0 : std::max(1ll, std::min<long long>(a.rows, static_cast<long long>(sm_count()) * 8 / cols));
+            window_kernel<kD, kO, E><<<dim3(static_cast<unsigned>(w.windows + clear), cols), threads, 0, stream>>>(
+                w, static_cast<const Bits<kD>*>(dy), dy_stride, static_cast<Bits<kO>*>(dtable));
+            cudaError_t err = cudaGetLastError();
+            if (err != cudaSuccess || w.windows == 1) return err;
+            join_kernel<kO, E><<<dim3(static_cast<unsigned>(w.windows - 1), cols), threads, 0, stream>>>(
+                w, static_cast<Bits<kO>*>(dtable));
+            return cudaGetLastError();
+        };
+        return wide ? go(Int<kE>{}) : go(Int<1>{});
+    });
+}
+
+}  // namespace bccl

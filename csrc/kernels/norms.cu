@@ -1,0 +1,543 @@
+// Layer norm and RMS norm over the last dimension, forward and backward.
+//
+//   xh = (x - mean) * rstd,  y = xh * w + b,  rstd = 1 / sqrt(mean((x - mean)^2) + eps)
+//   g = dy * w,  dx = rstd * (g - mean(g) - xh * mean(g * xh)),  dw = sum_rows dy * xh,  db = sum_rows dy
+//   (RMS norm: mean = 0 and no mean(g) term)
+//
+// A row stays in the registers of one warp (short rows) or one block, so x is read once; the
+// variance is the mean of squared distances from the mean, not a difference of large sums.
+// Blocks are persistent and walk the rows: a thread keeps the same columns for every row, so
+// the weights are loaded once, the next row is in flight while this one is reduced, and the
+// backward pass adds dw and db up in registers. Each block then writes one row of partial sums
+// and a second kernel adds them in a fixed order (no atomics).
+// Bound by memory: x in and y out; x and dy in and dx out.
+#include "kernels/ops.h"
+#include "kernels/ops_common.cuh"
+
+#include <algorithm>
+
+namespace bccl {
+namespace ops {
+namespace {
+
+constexpr int kWarpRows = 8;  // rows of a block whose warps work on a row each
+
+// Columns of access v of a thread: accesses of neighbouring threads are adjacent.
+template <int E> __device__ __forceinline__ long long col_of(int v, int tx, int g) {
+    return static_cast<long long>(v * g + tx) * E;
+}
+
+// WARP: blockDim = (32, kWarpRows), a row per warp; else blockDim = (g, 1), a row per block.
+template <int D, int WD, int E, int NV, bool LAYER, bool WARP>
+__global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 512) norm_forward_kernel(const NormForwardArgs a) {
+    __shared__ float buf[2][32];
+    const int tx = threadIdx.x, g = blockDim.x;
+    const long long step = WARP ? static_cast<long long>(gridDim.x) * kWarpRows : gridDim.x;
+    long long row = WARP ? static_cast<long long>(blockIdx.x) * kWarpRows + threadIdx.y : blockIdx.x;
+    const int warps = g >> 5;
+    const float inv_h = 1.0f / static_cast<float>(a.h);
+    const Bits<D>* x = static_cast<const Bits<D>*>(a.x);
+    int parity = 0;
+    auto sum = [&](float v) {
+        if constexpr (WARP) return warp_sum(v);
+        const float s = block_sum(v, buf, parity, tx, warps);
+        parity ^= 1;
+        return s;
+    };
+    Raw<D, E> next[NV];
+    auto fetch = [&](long long r) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const long long c = col_of<E>(v, tx, g);
+            next[v] = c < a.h && r < a.rows ? load_raw_cs<D, E>(x + r * a.x_stride + c) : zero_raw<D, E>();
+        }
+    };
+    fetch(row);
+    for (; row < a.rows; row += step) {
+        float f[NV][E];
+        float s = 0.0f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            unpack<D, E>(next[v], f[v]);
+#pragma unroll
+            for (int e = 0; e < E; ++e) s += LAYER ? f[v][e] : f[v][e] * f[v][e];
+        }
+        fetch(row + step);
+        float mean = 0.0f;
+        if constexpr (LAYER) {
+            mean = sum(s) * inv_h;
+            s = 0.0f;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                if (col_of<E>(v, tx, g) < a.h) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        f[v][e] -= mean;
+                        s = fmaf(f[v][e], f[v][e], s);
+                    }
+                }
+            }
+        }
+        const float rstd = 1.0f / sqrtf(sum(s) * inv_h + a.eps);
+        if (tx == 0) {
+            if (LAYER) a.mean[row] = mean;
+            a.rstd[row] = rstd;
+        }
+        Bits<D>* y = static_cast<Bits<D>*>(a.y) + row * a.y_stride;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const long long c = col_of<E>(v, tx, g);
+            if (c >= a.h) continue;
+            float w[E], b[E];
+            if (a.w != nullptr) load_f<WD, E>(static_cast<const Bits<WD>*>(a.w) + c, w);
+            if (LAYER && a.b != nullptr) load_f<WD, E>(static_cast<const Bits<WD>*>(a.b) + c, b);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                f[v][e] *= rstd;
+                if (a.w != nullptr) f[v][e] *= w[e];
+                if (LAYER && a.b != nullptr) f[v][e] += b[e];
+            }
+            store_f_cs<D, E>(y + c, f[v]);
+        }
+    }
+}
+
+// Rows longer than a block's registers hold: three passes over the row, the later ones from L2.
+template <int D, int WD, int E, bool LAYER>
+__global__ void __launch_bounds__(1024) norm_forward_long_kernel(const NormForwardArgs a) {
+    __shared__ float buf[2][32];
+    const int tx = threadIdx.x;
+    const long long step = static_cast<long long>(blockDim.x) * E;
+    const float inv_h = 1.0f / static_cast<float>(a.h);
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const Bits<D>* x = static_cast<const Bits<D>*>(a.x) + row * a.x_stride;
+        Bits<D>* y = static_cast<Bits<D>*>(a.y) + row * a.y_stride;
+        float mean = 0.0f;
+        if constexpr (LAYER) {
+            float s = 0.0f;
+            for (long long c = static_cast<long long>(tx) * E; c < a.h; c += step) {
+                float f[E];
+                unpack<D, E>(load_raw<D, E>(x + c), f);
+#pragma unroll
+                for (int e = 0; e < E; ++e) s += f[e];
+            }
+            mean = block_sum(s, buf, 0, tx, blockDim.x >> 5) * inv_h;
+        }
+        float s = 0.0f;
+        for (long long c = static_cast<long long>(tx) * E; c < a.h; c += step) {
+            float f[E];
+            unpack<D, E>(load_raw<D, E>(x + c), f);
+#pragma unroll
+            for (int e = 0; e < E; ++e) s = fmaf(f[e] - mean, f[e] - mean, s);
+        }
+        const float rstd = 1.0f / sqrtf(block_sum(s, buf, 1, tx, blockDim.x >> 5) * inv_h + a.eps);
+        __syncthreads();  // RMS norm sums once per row: its buffer is free only now
+        if (tx == 0) {
+            if (LAYER) a.mean[row] = mean;
+            a.rstd[row] = rstd;
+        }
+        for (long long c = static_cast<long long>(tx) * E; c < a.h; c += step) {
+            float f[E], w[E], b[E];
+            unpack<D, E>(load_raw<D, E>(x + c), f);
+            if (a.w != nullptr) load_f<WD, E>(static_cast<const Bits<WD>*>(a.w) + c, w);
+            if (LAYER && a.b != nullptr) load_f<WD, E>(static_cast<const Bits<WD>*>(a.b) + c, b);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                f[e] = (f[e] - mean) * rstd;
+                if (a.w != nullptr) f[e] *= w[e];
+                if (LAYER && a.b != nullptr) f[e] += b[e];
+            }
+            store_f_cs<D, E>(y + c, f);
+        }
+    }
+}
+
+template <int D, int WD, int E, int NV, bool LAYER, bool WARP>
+__global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 512) norm_backward_kernel(const NormBackwardArgs a) {
+    extern __shared__ float rows_sum[];  // WARP: one row of partial sums per warp
+    __shared__ float2 buf[2][32];
+    const int tx = threadIdx.x, g = blockDim.x;
+    const long long step = WARP ? static_cast<long long>(gridDim.x) * kWarpRows : gridDim.x;
+    long long row = WARP ? static_cast<long long>(blockIdx.x) * kWarpRows + threadIdx.y : blockIdx.x;
+    const int warps = g >> 5;
+    const float inv_h = 1.0f / static_cast<float>(a.h);
+    const Bits<D>* x = static_cast<const Bits<D>*>(a.x);
+    const Bits<D>* dy = static_cast<const Bits<D>*>(a.dy);
+    int parity = 0;
+    float dw[NV][E], db[LAYER ? NV : 1][LAYER ? E : 1];
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            dw[v][e] = 0.0f;
+            if (LAYER) db[v][e] = 0.0f;
+        }
+    Raw<D, E> nx[NV], ny[NV];
+    auto fetch = [&](long long r) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const long long c = col_of<E>(v, tx, g);
+            const bool in = c < a.h && r < a.rows;
+            nx[v] = in ? load_raw_cs<D, E>(x + r * a.x_stride + c) : zero_raw<D, E>();
+            ny[v] = in ? load_raw_cs<D, E>(dy + r * a.dy_stride + c) : zero_raw<D, E>();
+        }
+    };
+    fetch(row);
+    for (; row < a.rows; row += step) {
+        const float mean = LAYER ? __ldg(a.mean + row) : 0.0f;
+        const float rstd = __ldg(a.rstd + row);
+        float xh[NV][E], gr[NV][E];
+        float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const long long c = col_of<E>(v, tx, g);
+            unpack<D, E>(nx[v], xh[v]);
+            unpack<D, E>(ny[v], gr[v]);
+            if (c >= a.h) continue;
+            float w[E];
+            if (a.w != nullptr) load_f<WD, E>(static_cast<const Bits<WD>*>(a.w) + c, w);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                xh[v][e] = (xh[v][e] - mean) * rstd;
+                dw[v][e] = fmaf(gr[v][e], xh[v][e], dw[v][e]);
+                if (LAYER) db[v][e] += gr[v][e];
+                if (a.w != nullptr) gr[v][e] *= w[e];
+                s.x += gr[v][e];
+                s.y = fmaf(gr[v][e], xh[v][e], s.y);
+            }
+        }
+        fetch(row + step);
+        if constexpr (WARP) {
+            s = warp_sum(s);
+        } else {
+            s = block_sum(s, buf, parity, tx, warps);
+            parity ^= 1;
+        }
+        const float m1 = LAYER ? s.x * inv_h : 0.0f, m2 = s.y * inv_h;
+        Bits<D>* dx = static_cast<Bits<D>*>(a.dx) + row * a.dx_stride;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const long long c = col_of<E>(v, tx, g);
+            if (c >= a.h) continue;
+#pragma unroll
+            for (int e = 0; e < E; ++e) gr[v][e] = rstd * (gr[v][e] - m1 - xh[v][e] * m2);
+            store_f_cs<D, E>(dx + c, gr[v]);
+        }
+    }
+    if (a.partials == nullptr) return;
+    // partials: [blocks][h] of dw, then of db.
+    float* pw = a.partials + blockIdx.x * a.h;
+    float* pb = a.partials + (static_cast<long long>(gridDim.x) + blockIdx.x) * a.h;
+    auto put = [&](float* to, float (&sum)[NV][E]) {
+        if constexpr (WARP) {
+            __syncthreads();
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const long long c = col_of<E>(v, tx, g) + e;
+                    if (c < a.h) rows_sum[threadIdx.y * a.h + c] = sum[v][e];
+                }
+            __syncthreads();
+            for (long long c = threadIdx.y * 32 + tx; c < a.h; c += 32 * kWarpRows) {
+                float t = 0.0f;
+#pragma unroll
+                for (int r = 0; r < kWarpRows; ++r) t += rows_sum[r * a.h + c];
+                to[c] = t;
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const long long c = col_of<E>(v, tx, g);
+                if (c < a.h) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) to[c + e] = sum[v][e];
+                }
+            }
+        }
+    };
+    if (a.dw != nullptr) put(pw, dw);
+    if constexpr (LAYER) {
+        if (a.db != nullptr) put(pb, db);
+    }
+}
+
+// Rows longer than a block's registers hold: dx in two passes over the row, and dw / db by a
+// second kernel that reads x and dy again by columns.
+template <int D, int WD, int E, bool LAYER>
+__global__ void __launch_bounds__(1024) norm_backward_long_kernel(const NormBackwardArgs a) {
+    __shared__ float2 buf[2][32];
+    const int tx = threadIdx.x;
+    const long long step = static_cast<long long>(blockDim.x) * E;
+    const float inv_h = 1.0f / static_cast<float>(a.h);
+    int parity = 0;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, parity ^= 1) {
+        const Bits<D>* x = static_cast<const Bits<D>*>(a.x) + row * a.x_stride;
+        const Bits<D>* dy = static_cast<const Bits<D>*>(a.dy) + row * a.dy_stride;
+        Bits<D>* dx = static_cast<Bits<D>*>(a.dx) + row * a.dx_stride;
+        const float mean = LAYER ? __ldg(a.mean + row) : 0.0f;
+        const float rstd = __ldg(a.rstd + row);
+        float2 s = make_float2(0.0f, 0.0f);
+        auto load = [&](long long c, float (&xh)[E], float (&gr)[E]) {
+            float w[E];
+            unpack<D, E>(load_raw<D, E>(x + c), xh);
+            unpack<D, E>(load_raw<D, E>(dy + c), gr);
+            if (a.w != nullptr) load_f<WD, E>(static_cast<const Bits<WD>*>(a.w) + c, w);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                xh[e] = (xh[e] - mean) * rstd;
+                if (a.w != nullptr) gr[e] *= w[e];
+            }
+        };
+        for (long long c = static_cast<long long>(tx) * E; c < a.h; c += step) {
+            float xh[E], gr[E];
+            load(c, xh, gr);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                s.x += gr[e];
+                s.y = fmaf(gr[e], xh[e], s.y);
+            }
+        }
+        s = block_sum(s, buf, parity, tx, blockDim.x >> 5);
+        const float m1 = LAYER ? s.x * inv_h : 0.0f, m2 = s.y * inv_h;
+        for (long long c = static_cast<long long>(tx) * E; c < a.h; c += step) {
+            float xh[E], gr[E];
+            load(c, xh, gr);
+#pragma unroll
+            for (int e = 0; e < E; ++e) gr[e] = rstd * (gr[e] - m1 - xh[e] * m2);
+            store_f_cs<D, E>(dx + c, gr);
+        }
+    }
+}
+
+template <int D, int E, bool LAYER>
+__global__ void __launch_bounds__(256) norm_columns_kernel(const NormBackwardArgs a) {
+    __shared__ float part[8][32 * E];
+    const long long c = (static_cast<long long>(blockIdx.x) * 32 + threadIdx.x) * E;
+    float dw[E] = {}, db[E] = {};
+    if (c < a.h) {
+        for (long long row = static_cast<long long>(blockIdx.y) * 8 + threadIdx.y; row < a.rows;
+             row += static_cast<long long>(gridDim.y) * 8) {
+            float x[E], dy[E];
+            unpack<D, E>(load_raw_cs<D, E>(static_cast<const Bits<D>*>(a.x) + row * a.x_stride + c), x);
+            unpack<D, E>(load_raw_cs<D, E>(static_cast<const Bits<D>*>(a.dy) + row * a.dy_stride + c), dy);
+            const float mean = LAYER ? __ldg(a.mean + row) : 0.0f, rstd = __ldg(a.rstd + row);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                dw[e] = fmaf(dy[e], (x[e] - mean) * rstd, dw[e]);
+                db[e] += dy[e];
+            }
+        }
+    }
+    auto put = [&](float* to, const float (&sum)[E]) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < E; ++e) part[threadIdx.y][threadIdx.x * E + e] = sum[e];
+        __syncthreads();
+        for (int i = threadIdx.y * 32 + threadIdx.x; i < 32 * E; i += 256) {
+            const long long col = static_cast<long long>(blockIdx.x) * 32 * E + i;
+            if (col >= a.h) continue;
+            float t = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) t += part[r][i];
+            to[col] = t;
+        }
+    };
+    if (a.dw != nullptr) put(a.partials + blockIdx.y * a.h, dw);
+    if (LAYER && a.db != nullptr) put(a.partials + (static_cast<long long>(gridDim.y) + blockIdx.y) * a.h, db);
+}
+
+// Sums `blocks` rows of partials: 32 columns per block, 32 threads down each column.
+// blockIdx.y: 0 dw, 1 db.
+template <int WD>
+__global__ void __launch_bounds__(1024) norm_weights_kernel(const float* __restrict__ partials, int blocks, long long h,
+                                                            void* dw, void* db) {
+    __shared__ float part[32][33];
+    void* out = blockIdx.y == 0 ? dw : db;
+    if (out == nullptr) return;
+    const float* p = partials + (blockIdx.y == 0 ? 0 : blocks * h);
+    const long long c = static_cast<long long>(blockIdx.x) * 32 + threadIdx.x;
+    float t = 0.0f;
+    if (c < h) {
+#pragma unroll 4
+        for (int b = threadIdx.y; b < blocks; b += 32) t += p[b * h + c];
+    }
+    part[threadIdx.y][threadIdx.x] = t;
+    __syncthreads();
+    t = warp_sum(part[threadIdx.x][threadIdx.y]);
+    const long long col = static_cast<long long>(blockIdx.x) * 32 + threadIdx.y;
+    if (threadIdx.x == 0 && col < h) static_cast<Bits<WD>*>(out)[col] = Ty<WD>::store(t);
+}
+
+// How a row is spread: accesses per thread and threads per row (32: a warp). Zero threads: long.
+struct Shape {
+    int nv, threads;
+};
+// Widths tried in order, the first that fits; more accesses per thread mean fewer warps to
+// synchronise per row, fewer accesses more rows in flight.
+Shape forward_shape(long long h, int e) {
+    const long long n = ceil_div(h, e);
+    if (e > 1) {
+        for (int nv : {1, 2, 4})
+            if (n <= 32 * nv) return {nv, 32};
+        if (n <= 512) return {1, round32(n)};
+        if (n <= 1024) return {2, round32(ceil_div(n, 2))};
+        if (n <= 2048) return {4, round32(ceil_div(n, 4))};
+        if (n <= 4096 && e == 4) return {8, round32(ceil_div(n, 8))};
+    } else {
+        for (int nv : {4, 16})
+            if (n <= 32 * nv) return {nv, 32};
+        if (n <= 2048) return {4, round32(ceil_div(n, 4))};
+        if (n <= 8192) return {16, round32(ceil_div(n, 16))};
+    }
+    return {0, 0};
+}
+Shape backward_shape(long long h, int e) {
+    const long long n = ceil_div(h, e);
+    if (e > 1) {
+        for (int nv : {1, 2})
+            if (n <= 32 * nv) return {nv, 32};
+        if (n <= 512) return {1, round32(n)};
+        if (n <= 1024) return {2, round32(ceil_div(n, 2))};
+    } else {
+        for (int nv : {4, 16})
+            if (n <= 32 * nv) return {nv, 32};
+        if (n <= 2048) return {4, round32(ceil_div(n, 4))};
+        if (n <= 8192) return {16, round32(ceil_div(n, 16))};
+    }
+    return {0, 0};
+}
+
+// Blocks of the persistent kernels: what the SMs hold (2048 threads each), no more than rows.
+int row_blocks(long long rows, int threads, int per_sm_threads) {
+    const bool warp = threads == 32;
+    const long long work = warp ? ceil_div(rows, kWarpRows) : rows;
+    const int block = warp ? 32 * kWarpRows : threads;
+    return static_cast<int>(std::max(1ll, std::min<long long>(work, static_cast<long long>(sm_count()) *
+                                                                        std::max(1, per_sm_threads / block))));
+}
+constexpr int kForwardThreads = 2048;   // resident threads per SM the forward kernels are sized for
+constexpr int kBackwardThreads = 1024;  // and the backward ones, which hold about twice the registers
+
+constexpr int kColumnChunks = 64;  // row chunks of norm_columns_kernel at most
+
+template <int D, int WD, int E, int NV, bool LAYER>
+cudaError_t forward(const NormForwardArgs& a, int threads, cudaStream_t s) {
+    const int grid = row_blocks(a.rows, threads, kForwardThreads);
+    if (threads == 32)
+        norm_forward_kernel<D, WD, E, NV, LAYER, true><<<grid, dim3(32, kWarpRows), 0, s>>>(a);
+    else
+        norm_forward_kernel<D, WD, E, NV, LAYER, false><<<grid, threads, 0, s>>>(a);
+    return cudaGetLastError();
+}
+
+template <int D, int WD, int E, bool LAYER>
+cudaError_t forward_any(const NormForwardArgs& a, cudaStream_t s) {
+    const Shape sh = forward_shape(a.h, E);
+    if constexpr (E > 1) {
+        if (sh.nv == 1) return forward<D, WD, E, 1, LAYER>(a, sh.threads, s);
+        if (sh.nv == 2) return forward<D, WD, E, 2, LAYER>(a, sh.threads, s);
+        if (sh.nv == 4) return forward<D, WD, E, 4, LAYER>(a, sh.threads, s);
+        if constexpr (E == 4) {
+            if (sh.nv == 8) return forward<D, WD, E, 8, LAYER>(a, sh.threads, s);
+        }
+    } else {
+        if (sh.nv == 4) return forward<D, WD, E, 4, LAYER>(a, sh.threads, s);
+        if (sh.nv == 16) return forward<D, WD, E, 16, LAYER>(a, sh.threads, s);
+    }
+    const int grid = static_cast<int>(std::min<long long>(a.rows, sm_count() * 2));
+    norm_forward_long_kernel<D, WD, E, LAYER><<<grid, 1024, 0, s>>>(a);
+    return cudaGetLastError();
+}
+
+template <int D, int WD, int E, int NV, bool LAYER>
+cudaError_t backward(const NormBackwardArgs& a, int threads, int grid, cudaStream_t s) {
+    if (threads == 32)
+        norm_backward_kernel<D, WD, E, NV, LAYER, true>
+            <<<grid, dim3(32, kWarpRows), sizeof(float) * kWarpRows * a.h, s>>>(a);
+    else
+        norm_backward_kernel<D, WD, E, NV, LAYER, false><<<grid, threads, 0, s>>>(a);
+    return cudaGetLastError();
+}
+
+// Rows of partial sums that the backward pass of this shape writes.
+int partial_rows(long long rows, long long h, int e) {
+    const Shape sh = backward_shape(h, e);
+    if (sh.threads != 0) return row_blocks(rows, sh.threads, kBackwardThreads);
+    return static_cast<int>(std::max(1ll, std::min<long long>(ceil_div(rows, 8), kColumnChunks)));
+}
+
+template <int D, int WD, int E, bool LAYER>
+cudaError_t backward_any(const NormBackwardArgs& a, cudaStream_t s) {
+    const Shape sh = backward_shape(a.h, E);
+    const int parts = partial_rows(a.rows, a.h, E);
+    cudaError_t e = cudaSuccess;
+    if (sh.threads != 0) {
+        if constexpr (E > 1)
+            e = sh.nv == 1 ? backward<D, WD, E, 1, LAYER>(a, sh.threads, parts, s)
+                           : backward<D, WD, E, 2, LAYER>(a, sh.threads, parts, s);
+        else
+            e = sh.nv == 4 ? backward<D, WD, E, 4, LAYER>(a, sh.threads, parts, s)
+                           : backward<D, WD, E, 16, LAYER>(a, sh.threads, parts, s);
+    } else {
+        norm_backward_long_kernel<D, WD, E, LAYER>
+            <<<static_cast<int>(std::min<long long>(a.rows, sm_count() * 2)), 1024, 0, s>>>(a);
+        e = cudaGetLastError();
+        if (e == cudaSuccess && a.partials != nullptr) {
+            const dim3 grid(static_cast<unsigned>(ceil_div(a.h, 32 * E)), parts);
+            norm_columns_kernel<D, E, LAYER><<<grid, dim3(32, 8), 0, s>>>(a);
+            e = cudaGetLastError();
+        }
+    }
+    if (e != cudaSuccess || a.partials == nullptr) return e;
+    const dim3 grid(static_cast<unsigned>(ceil_div(a.h, 32)), a.db != nullptr ? 2 : 1);
+    norm_weights_kernel<WD><<<grid, dim3(32, 32), 0, s>>>(a.partials, parts, a.h, a.dw, a.db);
+    return cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace ops
+
+cudaError_t LaunchNormForward(bool layer, const NormForwardArgs& a, int dtype, int wdtype, cudaStream_t stream) {
+    using namespace ops;
+    if (a.rows == 0) return cudaSuccess;
+    const int size = size_of(dtype);
+    const bool wide = rows16(a.x, a.x_stride, a.h, size) && rows16(a.y, a.y_stride, a.h, size) &&
+                      (a.w == nullptr || on16(a.w)) && (a.b == nullptr || on16(a.b));
+    return with_types(dtype, wdtype, [&](auto D, auto W) {
+        constexpr int kD = decltype(D)::value, kW = decltype(W)::value, kE = Vec<kD>::E;
+        if (layer)
+            return wide ? forward_any<kD, kW, kE, true>(a, stream) : forward_any<kD, kW, 1, true>(a, stream);
+        return wide ? forward_any<kD, kW, kE, false>(a, stream) : forward_any<kD, kW, 1, false>(a, stream);
+    });
+}
+
+size_t NormBackwardWorkspace(bool layer, long long rows, long long h, int dtype) {
+    using namespace ops;
+    if (rows == 0 || h == 0) return 0;
+    // Either width may run, by the alignment of the call's pointers.
+    const int parts = std::max(partial_rows(rows, h, 16 / size_of(dtype)), partial_rows(rows, h, 1));
+    return sizeof(float) * (layer ? 2 : 1) * static_cast<size_t>(parts) * static_cast<size_t>(h);
+}
+
+cudaError_t LaunchNormBackward(bool layer, NormBackwardArgs a, int dtype, int wdtype, cudaStream_t stream) {
+    using namespace ops;
+    if (a.dw == nullptr && a.db == nullptr) a.partials = nullptr;
+    if (a.rows == 0) {  // sums over no rows
+        const size_t bytes = static_cast<size_t>(a.h) * size_of(wdtype);
+        cudaError_t e = a.dw != nullptr ? cudaMemsetAsync(a.dw, 0, bytes, stream) : cudaSuccess;
+        if (e == cudaSuccess && a.db != nullptr) e = cudaMemsetAsync(a.db, 0, bytes, stream);
+        return e;
+    }
+    const int size = size_of(dtype);
+    const bool wide = rows16(a.x, a.x_stride, a.h, size) && rows16(a.dy, a.dy_stride, a.h, size) &&
+                      rows16(a.dx, a.dx_stride, a.h, size) && (a.w == nullptr || on16(a.w));
+    return with_types(dtype, wdtype, [&](auto D, auto W) {
+        constexpr int kD = decltype(D)::value, kW = decltype(W)::value, kE = Vec<kD>::E;
+        if (layer)
+            return wide ? backward_any<kD, kW, kE, true>(a, stream) : backward_any<kD, kW, 1, true>(a, stream);
+        return wide ? backward_any<kD, kW, kE, false>(a, stream) : backward_any<kD, kW, 1, false>(a, stream);
+    });
+}
+
+}  // namespace bccl

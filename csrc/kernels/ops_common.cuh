@@ -1,0 +1,180 @@
+// Shared by the compute operators (grad_norm.cu, norms.cu, embedding.cu, experts.cu): loads and
+// stores of E adjacent elements as floats, reductions over a block, launch helpers.
+//
+// Each kernel exists in two widths: E elements that fill 16 bytes, where every row starts on a
+// 16-byte boundary (base pointers and row strides), and E = 1 for every other layout. A warp's
+// 16-byte accesses cover 512 adjacent bytes; element accesses of 2 or 4 bytes 64 or 128.
+#pragma once
+
+#include "kernels/common.cuh"
+
+#include <climits>
+
+namespace bccl {
+namespace ops {
+
+using dev::kBF16;
+using dev::kF16;
+using dev::kF32;
+using dev::kI32;
+using dev::kI64;
+using dev::Ty;
+using dev::Vec;
+
+template <int D> using Bits = typename Ty<D>::Bits;
+
+// What one access of E elements holds before conversion (kept in registers for prefetching).
+template <int D, int E> struct Raw { uint4 v; };
+template <int D> struct Raw<D, 1> { Bits<D> v; };
+
+template <int D, int E>
+__device__ __forceinline__ Raw<D, E> load_raw(const Bits<D>* p) {
+    Raw<D, E> r;
+    if constexpr (E == 1) r.v = __ldg(p);
+    else r.v = __ldg(reinterpret_cast<const uint4*>(p));
+    return r;
+}
+// Streaming form for data that is read once: does not displace what other CTAs keep in L2.
+template <int D, int E>
+__device__ __forceinline__ Raw<D, E> load_raw_cs(const Bits<D>* p) {
+    Raw<D, E> r;
+    if constexpr (E == 1) r.v = __ldcs(p);
+    else r.v = __ldcs(reinterpret_cast<const uint4*>(p));
+    return r;
+}
+template <int D, int E>
+__device__ __forceinline__ void unpack(const Raw<D, E>& r, float (&a)[E]) {
+    if constexpr (E == 1) a[0] = Ty<D>::load(r.v);
+    else Vec<D>::unpack(r.v, a);
+}
+template <int D, int E>
+__device__ __forceinline__ Raw<D, E> zero_raw() {
+    Raw<D, E> r;
+    if constexpr (E == 1) r.v = 0;
+    else r.v = make_uint4(0, 0, 0, 0);
+    return r;
+}
+
+// E elements of a (possibly wider) type: vectors of parameters next to 16-bit activations.
+template <int D, int E>
+__device__ __forceinline__ void load_f(const Bits<D>* p, float (&a)[E]) {
+    if constexpr (E == 1) {
+        a[0] = Ty<D>::load(__ldg(p));
+    } else {
+        constexpr int W = Vec<D>::E;
+        static_assert(E % W == 0, "whole 16-byte accesses");
+#pragma unroll
+        for (int i = 0; i < E / W; ++i) {
+            float t[W];
+            Vec<D>::unpack(__ldg(reinterpret_cast<const uint4*>(p) + i), t);
+#pragma unroll
+            for (int e = 0; e < W; ++e) a[i * W + e] = t[e];
+        }
+    }
+}
+template <int D, int E>
+__device__ __forceinline__ void store_f(Bits<D>* p, const float (&a)[E]) {
+    if constexpr (E == 1) {
+        *p = Ty<D>::store(a[0]);
+    } else {
+        constexpr int W = Vec<D>::E;
+        static_assert(E % W == 0, "whole 16-byte accesses");
+#pragma unroll
+        for (int i = 0; i < E / W; ++i) {
+            float t[W];
+#pragma unroll
+            for (int e = 0; e < W; ++e) t[e] = a[i * W + e];
+            *(reinterpret_cast<uint4*>(p) + i) = Vec<D>::pack(t);
+        }
+    }
+}
+// Streaming stores for outputs far larger than what is read again soon.
+template <int D, int E>
+__device__ __forceinline__ void store_f_cs(Bits<D>* p, const float (&a)[E]) {
+    if constexpr (E == 1) {
+        __stcs(p, Ty<D>::store(a[0]));
+    } else {
+        constexpr int W = Vec<D>::E;
+        static_assert(E % W == 0, "whole 16-byte accesses");
+#pragma unroll
+        for (int i = 0; i < E / W; ++i) {
+            float t[W];
+#pragma unroll
+            for (int e = 0; e < W; ++e) t[e] = a[i * W + e];
+            __stcs(reinterpret_cast<uint4*>(p) + i, Vec<D>::pack(t));
+        }
+    }
+}
+template <int D, int E>
+__device__ __forceinline__ void store_raw_cs(Bits<D>* p, const Raw<D, E>& r) {
+    if constexpr (E == 1) __stcs(p, r.v);
+    else __stcs(reinterpret_cast<uint4*>(p), r.v);
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ float2 warp_sum(float2 v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+        v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    }
+    return v;
+}
+
+// Sums over all threads of a block (a multiple of 32, at most 1024) in a fixed order, result in
+// every thread. `parity` alternates between calls: a call's buffer is written again only two
+// calls later, after the barrier of the call between, so one barrier per sum is enough.
+__device__ __forceinline__ float block_sum(float v, float (&buf)[2][32], int parity, int tid, int warps) {
+    v = warp_sum(v);
+    if ((tid & 31) == 0) buf[parity][tid >> 5] = v;
+    __syncthreads();
+    return warp_sum((tid & 31) < warps ? buf[parity][tid & 31] : 0.0f);
+}
+__device__ __forceinline__ float2 block_sum(float2 v, float2 (&buf)[2][32], int parity, int tid, int warps) {
+    v = warp_sum(v);
+    if ((tid & 31) == 0) buf[parity][tid >> 5] = v;
+    __syncthreads();
+    return warp_sum((tid & 31) < warps ? buf[parity][tid & 31] : make_float2(0.0f, 0.0f));
+}
+
+inline bool float_type(int d) { return d == kF32 || d == kBF16 || d == kF16; }
+inline int size_of(int d) { return d == kF32 || d == kI32 ? 4 : d == kI64 ? 8 : 2; }
+inline bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Rows of `h` elements, `stride` apart from `p`, that all start and end on 16-byte boundaries.
+inline bool rows16(const void* p, long long stride, long long h, int size) {
+    return on16(p) && (stride * size) % 16 == 0 && (h * size) % 16 == 0;
+}
+inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+inline int round32(long long v) { return static_cast<int>((v + 31) / 32 * 32); }
+
+// SMs of the current device (148 on a B200); looked up once per device.
+int sm_count();
+
+// f(integral_constant<D>) for a floating-point type code.
+template <int V> struct Int { static constexpr int value = V; };
+template <typename F>
+cudaError_t with_type(int d, F&& f) {
+    switch (d) {
+    case kF32: return f(Int<kF32>{});
+    case kBF16: return f(Int<kBF16>{});
+    case kF16: return f(Int<kF16>{});
+    default: return cudaErrorInvalidValue;
+    }
+}
+// A type and the type of what goes with it: the same, or f32.
+template <typename F>
+cudaError_t with_types(int d, int w, F&& f) {
+    return with_type(d, [&](auto D) {
+        constexpr int kD = decltype(D)::value;
+        if (w == kD) return f(Int<kD>{}, Int<kD>{});
+        if (w == kF32) return f(Int<kD>{}, Int<kF32>{});
+        return cudaErrorInvalidValue;
+    });
+}
+
+}  // namespace ops
+}  // namespace bccl

@@ -48,6 +48,7 @@ def load(path: Path | None = None) -> ctypes.CDLL:
     _point_at_nccl()
     lib = ctypes.CDLL(str(path), mode=ctypes.RTLD_GLOBAL)
     c_int, c_size, vp, u64 = ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_uint64
+    i64, c_float = ctypes.c_int64, ctypes.c_float
     up = ctypes.c_size_t  # uintptr_t
     sig = {
         "bcclCommCreate": (c_int, [ctypes.POINTER(vp)]),
@@ -96,6 +97,20 @@ def load(path: Path | None = None) -> ctypes.CDLL:
         "bcclGemmUsesPair": (c_int, []),
         "bcclGemmTileWidth": (c_int, [c_int, c_int]),
         "bcclCommAbort": (c_int, [vp]),
+        "bcclGradSquares": (c_int, [vp, vp, c_int, c_int, c_int, vp, vp]),
+        "bcclGradClip": (c_int, [vp, vp, vp, c_int, c_int, c_int, vp, c_float, c_float, vp, vp]),
+        "bcclNormForward": (c_int, [c_int, vp, i64, vp, vp, vp, i64, vp, vp, i64, i64, c_float, c_int, c_int, vp]),
+        "bcclNormBackwardWorkspace": (c_size, [c_int, i64, i64, c_int]),
+        "bcclNormBackward": (c_int, [c_int, vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, vp, i64, i64, c_int, c_int, vp,
+                                     c_size, vp]),
+        "bcclEmbeddingForward": (c_int, [vp, c_int, i64, vp, i64, i64, i64, i64, c_float, vp, i64, c_int, vp]),
+        "bcclEmbeddingBackwardWorkspace": (c_size, [i64, i64, i64]),
+        "bcclEmbeddingBackward": (c_int, [vp, i64, vp, c_int, i64, vp, i64, i64, i64, c_float, i64, c_int, c_int, c_int,
+                                          c_int, vp, c_size, vp]),
+        "bcclExpertSort": (c_int, [vp, c_int, i64, c_int, c_int, vp, vp, vp, vp]),
+        "bcclExpertDispatch": (c_int, [vp, i64, vp, vp, i64, c_int, c_int, i64, vp, c_int, vp]),
+        "bcclExpertCombine": (c_int, [vp, vp, vp, c_int, i64, c_int, i64, vp, i64, c_int, vp]),
+        "bcclExpertCombineBackward": (c_int, [vp, i64, vp, vp, vp, vp, c_int, i64, c_int, c_int, i64, vp, vp, c_int, vp]),
         "bcclTpAllGatherGemm": (c_int, [vp, vp, vp, vp, c_int, c_int, c_int, c_int, up, c_int]),
         "bcclTpGemmReduceScatter": (c_int, [vp, vp, vp, vp, c_int, c_int, c_int, up, c_int]),
         "bcclTraceDump": (ctypes.c_long, [vp, ctypes.c_char_p]),

@@ -94,11 +94,16 @@ class LlamaMLP(nn.Module):
 
 class TinyLlamaStack(nn.Module):
     """RMSNorm + MLP residual blocks with biases: a small trainable model whose gradients have both
-    large matrices (bucketed by the data-parallel sync) and small vectors (synced as one group)."""
+    large matrices (bucketed by the data-parallel sync) and small vectors (synced as one group).
+
+    With ``vocab`` the input is token ids, looked up in an embedding table scaled by sqrt(hidden).
+    ``native=True`` (CUDA) runs the norms and the lookup, forward and backward, on this package's
+    kernels (:mod:`originccl_b200.ops`) instead of torch's; parameters and their names are the same."""
 
     def __init__(self, hidden: int = 256, ffn: int = 768, layers: int = 2, *, dtype=torch.float32, device=None,
-                 seed: int = 0) -> None:
+                 seed: int = 0, vocab: int = 0, native: bool = False) -> None:
         super().__init__()
+        self.native = native
         g = torch.Generator(device="cpu").manual_seed(seed)
         self.blocks = nn.ModuleList()
         for _ in range(layers):
@@ -112,8 +117,27 @@ class TinyLlamaStack(nn.Module):
                     lin.weight.copy_(torch.randn(lin.weight.shape, generator=g) * 0.02)
                     lin.bias.copy_(torch.randn(lin.bias.shape, generator=g) * 0.02)
             self.blocks.append(blk)
+        self.embed = None
+        if vocab:  # drawn last: a seed gives the blocks the same weights with and without a table
+            self.embed = nn.Parameter((torch.randn(vocab, hidden, generator=g) * 0.02).to(device=device, dtype=dtype))
+
+    def _norm(self, norm, x):
+        if not self.native:
+            return norm(x)
+        from ..ops import norm as native_norm
+        return native_norm.rms_norm(x, norm.weight, torch.finfo(x.dtype).eps if norm.eps is None else norm.eps)
+
+    def _lookup(self, ids):
+        scale = self.embed.shape[1] ** 0.5
+        if not self.native:
+            return torch.nn.functional.embedding(ids, self.embed) * scale
+        from ..ops import embedding
+        return embedding.embedding(ids, self.embed, scale=scale)
 
     def forward(self, x):
+        """x: activations [..., hidden], or token ids [...] where the stack has a table."""
+        if self.embed is not None:
+            x = self._lookup(x)
         for blk in self.blocks:
-            x = x + blk["down"](torch.nn.functional.silu(blk["up"](blk["norm"](x))))
+            x = x + blk["down"](torch.nn.functional.silu(blk["up"](self._norm(blk["norm"], x))))
         return x

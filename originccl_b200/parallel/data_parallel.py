@@ -188,6 +188,16 @@ class DataParallelSync:
         self.comm.all_reduce_many(self._bucket_batch, ReduceOp.SUM, scale=self.scale, grouped=False, stream=s)
         self._sync_small(s)
 
+    def clip_grad_norm_(self, max_norm: float, *, eps: float = 1e-6, shards=None):
+        """Scales the synced gradients by ``min(1, max_norm / (norm + eps))`` and returns their global
+        norm (a float32 tensor of no dimensions; the host does not wait). Call it after :meth:`sync` or
+        :meth:`finish`: every rank then holds the same gradients and computes the same norm. Where the
+        parameters are also sharded, ``shards`` is the communicator of the ranks that hold the other
+        shards (``Mesh.tp``), and all of them call this together."""
+        from ..ops import gradients
+        flats = [t for t in (self.grads.flat, self.grads.small_flat) if t.numel()]
+        return gradients.clip_grad_norm(flats, max_norm, eps=eps, comm=shards)
+
     def _sync_small(self, s) -> None:
         if self._small_batch.n:
             self.comm.all_reduce_many(self._small_batch, ReduceOp.SUM, scale=self.scale, grouped=True, stream=s)

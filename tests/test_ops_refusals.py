@@ -1,0 +1,205 @@
+"""Argument checks of the compute operators and their host path (CPU): wrong types, shapes, devices and
+sizes are refused in Python or by the C interface before any pointer reaches a kernel."""
+import ctypes
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from originccl_b200 import _native  # noqa: E402
+from originccl_b200.ops import embedding, experts, gradients, norm  # noqa: E402
+
+bf = torch.bfloat16
+
+
+def test_norms_refuse():
+    x, w = torch.zeros(4, 8, dtype=bf), torch.zeros(8, dtype=bf)
+    with pytest.raises(TypeError, match="float32"):
+        norm.rms_norm_forward(x.double())
+    with pytest.raises(TypeError, match="weight"):
+        norm.rms_norm_forward(x, w.half())
+    with pytest.raises(TypeError, match="bias"):
+        norm.layer_norm_forward(x, w, w.float())
+    with pytest.raises(TypeError, match="bias"):
+        norm.layer_norm_forward(x, None, w)
+    with pytest.raises(ValueError, match="shape"):
+        norm.layer_norm_forward(x, torch.zeros(7, dtype=bf))
+    with pytest.raises(ValueError, match="last dimension"):
+        norm.layer_norm_forward(torch.zeros(4, 0))
+    with pytest.raises(ValueError, match="last dimension"):
+        norm.rms_norm_forward(torch.zeros(()))
+    with pytest.raises(ValueError, match="eps"):
+        norm.layer_norm_forward(x, w, eps=-1.0)
+    with pytest.raises(ValueError, match="eps"):
+        norm.layer_norm_forward(x, w, eps=float("nan"))
+    with pytest.raises(ValueError, match="CUDA"):
+        norm.layer_norm_forward(x, w)
+    with pytest.raises(ValueError, match="dy"):
+        norm.rms_norm_backward(x.float(), x, torch.zeros(4), w)
+    with pytest.raises(ValueError, match="dy"):
+        norm.rms_norm_backward(x[:3], x, torch.zeros(4), w)
+    with pytest.raises(ValueError, match="rstd"):
+        norm.rms_norm_backward(x, x, torch.zeros(3), w)
+    with pytest.raises(ValueError, match="mean"):
+        norm.layer_norm_backward(x, x, torch.zeros(4, dtype=bf), torch.zeros(4), w)
+
+
+def test_embedding_refuses():
+    ids, w = torch.zeros(5, dtype=torch.int64), torch.zeros(6, 8, dtype=bf)
+    with pytest.raises(TypeError, match="ids"):
+        embedding.embedding_forward(ids.to(torch.int16), w)
+    with pytest.raises(TypeError, match="weight"):
+        embedding.embedding_forward(ids, w.double())
+    with pytest.raises(ValueError, match="2-D"):
+        embedding.embedding_forward(ids, w[0])
+    with pytest.raises(ValueError, match="first_row"):
+        embedding.embedding_forward(ids, w, first_row=-1)
+    with pytest.raises(ValueError, match="CUDA"):
+        embedding.embedding_forward(ids, w)
+    dy = torch.zeros(5, 8, dtype=bf)
+    with pytest.raises(ValueError, match="one row per id"):
+        embedding.embedding_backward(dy[:4], ids, 6)
+    with pytest.raises(ValueError, match="padding_idx"):
+        embedding.embedding_backward(dy, ids, 6, padding_idx=-1)
+    with pytest.raises(ValueError, match="padding_idx"):
+        embedding.embedding(ids, w, padding_idx=-2)
+    with pytest.raises(ValueError, match="num_rows"):
+        embedding.embedding_backward(dy, ids, -1)
+    with pytest.raises(ValueError, match="accumulate"):
+        embedding.embedding_backward(dy, ids, 6, accumulate=True)
+
+
+def test_experts_refuse():
+    ids = torch.zeros(5, 2, dtype=torch.int32)
+    with pytest.raises(TypeError, match="expert_ids"):
+        experts.sort_by_expert(ids.float(), 4)
+    with pytest.raises(ValueError, match="experts"):
+        experts.sort_by_expert(ids, 1024)
+    with pytest.raises(ValueError, match="experts"):
+        experts.sort_by_expert(ids, 0)
+    with pytest.raises(ValueError, match="per token"):
+        experts.sort_by_expert(torch.zeros(5, 65, dtype=torch.int32), 100)
+    with pytest.raises(ValueError, match="per token"):
+        experts.sort_by_expert(torch.zeros(5, 0, dtype=torch.int32), 100)
+    with pytest.raises(ValueError, match="tokens, top"):
+        experts.sort_by_expert(ids[None], 4)
+    with pytest.raises(ValueError, match="CUDA"):
+        experts.sort_by_expert(ids, 4)
+    order = experts.ExpertOrder(ids, ids.reshape(-1), torch.zeros(5, dtype=torch.int32))
+    assert order.num_experts == 4
+    with pytest.raises(ValueError, match="split"):
+        order.rank_counts(3)
+    with pytest.raises(ValueError, match="CUDA"):
+        experts.dispatch_forward(torch.zeros(5, 8), order)
+    with pytest.raises(ValueError, match="order"):
+        experts.dispatch_forward(torch.zeros(5, 8), order._replace(slots=ids.long()))
+
+
+def test_clipping_refuses():
+    g = torch.ones(4)
+    with pytest.raises(ValueError, match="no gradients"):
+        gradients.grad_norm([])
+    with pytest.raises(ValueError, match="max_norm"):
+        gradients.clip_grad_norm([g], -1.0)
+    with pytest.raises(ValueError, match="max_norm"):
+        gradients.clip_grad_norm([g], float("nan"))
+    with pytest.raises(ValueError, match="eps"):
+        gradients.clip_grad_norm([g], 1.0, eps=-1e-6)
+    with pytest.raises(ValueError, match="outs"):
+        gradients.clip_grad_norm([g], 1.0, outs=[])
+    with pytest.raises(ValueError, match="gradients"):
+        gradients.clip_grad_norm([g.double()], 1.0)
+
+
+def test_host_gradients_are_clipped():
+    grads = [torch.full((3, 4), 2.0), torch.full((5,), -1.0, dtype=bf)]
+    norm64 = (48.0 + 5.0) ** 0.5
+    got = gradients.clip_grad_norm(grads, 1.0)
+    assert abs(got.item() - norm64) <= norm64 * 2 ** -23
+    assert torch.allclose(grads[0], torch.full((3, 4), 2.0 / norm64), rtol=2 ** -21)
+    assert torch.allclose(grads[1].float(), torch.full((5,), -1.0 / norm64), rtol=2 ** -8)
+    assert gradients.grad_norm(grads).item() <= 1.0 + 2 ** -8
+
+
+def p(n):
+    return ctypes.c_void_p(n)
+
+
+def test_the_c_interface_refuses():
+    """Bad arguments return an error with a message; no GPU is needed to refuse them."""
+    lib = _native.lib()
+
+    def refused(rc, what):
+        assert rc != 0 and what in _native.last_error(), _native.last_error()
+    one = (ctypes.c_size_t * 1)(4)
+    tensor = (ctypes.c_void_p * 1)(64)
+    odd = (ctypes.c_void_p * 1)(66)
+    refused(lib.bcclGradSquares(tensor, one, -1, 0, 0, p(64), None), "tensor list")
+    refused(lib.bcclGradSquares(None, one, 1, 0, 0, p(64), None), "tensor list")
+    refused(lib.bcclGradSquares(tensor, one, 1, 1, 0, p(64), None), "dtype")
+    refused(lib.bcclGradSquares(odd, one, 1, 0, 0, p(64), None), "misaligned")
+    refused(lib.bcclGradSquares(tensor, one, 1, 0, 0, None, None), "partials")
+    refused(lib.bcclGradClip(tensor, tensor, one, 1, 4, 0, p(64), 1.0, 0.0, None, None), "in place")
+    refused(lib.bcclGradClip(tensor, tensor, one, 1, 0, 4, p(64), 1.0, 0.0, None, None), "dtypes")
+    refused(lib.bcclGradClip(tensor, tensor, one, 1, 0, 0, p(64), -1.0, 0.0, None, None), "max_norm")
+    refused(lib.bcclGradClip(tensor, tensor, one, 1, 0, 0, p(64), float("nan"), 0.0, None, None), "max_norm")
+
+    def fwd(kind=0, x=64, xs=8, w=64, b=64, y=64, ys=8, mean=64, rstd=64, rows=2, h=8, eps=1e-5, d=0, wd=0):
+        return lib.bcclNormForward(kind, p(x), xs, p(w), p(b), p(y), ys, p(mean), p(rstd), rows, h, eps, d, wd, None)
+    refused(fwd(kind=2), "kind")
+    refused(fwd(kind=1), "bias")
+    refused(fwd(d=2), "dtypes")
+    refused(fwd(d=0, wd=4), "dtypes")
+    refused(fwd(h=0), "shape")
+    refused(fwd(h=(1 << 23) + 1), "shape")
+    refused(fwd(rows=-1), "shape")
+    refused(fwd(eps=-1.0), "eps")
+    refused(fwd(x=0), "input")
+    refused(fwd(x=66), "input")
+    refused(fwd(ys=7), "input or output")
+    refused(fwd(xs=-8), "input")
+    refused(fwd(rstd=0), "statistics")
+    refused(fwd(mean=0), "statistics")
+
+    def bwd(ws=64, size=1 << 30, **k):
+        a = dict(kind=0, dy=64, x=64, mean=64, rstd=64, w=64, dx=64, dxs=8, dw=64, db=64, rows=2, h=8, d=0, wd=0)
+        a.update(k)
+        return lib.bcclNormBackward(a["kind"], p(a["dy"]), 8, p(a["x"]), 8, p(a["mean"]), p(a["rstd"]), p(a["w"]), p(a["dx"]),
+                                    a["dxs"], p(a["dw"]), p(a["db"]), a["rows"], a["h"], a["d"], a["wd"], p(ws), size, None)
+    assert lib.bcclNormBackwardWorkspace(0, 2, 8, 0) > 0
+    refused(bwd(size=lib.bcclNormBackwardWorkspace(0, 2, 8, 0) - 1), "workspace")
+    refused(bwd(ws=0), "workspace")
+    refused(bwd(ws=72), "workspace")
+    refused(bwd(kind=1), "gradient")
+    refused(bwd(dxs=4), "input or output")
+    refused(bwd(dy=0), "input")
+
+    def emb(ids=64, it=3, n=2, t=64, ts=8, rows=4, h=8, first=0, out=64, os=8, d=0):
+        return lib.bcclEmbeddingForward(p(ids), it, n, p(t), ts, rows, h, first, 1.0, p(out), os, d, None)
+    refused(emb(it=0), "dtypes")
+    refused(emb(ids=0), "ids")
+    refused(emb(ids=68), "ids")
+    refused(emb(n=1 << 31), "shape")
+    refused(emb(rows=(1 << 31) - 1), "shape")
+    refused(emb(first=-1), "shape")
+    refused(emb(t=0), "table")
+    refused(emb(os=4), "output")
+
+    def embb(size=1 << 40, **k):
+        a = dict(n=2, rows=4, h=8, d=4, od=4, ws=64)
+        a.update(k)
+        return lib.bcclEmbeddingBackward(p(64), 8, p(64), 3, a["n"], p(64), a["rows"], a["h"], 0, 1.0, 0, 0, 0, a["d"], a["od"],
+                                         p(a["ws"]), size, None)
+    refused(embb(size=lib.bcclEmbeddingBackwardWorkspace(2, 4, 8) - 1), "workspace")
+    refused(embb(od=5), "dtypes")
+    refused(embb(n=-1), "shape")
+
+    refused(lib.bcclExpertSort(p(64), 2, 4, 65, 8, p(64), p(64), p(64), None), "shape")
+    refused(lib.bcclExpertSort(p(64), 2, 4, 2, 1024, p(64), p(64), p(64), None), "shape")
+    refused(lib.bcclExpertSort(p(64), 2, (1 << 31) // 2, 2, 8, p(64), p(64), p(64), None), "shape")
+    refused(lib.bcclExpertSort(p(64), 2, 4, 2, 8, p(0), p(64), p(64), None), "null")
+    refused(lib.bcclExpertDispatch(p(64), 8, p(64), p(64), 4, 2, 8, 0, p(64), 0, None), "shape")
+    refused(lib.bcclExpertDispatch(p(66), 8, p(64), p(64), 4, 2, 8, 8, p(64), 0, None), "misaligned")
+    refused(lib.bcclExpertCombine(p(64), p(64), p(64), 4, 4, 2, 8, p(64), 8, 0, None), "dtypes")
+    refused(lib.bcclExpertCombine(p(64), None, p(64), 0, 4, 2, 8, p(64), 8, 0, None), "null")
+    refused(lib.bcclExpertCombineBackward(p(64), 8, p(0), p(64), p(64), p(64), 0, 4, 2, 8, 8, p(64), p(64), 0, None), "null")
