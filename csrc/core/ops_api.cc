@@ -38,25 +38,28 @@ cudaStream_t Stream(void* s) { return static_cast<cudaStream_t>(s); }
 
 extern "C" {
 
-int bcclGradSquares(const void* const* grads, const size_t* counts, int n, int dtype, int accumulate,
-                    double* partials, void* stream) {
+int bcclGradSquares(const void* const* grads, const size_t* counts, int n, int dtype, int accumulate, double* sum,
+                    void* workspace, size_t workspace_bytes, void* stream) {
     const char* op = "grad squares";
     if (n < 0 || (n > 0 && (grads == nullptr || counts == nullptr))) return Bad(op, "invalid tensor list");
     if (!FloatType(dtype)) return Bad(op, "invalid dtype (f32, bf16, f16)");
-    if (partials == nullptr || !Aligned(partials, 8)) return Bad(op, "partials must be an array of doubles");
+    if (sum == nullptr || !Aligned(sum, 8)) return Bad(op, "sum must be a double");
     for (int i = 0; i < n; ++i)
         if (counts[i] > 0 && (grads[i] == nullptr || !Aligned(grads[i], SizeOf(dtype))))
             return Bad(op, "null or misaligned tensor");
-    return Launched(op, bccl::LaunchGradSquares(grads, counts, n, dtype, accumulate != 0, partials, Stream(stream)));
+    if (workspace == nullptr || !Aligned(workspace, 16) ||
+        workspace_bytes < bccl::GradSquaresWorkspace(grads, counts, n, dtype))
+        return Bad(op, "workspace too small or misaligned");
+    return Launched(op, bccl::LaunchGradSquares(grads, counts, n, dtype, accumulate != 0, sum, workspace, Stream(stream)));
 }
 
 int bcclGradClip(const void* const* grads, void* const* outs, const size_t* counts, int n, int dtype, int out_dtype,
-                 const double* partials, float max_norm, float eps, float* norm, void* stream) {
+                 const double* sum, float max_norm, float eps, float* norm, void* stream) {
     const char* op = "grad clip";
     if (n < 0 || (n > 0 && (grads == nullptr || outs == nullptr || counts == nullptr)))
         return Bad(op, "invalid tensor list");
     if (!FloatType(dtype) || !SameOrF32(out_dtype, dtype)) return Bad(op, "invalid dtypes (out: the gradients' or f32)");
-    if (partials == nullptr || !Aligned(partials, 8)) return Bad(op, "partials must be an array of doubles");
+    if (sum == nullptr || !Aligned(sum, 8)) return Bad(op, "sum must be a double");
     if (!(max_norm >= 0.0f) || !(eps >= 0.0f)) return Bad(op, "max_norm and eps must not be negative or NaN");
     for (int i = 0; i < n; ++i) {
         if (counts[i] == 0) continue;
@@ -65,7 +68,7 @@ int bcclGradClip(const void* const* grads, void* const* outs, const size_t* coun
             return Bad(op, "null or misaligned tensor");
         if (grads[i] == outs[i] && dtype != out_dtype) return Bad(op, "in place needs one dtype");
     }
-    return Launched(op, bccl::LaunchGradClip(grads, outs, counts, n, dtype, out_dtype, partials, max_norm, eps, norm,
+    return Launched(op, bccl::LaunchGradClip(grads, outs, counts, n, dtype, out_dtype, sum, max_norm, eps, norm,
                                              Stream(stream)));
 }
 

@@ -26,18 +26,18 @@ extern "C" {
 #endif
 
 /* ---- Gradients. Global norm: sqrt(sum over tensors and elements of g^2).
- * bcclGradSquares writes (accumulate == 0) or adds to (accumulate != 0) BCCL_GRAD_PARTIALS partial
- * sums of squares; calls for lists of different types add to the same array, and ranks that hold
- * shards of the parameters may AllReduce (SUM) it before it is used. The sums do not depend on
- * timing. The pointer and count arrays are host memory, read before the call returns.
- * bcclGradClip: norm = sqrt(sum of partials), c = min(1, max_norm / (norm + eps)), NaN kept;
- * outs[i] = c * grads[i] (outs[i] == grads[i] with one type: in place, and nothing is moved when
- * c == 1). norm (one float, may be NULL) receives the norm. n may be 0. */
-#define BCCL_GRAD_PARTIALS 592
+ * bcclGradSquares writes (accumulate == 0) the sum of the squares to *sum or adds it (accumulate != 0: lists of
+ * another type); ranks that hold shards of the parameters may AllReduce (SUM) it before it is used. The
+ * sum does not depend on timing. The pointer and count arrays are host memory, read before the call
+ * returns. workspace_bytes of BCCL_GRAD_WORKSPACE(total elements, n) are always enough.
+ * bcclGradClip: norm = sqrt(*sum), c = min(1, max_norm / (norm + eps)), NaN kept; outs[i] = c * grads[i]
+ * (outs[i] == grads[i] with one type: in place, and nothing is moved when c == 1). Outputs must not
+ * otherwise overlap tensors of the list. norm (one float, may be NULL) receives the norm. n may be 0. */
+#define BCCL_GRAD_WORKSPACE(elements, n) (((size_t)(elements) / 8192 + 2 * (size_t)(n) + 1) * sizeof(double))
 int bcclGradSquares(const void* const* grads_host, const size_t* counts_host, int n, int dtype, int accumulate,
-                    double* partials, void* stream);
+                    double* sum, void* workspace, size_t workspace_bytes, void* stream);
 int bcclGradClip(const void* const* grads_host, void* const* outs_host, const size_t* counts_host, int n, int dtype,
-                 int out_dtype, const double* partials, float max_norm, float eps, float* norm, void* stream);
+                 int out_dtype, const double* sum, float max_norm, float eps, float* norm, void* stream);
 
 /* ---- Norms over the last dimension: y = (x - mean) * rstd * weight + bias, with
  * rstd = 1 / sqrt(var + eps) and var the mean of (x - mean)^2; kind 0 layer norm, kind 1 RMS norm (mean = 0, no bias).

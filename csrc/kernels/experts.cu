@@ -177,23 +177,8 @@ cudaError_t LaunchExpertSort(const void* ids, int ids64, long long n, int expert
     if (n == 0) return cudaMemsetAsync(offsets, 0, sizeof(int) * (experts + 1), stream);
     int bits = 1;
     while ((1 << bits) < experts + 1) ++bits;
-    const int threads = 1024;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = sort_blocks(n);
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(sort_blocks(n));
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = sort_smem(threads, bits);
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    cudaError_t e = cudaFuncSetAttribute(expert_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(sort_smem(1024, kSortMaxBits)));
-    if (e != cudaSuccess) return e;
     const KeySource key{ids, ids64, 0, experts, 0, 0};
-    return cudaLaunchKernelEx(&cfg, expert_sort_kernel, key, n, bits, slots, sources, offsets);
+    return launch_sort(expert_sort_kernel, n, bits, stream, key, n, bits, slots, sources, offsets);
 }
 
 cudaError_t LaunchExpertDispatch(const void* x, long long x_stride, const int* slots, const int* offsets,
@@ -259,7 +244,8 @@ cudaError_t LaunchExpertCombineBackward(const void* dy, long long dy_stride, con
             return cudaGetLastError();
         };
         if (top <= 2) return wide ? go(Int<kE>{}, Int<2>{}) : go(Int<1>{}, Int<2>{});
-        return wide ? go(Int<kE>{}, Int<4>{}) : go(Int<1>{}, Int<4>{});
+        if (top <= 4) return wide ? go(Int<kE>{}, Int<4>{}) : go(Int<1>{}, Int<4>{});
+        return wide ? go(Int<kE>{}, Int<8>{}) : go(Int<1>{}, Int<8>{});
     });
 }
 

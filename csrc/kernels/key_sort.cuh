@@ -5,8 +5,8 @@
 // distributed shared memory) and digits, and then every warp walks its stretch in order again and
 // writes each element to its place: equal digits keep their order, whatever the timing. Elements
 // between passes travel through global memory (L2); the barrier between passes is the hardware's
-// cluster barrier, so there is nothing to spin on. Bound by latency: at 65536 keys a warp has 8
-// steps of 32 keys in each of two walks per pass.
+// cluster barrier, so there is nothing to spin on. Bound by latency: a warp loads kBatch steps of
+// 32 keys at once, and stretches of one batch stay in registers for the second walk.
 #pragma once
 
 #include "kernels/ops_common.cuh"
@@ -16,7 +16,9 @@
 namespace bccl {
 namespace ops {
 
-constexpr int kSortMaxBits = 10;  // digit width: 1024 bins x 32 warps of counters fill 128 KiB
+constexpr int kSortWarps = 32;
+constexpr int kSortMaxBits = 10;  // digit width: 1024 bins, a thread each; x 32 warps of counters fill 128 KiB
+constexpr int kBatch = 8;
 
 // Key of element i: ids[i] - first where that lies in [0, bins), else `bins` (sorted last).
 struct KeySource {
@@ -33,98 +35,142 @@ struct KeySource {
     }
 };
 
-// One pass over n elements by digit (key >> shift) & (2^bits - 1). get(i) gives {key, position};
-// put(place, key, position) stores it; totals(digit, first place) is called once per digit by block 0.
-// counters: [warps][2^bits] and then 2 x 2^bits words of shared memory.
+// One pass over n elements by digit (key >> shift) & (2^bits - 1), blockDim.x == 1024. get(i) gives
+// {key, position}; put(place, key, position) stores it; totals(digit, first place) is called once
+// per digit by block 0. counters: shared memory, [warps][2^bits] and 2^bits + 32 words.
 template <typename Get, typename Put, typename Totals>
 __device__ __forceinline__ void sort_pass(unsigned int* counters, long long n, int shift, int bits, Get get, Put put,
                                           Totals totals) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
-    const int nbins = 1 << bits, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int nbins = 1 << bits, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rank = static_cast<int>(cluster.block_rank()), blocks = static_cast<int>(cluster.num_blocks());
+    const unsigned int mask = nbins - 1, lower = (1u << lane) - 1;
     unsigned int* mine = counters + warp * nbins;
-    unsigned int* block_total = counters + warps * nbins;  // read by the other blocks
-    unsigned int* place = block_total + nbins;             // scratch of the scan over digits
-    const long long per = ((n + static_cast<long long>(warps) * blocks * 32 - 1) / (static_cast<long long>(warps) * blocks * 32)) * 32;
-    const long long lo = min(n, (static_cast<long long>(rank) * warps + warp) * per), hi = min(n, lo + per);
-    const unsigned int mask = nbins - 1;
+    unsigned int* block_total = counters + kSortWarps * nbins;  // read by the other blocks
+    unsigned int* warp_total = block_total + nbins;
+    const long long share = static_cast<long long>(kSortWarps) * blocks * 32;
+    const long long per = (n + share - 1) / share * 32;
+    const long long lo = min(n, (static_cast<long long>(rank) * kSortWarps + warp) * per), hi = min(n, lo + per);
 
-    for (int i = threadIdx.x; i < warps * nbins; i += blockDim.x) counters[i] = 0;
-    __syncthreads();
-    for (long long i = lo + lane; i < hi + lane; i += 32) {  // the same trips for every lane
-        const bool in = i < hi;
-        const unsigned int d = in ? (get(i).x >> shift) & mask : nbins;
-        const unsigned int same = __match_any_sync(0xffffffffu, d);
-        if (in && lane == __ffs(same) - 1) mine[d] += __popc(same);
-        __syncwarp();
-    }
-    __syncthreads();
-    // Counts of the warps before this one, and the block's total, per digit.
-    for (int d = threadIdx.x; d < nbins; d += blockDim.x) {
-        unsigned int sum = 0;
-        for (int w = 0; w < warps; ++w) {
-            const unsigned int c = counters[w * nbins + d];
-            counters[w * nbins + d] = sum;
-            sum += c;
-        }
-        block_total[d] = sum;
-    }
-    cluster.sync();
-    for (int d = threadIdx.x; d < nbins; d += blockDim.x) {
-        unsigned int before = 0, all = 0;
-        for (int b = 0; b < blocks; ++b) {
-            const unsigned int c = cluster.map_shared_rank(block_total, b)[d];
-            if (b < rank) before += c;
-            all += c;
-        }
-        place[d] = all;
-        for (int w = 0; w < warps; ++w) counters[w * nbins + d] += before;
-    }
-    __syncthreads();
-    // Exclusive sum over digits, by one warp.
-    if (warp == 0) {
-        unsigned int run = 0;
-        for (int d0 = 0; d0 < nbins; d0 += 32) {
-            const int d = d0 + lane;
-            const unsigned int v = d < nbins ? place[d] : 0;
-            unsigned int incl = v;
+    for (int i = threadIdx.x; i < kSortWarps * nbins / 2; i += blockDim.x)
+        reinterpret_cast<uint2*>(counters)[i] = make_uint2(0, 0);
+    uint2 held[kBatch];
+    auto load = [&](long long i0) {
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const unsigned int t = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += t;
-            }
-            if (d < nbins) place[d] = run + incl - v;
-            run += __shfl_sync(0xffffffffu, incl, 31);
+        for (int b = 0; b < kBatch; ++b) {
+            const long long i = i0 + b * 32 + lane;
+            held[b] = i < hi ? get(i) : make_uint2(0, 0);
+        }
+    };
+    load(lo);
+    __syncthreads();
+    for (long long i0 = lo; i0 < hi; i0 += kBatch * 32) {
+        if (i0 != lo) load(i0);
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const long long base = i0 + b * 32;
+            if (base >= hi) break;
+            const bool in = base + lane < hi;
+            const unsigned int d = in ? (held[b].x >> shift) & mask : nbins;
+            const unsigned int same = __match_any_sync(0xffffffffu, d);
+            if (in && (same & lower) == 0) mine[d] += __popc(same);
+            __syncwarp();
         }
     }
     __syncthreads();
-    if (rank == 0)
-        for (int d = threadIdx.x; d < nbins; d += blockDim.x) totals(static_cast<unsigned int>(d), place[d]);
-    for (long long i = lo + lane; i < hi + lane; i += 32) {
-        const bool in = i < hi;
-        const uint2 kp = in ? get(i) : make_uint2(0, 0);
-        const unsigned int d = in ? (kp.x >> shift) & mask : nbins;
-        const unsigned int same = __match_any_sync(0xffffffffu, d);
-        const int leader = __ffs(same) - 1;
-        unsigned int base = 0;
-        if (in && lane == leader) {
-            base = mine[d];
-            mine[d] = base + __popc(same);
+    // A thread per digit: counts of the warps before each warp, the block's total, the blocks' totals.
+    const int d = threadIdx.x;
+    unsigned int before = 0, all = 0;
+    if (d < nbins) {
+        unsigned int c[kSortWarps];
+#pragma unroll
+        for (int w = 0; w < kSortWarps; ++w) c[w] = counters[w * nbins + d];
+#pragma unroll
+        for (int w = 0; w < kSortWarps; ++w) {
+            counters[w * nbins + d] = all;
+            all += c[w];
         }
-        base = __shfl_sync(0xffffffffu, base, leader);
-        if (in) put(place[d] + base + __popc(same & ((1u << lane) - 1)), kp.x, kp.y);
-        __syncwarp();
+        block_total[d] = all;
+    }
+    if (blocks > 1) {
+        cluster.sync();
+        all = 0;
+        if (d < nbins) {
+#pragma unroll 8
+            for (int b = 0; b < blocks; ++b) {
+                const unsigned int c = cluster.map_shared_rank(block_total, b)[d];
+                if (b < rank) before += c;
+                all += c;
+            }
+        }
+    }
+    // Exclusive sum over the digits.
+    unsigned int incl = all;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned int t = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += t;
+    }
+    if (lane == 31) warp_total[warp] = incl;
+    __syncthreads();
+    unsigned int first = lane < warp ? warp_total[lane] : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) first += __shfl_xor_sync(0xffffffffu, first, o);
+    first += incl - all;
+    if (d < nbins) {
+        if (rank == 0) totals(static_cast<unsigned int>(d), first);
+#pragma unroll
+        for (int w = 0; w < kSortWarps; ++w) counters[w * nbins + d] += first + before;
+    }
+    __syncthreads();
+    for (long long i0 = lo; i0 < hi; i0 += kBatch * 32) {
+        if (per > kBatch * 32) load(i0);
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const long long base = i0 + b * 32;
+            if (base >= hi) break;
+            const bool in = base + lane < hi;
+            const unsigned int dg = in ? (held[b].x >> shift) & mask : nbins;
+            const unsigned int same = __match_any_sync(0xffffffffu, dg);
+            const unsigned int at = in ? mine[dg] : 0;
+            __syncwarp();
+            if (in && (same & lower) == 0) mine[dg] = at + __popc(same);
+            __syncwarp();
+            if (in) put(at + __popc(same & lower), held[b].x, held[b].y);
+        }
     }
     // The next pass reads what all blocks wrote; and no block may leave, or reuse its totals,
     // while another reads them.
-    cluster.sync();
+    if (blocks > 1) cluster.sync();
+    else __syncthreads();
 }
 
-// Blocks of the cluster and their size for n elements: one block while it has few steps per warp.
-inline int sort_blocks(long long n) { return n <= 4096 ? 1 : 8; }
-inline size_t sort_smem(int threads, int bits) {
-    return sizeof(unsigned int) * (static_cast<size_t>(threads / 32) + 2) * (1u << bits);
+inline size_t sort_smem(int bits) {
+    return sizeof(unsigned int) * (static_cast<size_t>(kSortWarps + 1) * (1u << bits) + kSortWarps);
+}
+
+// Launches a kernel that sorts n elements by sort_pass: one block while it holds them in registers,
+// else a cluster of 8 (the largest that every GPU guarantees).
+template <typename... Params, typename... Args>
+cudaError_t launch_sort(void (*kernel)(Params...), long long n, int bits, cudaStream_t stream, Args... args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = n <= kSortWarps * kBatch * 32 ? 1 : 8;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(attr[0].val.clusterDim.x);
+    cfg.blockDim = dim3(kSortWarps * 32);
+    cfg.dynamicSmemBytes = sort_smem(bits);
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cfg.dynamicSmemBytes > 48 * 1024) {  // more than a kernel may have unasked
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   static_cast<int>(sort_smem(kSortMaxBits)));
+        if (e != cudaSuccess) return e;
+    }
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 }  // namespace ops

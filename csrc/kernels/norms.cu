@@ -4,12 +4,11 @@
 //   g = dy * w,  dx = rstd * (g - mean(g) - xh * mean(g * xh)),  dw = sum_rows dy * xh,  db = sum_rows dy
 //   (RMS norm: mean = 0 and no mean(g) term)
 //
-// A row stays in the registers of one warp (short rows) or one block, so x is read once; the
-// variance is the mean of squared distances from the mean, not a difference of large sums.
-// Blocks are persistent and walk the rows: a thread keeps the same columns for every row, so
-// the weights are loaded once, the next row is in flight while this one is reduced, and the
-// backward pass adds dw and db up in registers. Each block then writes one row of partial sums
-// and a second kernel adds them in a fixed order (no atomics).
+// A row stays on the chip, in the registers of one warp (short rows) or one block, so x is read
+// once; the variance is the mean of squared distances from the mean, not a difference of large
+// sums. Backward blocks walk several rows: a thread keeps the same columns for every row and adds
+// dw and db up in registers; each block then writes one row of partial sums and a second kernel adds
+// them in a fixed order (no atomics).
 // Bound by memory: x in and y out; x and dy in and dx out.
 #include "kernels/ops.h"
 #include "kernels/ops_common.cuh"
@@ -63,6 +62,15 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 512) norm_forward_kern
             for (int e = 0; e < E; ++e) s += LAYER ? f[v][e] : f[v][e] * f[v][e];
         }
         fetch(row + step);
+        // Asked for before the sums, so that they wait for x and the weights together.
+        float w[NV][E];
+        if (a.w != nullptr) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const long long c = col_of<E>(v, tx, g);
+                if (c < a.h) load_f<WD, E>(static_cast<const Bits<WD>*>(a.w) + c, w[v]);
+            }
+        }
         float mean = 0.0f;
         if constexpr (LAYER) {
             mean = sum(s) * inv_h;
@@ -88,13 +96,12 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 512) norm_forward_kern
         for (int v = 0; v < NV; ++v) {
             const long long c = col_of<E>(v, tx, g);
             if (c >= a.h) continue;
-            float w[E], b[E];
-            if (a.w != nullptr) load_f<WD, E>(static_cast<const Bits<WD>*>(a.w) + c, w);
+            float b[E];
             if (LAYER && a.b != nullptr) load_f<WD, E>(static_cast<const Bits<WD>*>(a.b) + c, b);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 f[v][e] *= rstd;
-                if (a.w != nullptr) f[v][e] *= w[e];
+                if (a.w != nullptr) f[v][e] *= w[v][e];
                 if (LAYER && a.b != nullptr) f[v][e] += b[e];
             }
             store_f_cs<D, E>(y + c, f[v]);
@@ -262,6 +269,129 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 512) norm_backward_ker
     }
 }
 
+// Rows of 16-byte accesses too long for a warp. Every thread copies its own columns of the next
+// STAGES - 1 rows of x and dy into shared memory with cp.async, and only reads what it copied
+// itself, so the copies need no barrier and keep 2 blocks' rings of up to 112 KiB in flight per SM; a
+// row costs one barrier, for its sums. The second use of a row reads it from shared memory again
+// instead of holding it in registers.
+__device__ __forceinline__ void copy16_async(void* smem, const void* global) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(smem))),
+                 "l"(global)
+                 : "memory");
+}
+
+template <int D, int WD, int NV, bool LAYER, int STAGES>
+__global__ void __launch_bounds__(512, NV <= 2 ? 2 : 1) norm_backward_ring_kernel(const NormBackwardArgs a) {
+    constexpr int E = Vec<D>::E;
+    extern __shared__ uint4 ring[];  // [STAGES][x, dy][NV][threads], then the weights' accesses
+    __shared__ float2 buf[2][32];
+    const int tx = threadIdx.x, g = blockDim.x, warps = g >> 5;
+    const float inv_h = 1.0f / static_cast<float>(a.h);
+    const Bits<D>* x = static_cast<const Bits<D>*>(a.x);
+    const Bits<D>* dy = static_cast<const Bits<D>*>(a.dy);
+    Bits<WD>* weights = reinterpret_cast<Bits<WD>*>(ring + static_cast<size_t>(STAGES) * 2 * NV * g);
+    auto issue = [&](long long row, int slot) {
+        if (row < a.rows) {
+            uint4* to = ring + static_cast<size_t>(slot) * 2 * NV * g + tx;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const long long c = col_of<E>(v, tx, g);
+                if (c < a.h) {
+                    copy16_async(to + v * g, x + row * a.x_stride + c);
+                    copy16_async(to + (NV + v) * g, dy + row * a.dy_stride + c);
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) issue(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
+    float dw[NV][E], db[LAYER ? NV : 1][E];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        const long long c = col_of<E>(v, tx, g);
+        if (a.w != nullptr && c < a.h) {  // kept as they are, at the thread's own place
+            float w[E];
+            load_f<WD, E>(static_cast<const Bits<WD>*>(a.w) + c, w);
+            store_f<WD, E>(weights + c, w);
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            dw[v][e] = 0.0f;
+            if constexpr (LAYER) db[v][e] = 0.0f;
+        }
+    }
+    int slot = 0, parity = 0;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        issue(row + static_cast<long long>(STAGES - 1) * gridDim.x, slot == 0 ? STAGES - 1 : slot - 1);
+        const float mean = LAYER ? __ldg(a.mean + row) : 0.0f;
+        const float rstd = __ldg(a.rstd + row);
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        const uint4* from = ring + static_cast<size_t>(slot) * 2 * NV * g + tx;
+        auto load = [&](int v, float (&xh)[E], float (&gr)[E], float (&w)[E]) {
+            Vec<D>::unpack(from[v * g], xh);
+            Vec<D>::unpack(from[(NV + v) * g], gr);
+#pragma unroll
+            for (int e = 0; e < E; ++e) xh[e] = (xh[e] - mean) * rstd;
+            if (a.w == nullptr) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) w[e] = 1.0f;
+            } else {
+                constexpr int W = Vec<WD>::E;
+#pragma unroll
+                for (int i = 0; i < E / W; ++i) {
+                    float t[W];
+                    Vec<WD>::unpack(reinterpret_cast<const uint4*>(weights + col_of<E>(v, tx, g))[i], t);
+#pragma unroll
+                    for (int e = 0; e < W; ++e) w[i * W + e] = t[e];
+                }
+            }
+        };
+        float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            if (col_of<E>(v, tx, g) >= a.h) continue;
+            float xh[E], gr[E], w[E];
+            load(v, xh, gr, w);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                dw[v][e] = fmaf(gr[e], xh[e], dw[v][e]);
+                if constexpr (LAYER) db[v][e] += gr[e];
+                const float gw = gr[e] * w[e];
+                if (LAYER) s.x += gw;
+                s.y = fmaf(gw, xh[e], s.y);
+            }
+        }
+        s = block_sum(s, buf, parity, tx, warps);
+        parity ^= 1;
+        const float m1 = LAYER ? s.x * inv_h : 0.0f, m2 = s.y * inv_h;
+        Bits<D>* dx = static_cast<Bits<D>*>(a.dx) + row * a.dx_stride;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const long long c = col_of<E>(v, tx, g);
+            if (c >= a.h) continue;
+            float xh[E], gr[E], w[E];
+            load(v, xh, gr, w);
+#pragma unroll
+            for (int e = 0; e < E; ++e) gr[e] = rstd * (gr[e] * w[e] - m1 - xh[e] * m2);
+            store_f_cs<D, E>(dx + c, gr);
+        }
+        slot = slot == STAGES - 1 ? 0 : slot + 1;
+    }
+    if (a.partials == nullptr) return;
+    float* pw = a.partials + blockIdx.x * a.h;
+    float* pb = a.partials + (static_cast<long long>(gridDim.x) + blockIdx.x) * a.h;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        const long long c = col_of<E>(v, tx, g);
+        if (c >= a.h) continue;
+        if (a.dw != nullptr) store_f<kF32, E>(reinterpret_cast<Bits<kF32>*>(pw + c), dw[v]);
+        if constexpr (LAYER) {
+            if (a.db != nullptr) store_f<kF32, E>(reinterpret_cast<Bits<kF32>*>(pb + c), db[v]);
+        }
+    }
+}
+
 // Rows longer than a block's registers hold: dx in two passes over the row, and dw / db by a
 // second kernel that reads x and dy again by columns.
 template <int D, int WD, int E, bool LAYER>
@@ -387,7 +517,6 @@ Shape forward_shape(long long h, int e) {
     } else {
         for (int nv : {4, 16})
             if (n <= 32 * nv) return {nv, 32};
-        if (n <= 2048) return {4, round32(ceil_div(n, 4))};
         if (n <= 8192) return {16, round32(ceil_div(n, 16))};
     }
     return {0, 0};
@@ -397,33 +526,36 @@ Shape backward_shape(long long h, int e) {
     if (e > 1) {
         for (int nv : {1, 2})
             if (n <= 32 * nv) return {nv, 32};
-        if (n <= 512) return {1, round32(n)};
         if (n <= 1024) return {2, round32(ceil_div(n, 2))};
+        if (n <= 2048) return {4, round32(ceil_div(n, 4))};
     } else {
         for (int nv : {4, 16})
             if (n <= 32 * nv) return {nv, 32};
-        if (n <= 2048) return {4, round32(ceil_div(n, 4))};
+        if (n <= 4096) return {8, round32(ceil_div(n, 8))};
         if (n <= 8192) return {16, round32(ceil_div(n, 16))};
     }
     return {0, 0};
 }
 
-// Blocks of the persistent kernels: what the SMs hold (2048 threads each), no more than rows.
-int row_blocks(long long rows, int threads, int per_sm_threads) {
+// Backward blocks that are resident at once: 1024 threads per SM at 64 registers (512 where a
+// thread holds 4 accesses), but 8 rows each where that still fills the SMs, since each block costs
+// a row of partial sums.
+int row_blocks(long long rows, int threads, int nv, int e) {
     const bool warp = threads == 32;
-    const long long work = warp ? ceil_div(rows, kWarpRows) : rows;
     const int block = warp ? 32 * kWarpRows : threads;
-    return static_cast<int>(std::max(1ll, std::min<long long>(work, static_cast<long long>(sm_count()) *
-                                                                        std::max(1, per_sm_threads / block))));
+    const int per_sm = std::max(1, std::min(8, (e > 1 && nv > 2 ? 512 : 1024) / block));
+    const long long work = warp ? ceil_div(rows, kWarpRows) : rows;
+    return static_cast<int>(std::min(std::min(work, static_cast<long long>(sm_count()) * per_sm),
+                                     std::max<long long>(sm_count(), ceil_div(work, 8))));
 }
-constexpr int kForwardThreads = 2048;   // resident threads per SM the forward kernels are sized for
-constexpr int kBackwardThreads = 1024;  // and the backward ones, which hold about twice the registers
 
 constexpr int kColumnChunks = 64;  // row chunks of norm_columns_kernel at most
 
 template <int D, int WD, int E, int NV, bool LAYER>
 cudaError_t forward(const NormForwardArgs& a, int threads, cudaStream_t s) {
-    const int grid = row_blocks(a.rows, threads, kForwardThreads);
+    // A row per block (or warp) and no persistent grid: with all SMs' blocks resident the rows in
+    // flight hide each other's latency.
+    const int grid = static_cast<int>(std::min<long long>(threads == 32 ? ceil_div(a.rows, kWarpRows) : a.rows, 1 << 20));
     if (threads == 32)
         norm_forward_kernel<D, WD, E, NV, LAYER, true><<<grid, dim3(32, kWarpRows), 0, s>>>(a);
     else
@@ -450,9 +582,9 @@ cudaError_t forward_any(const NormForwardArgs& a, cudaStream_t s) {
     return cudaGetLastError();
 }
 
-template <int D, int WD, int E, int NV, bool LAYER>
+template <int D, int WD, int E, int NV, bool LAYER, bool WARP>
 cudaError_t backward(const NormBackwardArgs& a, int threads, int grid, cudaStream_t s) {
-    if (threads == 32)
+    if (WARP)
         norm_backward_kernel<D, WD, E, NV, LAYER, true>
             <<<grid, dim3(32, kWarpRows), sizeof(float) * kWarpRows * a.h, s>>>(a);
     else
@@ -460,10 +592,32 @@ cudaError_t backward(const NormBackwardArgs& a, int threads, int grid, cudaStrea
     return cudaGetLastError();
 }
 
+template <int D, int WD, int NV, bool LAYER, int STAGES>
+cudaError_t backward_ring(const NormBackwardArgs& a, int threads, int grid, size_t smem, cudaStream_t s) {
+    auto* kernel = &norm_backward_ring_kernel<D, WD, NV, LAYER, STAGES>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+    kernel<<<grid, threads, smem, s>>>(a);
+    return cudaGetLastError();
+}
+// The deepest ring of 2 to 4 rows that leaves the SM room for all the blocks it should hold (227 KiB,
+// 1 KiB of them per block for the system).
+template <int D, int WD, int NV, bool LAYER>
+cudaError_t backward_ring(const NormBackwardArgs& a, int threads, int grid, cudaStream_t s) {
+    const size_t row = static_cast<size_t>(2) * NV * threads * 16;
+    const size_t weights = a.w != nullptr ? static_cast<size_t>(a.h) * sizeof(Bits<WD>) : 0;
+    const int per_sm = std::max(1, std::min(static_cast<int>(ceil_div(grid, sm_count())), (NV > 2 ? 512 : 1024) / threads));
+    const size_t room = static_cast<size_t>(227 * 1024) / per_sm - 2048;
+    if (weights + 4 * row <= room) return backward_ring<D, WD, NV, LAYER, 4>(a, threads, grid, weights + 4 * row, s);
+    if (weights + 3 * row <= room) return backward_ring<D, WD, NV, LAYER, 3>(a, threads, grid, weights + 3 * row, s);
+    return backward_ring<D, WD, NV, LAYER, 2>(a, threads, grid, weights + 2 * row, s);
+}
+
 // Rows of partial sums that the backward pass of this shape writes.
 int partial_rows(long long rows, long long h, int e) {
     const Shape sh = backward_shape(h, e);
-    if (sh.threads != 0) return row_blocks(rows, sh.threads, kBackwardThreads);
+    if (sh.threads != 0) return row_blocks(rows, sh.threads, sh.nv, e);
     return static_cast<int>(std::max(1ll, std::min<long long>(ceil_div(rows, 8), kColumnChunks)));
 }
 
@@ -473,12 +627,21 @@ cudaError_t backward_any(const NormBackwardArgs& a, cudaStream_t s) {
     const int parts = partial_rows(a.rows, a.h, E);
     cudaError_t e = cudaSuccess;
     if (sh.threads != 0) {
-        if constexpr (E > 1)
-            e = sh.nv == 1 ? backward<D, WD, E, 1, LAYER>(a, sh.threads, parts, s)
-                           : backward<D, WD, E, 2, LAYER>(a, sh.threads, parts, s);
-        else
-            e = sh.nv == 4 ? backward<D, WD, E, 4, LAYER>(a, sh.threads, parts, s)
-                           : backward<D, WD, E, 16, LAYER>(a, sh.threads, parts, s);
+        if constexpr (E > 1) {
+            if (sh.threads == 32)
+                e = sh.nv == 1 ? backward<D, WD, E, 1, LAYER, true>(a, sh.threads, parts, s)
+                               : backward<D, WD, E, 2, LAYER, true>(a, sh.threads, parts, s);
+            else
+                e = sh.nv == 2 ? backward_ring<D, WD, 2, LAYER>(a, sh.threads, parts, s)
+                               : backward_ring<D, WD, 4, LAYER>(a, sh.threads, parts, s);
+        } else {
+            if (sh.threads == 32)
+                e = sh.nv == 4 ? backward<D, WD, E, 4, LAYER, true>(a, sh.threads, parts, s)
+                               : backward<D, WD, E, 16, LAYER, true>(a, sh.threads, parts, s);
+            else
+                e = sh.nv == 8 ? backward<D, WD, E, 8, LAYER, false>(a, sh.threads, parts, s)
+                               : backward<D, WD, E, 16, LAYER, false>(a, sh.threads, parts, s);
+        }
     } else {
         norm_backward_long_kernel<D, WD, E, LAYER>
             <<<static_cast<int>(std::min<long long>(a.rows, sm_count() * 2)), 1024, 0, s>>>(a);

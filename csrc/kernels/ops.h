@@ -7,11 +7,11 @@
 
 namespace bccl {
 
+size_t GradSquaresWorkspace(const void* const* grads, const size_t* counts, int n, int dtype);
 cudaError_t LaunchGradSquares(const void* const* grads, const size_t* counts, int n, int dtype, bool accumulate,
-                              double* partials, cudaStream_t stream);
+                              double* sum, void* workspace, cudaStream_t stream);
 cudaError_t LaunchGradClip(const void* const* grads, void* const* outs, const size_t* counts, int n, int dtype,
-                           int out_dtype, const double* partials, float max_norm, float eps, float* norm,
-                           cudaStream_t stream);
+                           int out_dtype, const double* sum, float max_norm, float eps, float* norm, cudaStream_t stream);
 
 struct NormForwardArgs {
     const void* x;

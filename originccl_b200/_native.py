@@ -97,7 +97,7 @@ def load(path: Path | None = None) -> ctypes.CDLL:
         "bcclGemmUsesPair": (c_int, []),
         "bcclGemmTileWidth": (c_int, [c_int, c_int]),
         "bcclCommAbort": (c_int, [vp]),
-        "bcclGradSquares": (c_int, [vp, vp, c_int, c_int, c_int, vp, vp]),
+        "bcclGradSquares": (c_int, [vp, vp, c_int, c_int, c_int, vp, vp, c_size, vp]),
         "bcclGradClip": (c_int, [vp, vp, vp, c_int, c_int, c_int, vp, c_float, c_float, vp, vp]),
         "bcclNormForward": (c_int, [c_int, vp, i64, vp, vp, vp, i64, vp, vp, i64, i64, c_float, c_int, c_int, vp]),
         "bcclNormBackwardWorkspace": (c_size, [c_int, i64, i64, c_int]),

@@ -1,4 +1,8 @@
-"""What the compute ops share: dtype codes, operand checks, the call into the library."""
+"""What the compute ops share: dtype codes, operand checks, the call into the library.
+
+The smallest calls are bound by the host (a kernel of 2 us behind some 10 us of Python), so each
+operand property is read once and the entry points look nothing up by name.
+"""
 from __future__ import annotations
 
 import torch
@@ -8,59 +12,71 @@ from .. import _native
 FLOATS = {torch.float32: 0, torch.bfloat16: 4, torch.float16: 5}
 INTS = {torch.int32: 2, torch.int64: 3}
 
-_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
-_stream = (torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream")
-           else lambda d: torch.cuda.current_stream(d).cuda_stream)
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_current_stream = (torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream")
+                   else lambda d: torch.cuda.current_stream(d).cuda_stream)
 
 
-def run(function: str, device: int, *args) -> None:
-    """Calls a C entry point with the current stream of ``device`` as its last argument, with that
-    device current; raises what the library says when it refuses."""
-    fn = getattr(_native.lib(), function)
-    if _device() == device:
-        rc = fn(*args, _stream(device))
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, _stream(device))
-    if rc != 0:
-        raise RuntimeError(_native.last_error())
+class Entry:
+    """A C entry point whose last argument is the stream. Calling it with a device index first runs it
+    with that device current, on that device's current torch stream, and raises the library's
+    message when it refuses."""
+
+    __slots__ = ("name", "fn")
+
+    def __init__(self, name: str) -> None:
+        self.name, self.fn = name, None
+
+    def __call__(self, device: int, *args) -> None:
+        if self.fn is None:
+            self.fn = getattr(_native.lib(), self.name)
+        if _current_device() == device:
+            rc = self.fn(*args, _current_stream(device))
+        else:
+            with torch.cuda.device(device):
+                rc = self.fn(*args, _current_stream(device))
+        if rc != 0:
+            raise RuntimeError(_native.last_error())
 
 
-def float_code(op: str, what: str, t) -> int:
-    code = FLOATS.get(t.dtype)
+def float_code(op: str, what: str, dtype) -> int:
+    code = FLOATS.get(dtype)
     if code is None:
-        raise TypeError(f"{op}: {what} must be float32, bfloat16 or float16, got {t.dtype}")
+        raise TypeError(f"{op}: {what} must be float32, bfloat16 or float16, got {dtype}")
     return code
 
 
-def int_code(op: str, what: str, t) -> int:
-    code = INTS.get(t.dtype)
+def int_code(op: str, what: str, dtype) -> int:
+    code = INTS.get(dtype)
     if code is None:
-        raise TypeError(f"{op}: {what} must be int32 or int64, got {t.dtype}")
+        raise TypeError(f"{op}: {what} must be int32 or int64, got {dtype}")
     return code
 
 
-def like_or_f32(op: str, what: str, t, dtype) -> int:
-    """Code of a parameter next to operands of ``dtype``: the same type, or float32."""
-    if t.dtype != dtype and t.dtype != torch.float32:
-        raise TypeError(f"{op}: {what} must be {dtype} or float32, got {t.dtype}")
-    return FLOATS[t.dtype]
+def like_or_f32(op: str, what: str, got, dtype) -> int:
+    """Code of a parameter's type next to operands of ``dtype``: the same type, or float32."""
+    if got is not dtype and got is not torch.float32:
+        raise TypeError(f"{op}: {what} must be {dtype} or float32, got {got}")
+    return FLOATS[got]
 
 
 def one_device(op: str, *tensors) -> int:
     """Index of the CUDA device that holds every operand (None entries are skipped)."""
-    device = tensors[0].get_device() if tensors[0].is_cuda else -1
+    device = tensors[0].get_device()  # -1: host memory
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.get_device() != device):
+        if t is not None and (t.get_device() != device or device < 0):
             raise ValueError(f"{op}: operands must be CUDA tensors on one device, got "
                              f"{sorted({str(t.device) for t in tensors if t is not None})}")
     return device
 
 
-def rows(t):
-    """``t`` as rows of its last dimension: (tensor to read, row stride). Copies only layouts whose
-    rows are not evenly spaced with adjacent elements."""
-    h = t.shape[-1]
+def ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def rows(t, h: int):
+    """``t`` as rows of its last dimension, of ``h`` elements: (tensor to read, row stride). Copies only
+    layouts whose rows are not evenly spaced with adjacent elements."""
     if t.is_contiguous():
         return t, h
     if t.dim() == 2 and (h == 1 or t.stride(1) == 1):
@@ -68,9 +84,9 @@ def rows(t):
     return t.contiguous(), h
 
 
-def out_rows(op: str, out, shape, dtype):
+def out_rows(op: str, out, shape, dtype) -> int:
     """A caller's output of ``shape``: its row stride."""
-    if out.dtype != dtype or tuple(out.shape) != tuple(shape):
+    if out.dtype is not dtype or tuple(out.shape) != tuple(shape):
         raise ValueError(f"{op}: out must be a {dtype} tensor of shape {tuple(shape)}, got {out.dtype} "
                          f"{tuple(out.shape)}")
     h = shape[-1]

@@ -1,26 +1,27 @@
 """Global gradient norm over many tensors, and clipping by it (``csrc/kernels/grad_norm.cu``).
 
-``norm = sqrt(sum of g^2 over all tensors)``, ``c = min(1, max_norm / (norm + eps))``, ``g <- c * g``: two launches for up
-to 1024 tensors of one type, no synchronisation with the host, the same sum on every run. Where c is
+``norm = sqrt(sum of g^2 over all tensors)``, ``c = min(1, max_norm / (norm + eps))``, ``g <- c * g``: three launches
+for up to 1024 tensors of one type, no synchronisation with the host, the same sum on every run. Where c is
 1 nothing is written in place. A norm that is infinite or NaN makes c 0 or NaN, as in
 ``torch.nn.utils.clip_grad_norm_``.
 
 Gradients are float32, bfloat16 or float16, mixed if need be, each dense in memory (any order of
 dimensions). With ``comm`` the tensors are this rank's shards of the parameters (tensor
-parallelism) and the norm is that of all ranks' shards: one AllReduce of the partial sums between
-the launches; every rank of ``comm`` calls it together. Host tensors (ranks of a host communicator)
+parallelism) and the norm is that of all ranks' shards: one AllReduce of the sum of squares
+between the launches; every rank of ``comm`` calls it together. Host tensors (ranks of a host communicator)
 run on torch operations. The reference has no compute operators.
 """
 from __future__ import annotations
 
 from array import array
+from operator import attrgetter
 from typing import Optional, Sequence
 
 import torch
 
-from ._launch import FLOATS, run
+from ._launch import FLOATS, Entry
 
-PARTIALS = 592  # doubles that hold the partial sums of squares
+_squares, _clip = Entry("bcclGradSquares"), Entry("bcclGradClip")
 
 
 def _dense(t) -> bool:
@@ -35,62 +36,87 @@ def _dense(t) -> bool:
     return True
 
 
+_T = torch.Tensor
+_dtype = attrgetter("dtype")
+
+
 class _Group:
     """Pointer and count arrays of the tensors of one type (and of their outputs)."""
 
-    def __init__(self, tensors, outs) -> None:
-        first = tensors[0]
-        self.code, self.n = FLOATS[first.dtype], len(tensors)
-        self.ptrs = array("Q", [t.data_ptr() for t in tensors])
-        self.counts = array("Q", [t.numel() for t in tensors])
-        self.outs, self.out_code = self.ptrs, self.code
-        if outs is not None:
-            self.out_code = FLOATS[outs[0].dtype]
-            self.outs = array("Q", [t.data_ptr() for t in outs])
+    def __init__(self, dtype, ptrs, counts, out_dtype=None, outs=None) -> None:
+        self.code, self.n = FLOATS[dtype], len(ptrs)
+        self.ptrs, self.counts = array("Q", ptrs), array("Q", counts)
+        self.outs, self.out_code = (self.ptrs, self.code) if outs is None else (array("Q", outs), FLOATS[out_dtype])
 
     @property
     def inputs(self):
         return self.ptrs.buffer_info()[0], self.counts.buffer_info()[0]
 
 
+def _check_list(op, tensors, device):
+    """Types, device and layout of a list; the lists may be long, so each property is read once per
+    tensor in a loop that runs in C. Returns the types and whether all are contiguous."""
+    dtypes = set(map(_dtype, tensors))
+    if not dtypes <= FLOATS.keys():
+        raise TypeError(f"{op}: tensors must be float32, bfloat16 or float16, got {sorted(map(str, dtypes))}")
+    if set(map(_T.get_device, tensors)) != {device}:
+        raise ValueError(f"{op}: gradients and outs must be CUDA tensors on one device")
+    plain = all(map(_T.is_contiguous, tensors))
+    if not plain:
+        for t in tensors:
+            if not _dense(t):
+                raise ValueError(f"{op}: tensors must be dense in memory, got shape {tuple(t.shape)}, strides "
+                                 f"{t.stride()}")
+    return dtypes, plain
+
+
 def _groups(op, grads, outs, device, written=True):
     """The tensors by type, checked."""
-    for t in grads:
-        if t.dtype not in FLOATS:
-            raise TypeError(f"{op}: gradients must be float32, bfloat16 or float16, got {t.dtype}")
-        if t.get_device() != device:
-            raise ValueError(f"{op}: gradients must be CUDA tensors on one device")
-        if not t.is_contiguous() and not _dense(t):
-            raise ValueError(f"{op}: gradients must be dense in memory, got shape {tuple(t.shape)}, strides {t.stride()}")
+    dtypes, plain = _check_list(op, grads, device)
+    ptrs, counts = list(map(_T.data_ptr, grads)), list(map(_T.numel, grads))
+    optrs, odtypes = ptrs, dtypes
     if outs is not None:
-        for t, o in zip(grads, outs):
-            if o.shape != t.shape or o.get_device() != device or (o.dtype != t.dtype and o.dtype != torch.float32):
-                raise ValueError(f"{op}: each out must have its gradient's shape and device, and its type or float32")
-            if (o.stride() != t.stride() or not _dense(o)) and not (o.is_contiguous() and t.is_contiguous()):
-                raise ValueError(f"{op}: each out must be laid out like its gradient")
-            if o.data_ptr() == t.data_ptr() and o.dtype != t.dtype and o.numel():
-                raise ValueError(f"{op}: an out in its gradient's place must have its type")
-    if written:
-        ptrs = [t.data_ptr() for t in (grads if outs is None else outs) if t.numel()]
-        if len(set(ptrs)) != len(ptrs):
+        odtypes, oplain = _check_list(op, outs, device)
+        optrs = list(map(_T.data_ptr, outs))
+        same = list(map(_T.numel, outs)) == counts
+        if not (plain and oplain):  # laid out alike, whatever the order of the dimensions
+            same = same and all(o.shape == t.shape and (o.stride() == t.stride() or
+                                                        (o.is_contiguous() and t.is_contiguous()))
+                                for t, o in zip(grads, outs))
+        if not same:
+            raise ValueError(f"{op}: each out must have its gradient's shape and layout")
+    if written and len(set(optrs)) != len(optrs):
+        live = [p for p, c in zip(optrs, counts) if c]  # empty tensors have no place of their own
+        if len(set(live)) != len(live):
             raise ValueError(f"{op}: a tensor to be written is listed twice")
-    kinds = {}
-    for i, t in enumerate(grads):
-        key = (t.dtype, None if outs is None else outs[i].dtype)
-        kinds.setdefault(key, []).append(i)
-    if len(kinds) == 1:
-        return [_Group(grads, outs)]
-    return [_Group([grads[i] for i in idx], None if outs is None else [outs[i] for i in idx])
-            for idx in kinds.values()]
+    if len(dtypes) == 1 and len(odtypes) == 1:
+        kinds = {(*dtypes, *odtypes): None}
+    else:
+        kinds = {}
+        for i, t in enumerate(grads):
+            kinds.setdefault((t.dtype, t.dtype if outs is None else outs[i].dtype), []).append(i)
+    result = []
+    for (dtype, odtype), idx in kinds.items():
+        if odtype != dtype:
+            if odtype != torch.float32:
+                raise TypeError(f"{op}: an out has its gradient's type or float32, got {odtype} for {dtype}")
+            if not set(ptrs).isdisjoint(p for p in optrs if p):
+                raise ValueError(f"{op}: an out in a gradient's place must have its type")
+        pick = (lambda v: v) if idx is None else (lambda v: [v[i] for i in idx])
+        result.append(_Group(dtype, pick(ptrs), pick(counts), odtype, None if outs is None else pick(optrs)))
+    return result
 
 
-def _partials(groups, device, comm):
-    partials = torch.empty(PARTIALS, dtype=torch.float64, device=torch.device("cuda", device))
+def _sum_of_squares(like, groups, device, comm):
+    total = like.new_empty(1, dtype=torch.float64)
     for i, g in enumerate(groups):
-        run("bcclGradSquares", device, *g.inputs, g.n, g.code, int(i > 0), partials.data_ptr())
+        # A double per 32 KiB of gradients, two more per tensor for its ends (BCCL_GRAD_WORKSPACE).
+        size = 8 * (sum(g.counts) // 8192 + 2 * g.n + 1)
+        ws = like.new_empty(size, dtype=torch.uint8)
+        _squares(device, *g.inputs, g.n, g.code, i > 0, total.data_ptr(), ws.data_ptr(), size)
     if comm is not None and comm.world_size > 1:
-        comm.all_reduce(partials)
-    return partials
+        comm.all_reduce(total)
+    return total
 
 
 def _host(grads, comm):
@@ -125,9 +151,9 @@ def grad_norm(grads: Sequence[torch.Tensor], *, comm=None):
         return _host(grads, comm)
     device = grads[0].get_device()
     groups = _groups(op, grads, None, device, written=False)
-    partials = _partials(groups, device, comm)
-    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    run("bcclGradClip", device, None, None, None, 0, 0, 0, partials.data_ptr(), 0.0, 0.0, norm.data_ptr())
+    total = _sum_of_squares(grads[0], groups, device, comm)
+    norm = grads[0].new_empty((), dtype=torch.float32)
+    _clip(device, None, None, None, 0, 0, 0, total.data_ptr(), 0.0, 0.0, norm.data_ptr())
     return norm
 
 
@@ -152,10 +178,10 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, *, eps: float
         return norm
     device = grads[0].get_device()
     groups = _groups(op, grads, outs, device)
-    partials = _partials(groups, device, comm)
-    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    total = _sum_of_squares(grads[0], groups, device, comm)
+    norm = grads[0].new_empty((), dtype=torch.float32)
     for i, g in enumerate(groups):
         ptrs, counts = g.inputs
-        run("bcclGradClip", device, ptrs, g.outs.buffer_info()[0], counts, g.n, g.code, g.out_code, partials.data_ptr(),
-            max_norm, eps, norm.data_ptr() if i == 0 else None)
+        _clip(device, ptrs, g.outs.buffer_info()[0], counts, g.n, g.code, g.out_code, total.data_ptr(), max_norm, eps,
+              norm.data_ptr() if i == 0 else None)
     return norm

@@ -11,80 +11,86 @@ reference has no compute operators.
 """
 from __future__ import annotations
 
+import functools
 from typing import Tuple
 
 import torch
 
 from .. import _native
-from ._launch import float_code, like_or_f32, one_device, out_rows, rows, run
+from ._launch import Entry, float_code, like_or_f32, one_device, out_rows, ptr, rows
 
 _LAYER, _RMS = 0, 1
+_norm_forward, _norm_backward = Entry("bcclNormForward"), Entry("bcclNormBackward")
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace(kind: int, n: int, h: int, code: int) -> int:
+    return _native.lib().bcclNormBackwardWorkspace(kind, n, h, code)
 
 
 def _check(op, x, weight, bias):
-    code = float_code(op, "input", x)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"{op}: input needs a last dimension of at least 1, got shape {tuple(x.shape)}")
-    wcode = 0 if weight is None else like_or_f32(op, "weight", weight, x.dtype)
-    for what, p in (("weight", weight), ("bias", bias)):
-        if p is None:
-            continue
-        if weight is None or p.dtype != weight.dtype:
+    """(dtype code, weight's code, row length, contiguous weight and bias)"""
+    dtype = x.dtype
+    code = float_code(op, "input", dtype)
+    shape = x.shape
+    h = shape[-1] if shape else 0
+    if h < 1:
+        raise ValueError(f"{op}: input needs a last dimension of at least 1, got shape {tuple(shape)}")
+    if weight is None:
+        if bias is not None:
             raise TypeError(f"{op}: bias needs a weight of its own type")
-        if p.dim() != 1 or p.shape[0] != x.shape[-1]:
-            raise ValueError(f"{op}: {what} must have shape ({x.shape[-1]},), got {tuple(p.shape)}")
-    return code, wcode
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _dense(p):
-    return None if p is None else p.contiguous()
+        return code, 0, h, None, None
+    wcode = like_or_f32(op, "weight", weight.dtype, dtype)
+    if weight.shape != (h,):
+        raise ValueError(f"{op}: weight must have shape ({h},), got {tuple(weight.shape)}")
+    if bias is not None:
+        if bias.dtype is not weight.dtype:
+            raise TypeError(f"{op}: bias needs a weight of its own type")
+        if bias.shape != (h,):
+            raise ValueError(f"{op}: bias must have shape ({h},), got {tuple(bias.shape)}")
+        bias = bias.contiguous()
+    return code, wcode, h, weight.contiguous(), bias
 
 
 def _forward(kind, op, x, weight, bias, eps, out):
-    code, wcode = _check(op, x, weight, bias)
+    code, wcode, h, weight, bias = _check(op, x, weight, bias)
     if not eps >= 0.0:
         raise ValueError(f"{op}: eps must not be negative, got {eps}")
     device = one_device(op, x, weight, bias, out)
-    h, lead = x.shape[-1], x.shape[:-1]
-    xr, stride = rows(x)
-    weight, bias = _dense(weight), _dense(bias)
+    xr, stride = rows(x, h)
     if out is None:
-        out, ystride = torch.empty(x.shape, dtype=x.dtype, device=x.device), h
+        out, ystride = torch.empty_like(xr, memory_format=torch.contiguous_format), h
     else:
         ystride = out_rows(op, out, x.shape, x.dtype)
-    mean = torch.empty(lead, dtype=torch.float32, device=x.device) if kind == _LAYER else None
-    rstd = torch.empty(lead, dtype=torch.float32, device=x.device)
-    run("bcclNormForward", device, kind, xr.data_ptr(), stride, _ptr(weight), _ptr(bias), out.data_ptr(), ystride,
-        _ptr(mean), rstd.data_ptr(), x.numel() // h, h, eps, code, wcode)
+    lead = x.shape[:-1]
+    mean = x.new_empty(lead, dtype=torch.float32) if kind == _LAYER else None
+    rstd = x.new_empty(lead, dtype=torch.float32)
+    _norm_forward(device, kind, xr.data_ptr(), stride, ptr(weight), ptr(bias), out.data_ptr(), ystride, ptr(mean),
+                  rstd.data_ptr(), x.numel() // h, h, eps, code, wcode)
     return out, mean, rstd
 
 
 def _backward(kind, op, dy, x, mean, rstd, weight, weight_grad, bias_grad):
-    code, wcode = _check(op, x, weight, None)
-    if dy.dtype != x.dtype or dy.shape != x.shape:
-        raise ValueError(f"{op}: dy must be {x.dtype} of shape {tuple(x.shape)}, got {dy.dtype} {tuple(dy.shape)}")
+    code, wcode, h, weight, _ = _check(op, x, weight, None)
+    shape = x.shape
+    if dy.dtype is not x.dtype or dy.shape != shape:
+        raise ValueError(f"{op}: dy must be {x.dtype} of shape {tuple(shape)}, got {dy.dtype} {tuple(dy.shape)}")
     for what, t in (("mean", mean), ("rstd", rstd)):
-        if t is not None and (t.dtype != torch.float32 or t.shape != x.shape[:-1] or not t.is_contiguous()):
+        if t is not None and (t.dtype is not torch.float32 or t.shape != shape[:-1] or not t.is_contiguous()):
             raise ValueError(f"{op}: {what} must be the contiguous float32 tensor that the forward pass returned")
     device = one_device(op, x, dy, mean, rstd, weight)
-    h = x.shape[-1]
     n = x.numel() // h
-    xr, xstride = rows(x)
-    dyr, dystride = rows(dy)
-    weight = _dense(weight)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    xr, xstride = rows(x, h)
+    dyr, dystride = rows(dy, h)
+    dx = torch.empty_like(xr, memory_format=torch.contiguous_format)
     dw = torch.empty_like(weight) if weight is not None and weight_grad else None
     db = torch.empty_like(weight) if weight is not None and bias_grad else None
     ws, size = None, 0
     if dw is not None or db is not None:
-        size = _native.lib().bcclNormBackwardWorkspace(kind, n, h, code)
-        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
-    run("bcclNormBackward", device, kind, dyr.data_ptr(), dystride, xr.data_ptr(), xstride, _ptr(mean), rstd.data_ptr(),
-        _ptr(weight), dx.data_ptr(), h, _ptr(dw), _ptr(db), n, h, code, wcode, _ptr(ws), size)
+        size = _workspace(kind, n, h, code)
+        ws = x.new_empty(size, dtype=torch.uint8)
+    _norm_backward(device, kind, dyr.data_ptr(), dystride, xr.data_ptr(), xstride, ptr(mean), rstd.data_ptr(), ptr(weight),
+                   dx.data_ptr(), h, ptr(dw), ptr(db), n, h, code, wcode, ptr(ws), size)
     return dx, dw, db
 
 

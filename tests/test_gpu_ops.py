@@ -401,7 +401,9 @@ def test_expert_layouts_and_nothing():
     ids = some_ids(60, 6, "flat", 1).reshape(2, 30).t()  # not contiguous
     order = ex.sort_by_expert(ids, 6)
     same = ex.sort_by_expert(ids.contiguous(), 6)
-    assert all(torch.equal(a, b) for a, b in zip(order, same)) and order.num_experts == 6
+    assert order.num_experts == 6
+    for name in ("slots", "sources", "offsets"):
+        assert torch.equal(getattr(order, name), getattr(same, name))
     assert order.rank_counts(3).sum().item() == 60 and order.rank_counts(3).shape == (3,)
     wide = randn((30, 70), torch.bfloat16, 2)
     for view in (wide[:, 3:43], wide[:, 8:48], wide[:1, :40].expand(30, 40), wide.t()[:40].t()):
@@ -451,7 +453,7 @@ def check_clip(grads, max_norm, outs=None):
         exact = b.double() * coef
         check(o, exact, 40 * U * exact.abs())
         if outs is not None:
-            assert torch.equal(g.view(torch.uint8) if g.numel() else g, b.view(torch.uint8) if b.numel() else b)
+            assert torch.equal(g, b)
     return coef
 
 
@@ -462,9 +464,10 @@ def test_clip(dtype, sizes):
     for off in (0, 3):  # tensors at any alignment in one flat storage
         flat = randn(sum(sizes) + off, dtype, 1)
         grads = list(torch.split(flat[off:], sizes))
-        assert check_clip([g.clone() for g in grads], 0.4 * math.sqrt(sum(sizes))) < 1.0
+        bound = 0.4 * float(flat[off:].double().norm())
+        assert check_clip([g.clone() for g in grads], bound) < 1.0
         guard = flat[:off].clone()
-        check_clip(grads, 0.4 * math.sqrt(sum(sizes)))  # in place
+        check_clip(grads, bound)  # in place
         assert torch.equal(flat[:off], guard)
         flat = randn(sum(sizes) + off, dtype, 2)
         grads = list(torch.split(flat[off:], sizes))
@@ -554,7 +557,7 @@ def all_ops(seed):
         out += [embedding.embedding_forward(ids, x, 0.5), embedding.embedding_backward(dy, ids, 1500, 0.5)]
         order = ex.sort_by_expert(who, 9)
         rows = ex.dispatch_forward(x, order)
-        out += [*order, rows, ex.combine_forward(rows, order, cw), *ex.combine_backward(dy, rows, order, cw),
+        out += [order.slots, order.sources, order.offsets, rows, ex.combine_forward(rows, order, cw), *ex.combine_backward(dy, rows, order, cw),
                 ex.dispatch_backward(rows, order)]
         outs = [torch.empty_like(t) for t in (x, dy)]
         out += [gradients.clip_grad_norm([x, dy], 1.0, outs=outs), *outs]

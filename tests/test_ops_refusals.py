@@ -85,14 +85,12 @@ def test_experts_refuse():
         experts.sort_by_expert(ids[None], 4)
     with pytest.raises(ValueError, match="CUDA"):
         experts.sort_by_expert(ids, 4)
-    order = experts.ExpertOrder(ids, ids.reshape(-1), torch.zeros(5, dtype=torch.int32))
-    assert order.num_experts == 4
-    with pytest.raises(ValueError, match="split"):
-        order.rank_counts(3)
+    for parts in ((ids.long(), ids.reshape(-1), ids[:, 0]), (ids, ids.reshape(-1)[1:], ids[:, 0].contiguous()),
+                  (ids, ids.reshape(-1), ids.reshape(-1)[:1])):
+        with pytest.raises(ValueError, match="sort_by_expert"):
+            experts.ExpertOrder(*parts)
     with pytest.raises(ValueError, match="CUDA"):
-        experts.dispatch_forward(torch.zeros(5, 8), order)
-    with pytest.raises(ValueError, match="order"):
-        experts.dispatch_forward(torch.zeros(5, 8), order._replace(slots=ids.long()))
+        experts.ExpertOrder(ids, ids.reshape(-1), ids.reshape(-1)[:5])
 
 
 def test_clipping_refuses():
@@ -134,11 +132,16 @@ def test_the_c_interface_refuses():
     one = (ctypes.c_size_t * 1)(4)
     tensor = (ctypes.c_void_p * 1)(64)
     odd = (ctypes.c_void_p * 1)(66)
-    refused(lib.bcclGradSquares(tensor, one, -1, 0, 0, p(64), None), "tensor list")
-    refused(lib.bcclGradSquares(None, one, 1, 0, 0, p(64), None), "tensor list")
-    refused(lib.bcclGradSquares(tensor, one, 1, 1, 0, p(64), None), "dtype")
-    refused(lib.bcclGradSquares(odd, one, 1, 0, 0, p(64), None), "misaligned")
-    refused(lib.bcclGradSquares(tensor, one, 1, 0, 0, None, None), "partials")
+    def squares(t=tensor, n=1, d=0, total=64, ws=64, size=1 << 20):
+        return lib.bcclGradSquares(t, one, n, d, 0, p(total), p(ws), size, None)
+    refused(squares(n=-1), "tensor list")
+    refused(squares(t=None), "tensor list")
+    refused(squares(d=1), "dtype")
+    refused(squares(t=odd), "misaligned")
+    refused(squares(total=0), "sum")
+    refused(squares(total=68), "sum")
+    refused(squares(ws=0), "workspace")
+    refused(squares(size=8), "workspace")
     refused(lib.bcclGradClip(tensor, tensor, one, 1, 4, 0, p(64), 1.0, 0.0, None, None), "in place")
     refused(lib.bcclGradClip(tensor, tensor, one, 1, 0, 4, p(64), 1.0, 0.0, None, None), "dtypes")
     refused(lib.bcclGradClip(tensor, tensor, one, 1, 0, 0, p(64), -1.0, 0.0, None, None), "max_norm")
