@@ -197,11 +197,16 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const WindowArgs a, Bits
     if (row >= a.rows || __ldg(&a.sorted[end].x) != row) return;
     const long long begin = w * a.window;
     if (begin > 0 && __ldg(&a.sorted[begin - 1].x) == row) return;  // it began in an earlier window
-    // The last window that holds the token: the last whose first position has it.
-    long long lo = w + 1, hi = a.windows;
-    while (hi - lo > 1) {
-        const long long mid = (lo + hi) >> 1;
-        if (__ldg(&a.sorted[mid * a.window].x) == row) lo = mid; else hi = mid;
+    // The last window that holds the token, which is the last whose first position has it: mostly the
+    // next one, so search in growing steps.
+    long long lo = w + 1, step = 1;
+    while (lo + step < a.windows && __ldg(&a.sorted[(lo + step) * a.window].x) == row) {
+        lo += step;
+        step *= 2;
+    }
+    for (; step > 1; step /= 2) {
+        const long long mid = lo + step / 2;
+        if (mid < a.windows && __ldg(&a.sorted[mid * a.window].x) == row) lo = mid;
     }
     const long long c = (static_cast<long long>(blockIdx.y) * blockDim.x + threadIdx.x) * E;
     if (c >= a.h) return;

@@ -109,6 +109,123 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 512) norm_forward_kern
     }
 }
 
+__device__ __forceinline__ void copy16_async(void* smem, const void* global) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(smem))),
+                 "l"(global)
+                 : "memory");
+}
+
+// Parameters of a thread's columns in shared memory (its own place, so no barrier), read back as floats.
+template <int WD, int E>
+__device__ __forceinline__ void keep_params(Bits<WD>* smem, const void* params, long long c) {
+    float w[E];
+    load_f<WD, E>(static_cast<const Bits<WD>*>(params) + c, w);
+    store_f<WD, E>(smem + c, w);
+}
+template <int WD, int E>
+__device__ __forceinline__ void read_params(const Bits<WD>* smem, long long c, float (&w)[E]) {
+    constexpr int W = Vec<WD>::E;
+#pragma unroll
+    for (int i = 0; i < E / W; ++i) {
+        float t[W];
+        Vec<WD>::unpack(reinterpret_cast<const uint4*>(smem + c)[i], t);
+#pragma unroll
+        for (int e = 0; e < W; ++e) w[i * W + e] = t[e];
+    }
+}
+
+// Many rows of 16-byte accesses too long for a warp. Every thread copies its own columns of the next
+// STAGES - 1 rows into shared memory with cp.async and only reads what it copied itself, so the copies
+// need no barrier and stay in flight whatever the row at hand waits for; a row costs one barrier
+// per sum.
+template <int D, int WD, int NV, bool LAYER, int STAGES>
+__global__ void __launch_bounds__(512, NV <= 2 ? 2 : 1) norm_forward_ring_kernel(const NormForwardArgs a) {
+    constexpr int E = Vec<D>::E;
+    extern __shared__ uint4 ring[];  // [STAGES][NV][threads], then the parameters
+    __shared__ float buf[2][32];
+    const int tx = threadIdx.x, g = blockDim.x, warps = g >> 5;
+    const float inv_h = 1.0f / static_cast<float>(a.h);
+    const Bits<D>* x = static_cast<const Bits<D>*>(a.x);
+    Bits<WD>* w_smem = reinterpret_cast<Bits<WD>*>(ring + static_cast<size_t>(STAGES) * NV * g);
+    Bits<WD>* b_smem = w_smem + a.h;
+    auto issue = [&](long long row, int slot) {
+        if (row < a.rows) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const long long c = col_of<E>(v, tx, g);
+                if (c < a.h) copy16_async(ring + (static_cast<size_t>(slot) * NV + v) * g + tx, x + row * a.x_stride + c);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) issue(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        const long long c = col_of<E>(v, tx, g);
+        if (c >= a.h) continue;
+        if (a.w != nullptr) keep_params<WD, E>(w_smem, a.w, c);
+        if (LAYER && a.b != nullptr) keep_params<WD, E>(b_smem, a.b, c);
+    }
+    int slot = 0, parity = 0;
+    auto sum = [&](float v) {
+        const float s = block_sum(v, buf, parity, tx, warps);
+        parity ^= 1;
+        return s;
+    };
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        issue(row + static_cast<long long>(STAGES - 1) * gridDim.x, slot == 0 ? STAGES - 1 : slot - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        float f[NV][E], s = 0.0f, mean = 0.0f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            if (col_of<E>(v, tx, g) >= a.h) continue;
+            Vec<D>::unpack(ring[(static_cast<size_t>(slot) * NV + v) * g + tx], f[v]);
+#pragma unroll
+            for (int e = 0; e < E; ++e) s += LAYER ? f[v][e] : f[v][e] * f[v][e];
+        }
+        if constexpr (LAYER) {
+            mean = sum(s) * inv_h;
+            s = 0.0f;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                if (col_of<E>(v, tx, g) >= a.h) continue;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    f[v][e] -= mean;
+                    s = fmaf(f[v][e], f[v][e], s);
+                }
+            }
+        }
+        const float rstd = 1.0f / sqrtf(sum(s) * inv_h + a.eps);
+        if (tx == 0) {
+            if (LAYER) a.mean[row] = mean;
+            a.rstd[row] = rstd;
+        }
+        Bits<D>* y = static_cast<Bits<D>*>(a.y) + row * a.y_stride;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const long long c = col_of<E>(v, tx, g);
+            if (c >= a.h) continue;
+            float p[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) f[v][e] *= rstd;
+            if (a.w != nullptr) {
+                read_params<WD, E>(w_smem, c, p);
+#pragma unroll
+                for (int e = 0; e < E; ++e) f[v][e] *= p[e];
+            }
+            if (LAYER && a.b != nullptr) {
+                read_params<WD, E>(b_smem, c, p);
+#pragma unroll
+                for (int e = 0; e < E; ++e) f[v][e] += p[e];
+            }
+            store_f_cs<D, E>(y + c, f[v]);
+        }
+        slot = slot == STAGES - 1 ? 0 : slot + 1;
+    }
+}
+
 // Rows longer than a block's registers hold: three passes over the row, the later ones from L2.
 template <int D, int WD, int E, bool LAYER>
 __global__ void __launch_bounds__(1024) norm_forward_long_kernel(const NormForwardArgs a) {
@@ -274,12 +391,6 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 512) norm_backward_ker
 // itself, so the copies need no barrier and keep 2 blocks' rings of up to 112 KiB in flight per SM; a
 // row costs one barrier, for its sums. The second use of a row reads it from shared memory again
 // instead of holding it in registers.
-__device__ __forceinline__ void copy16_async(void* smem, const void* global) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(smem))),
-                 "l"(global)
-                 : "memory");
-}
-
 template <int D, int WD, int NV, bool LAYER, int STAGES>
 __global__ void __launch_bounds__(512, NV <= 2 ? 2 : 1) norm_backward_ring_kernel(const NormBackwardArgs a) {
     constexpr int E = Vec<D>::E;
@@ -310,11 +421,7 @@ __global__ void __launch_bounds__(512, NV <= 2 ? 2 : 1) norm_backward_ring_kerne
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         const long long c = col_of<E>(v, tx, g);
-        if (a.w != nullptr && c < a.h) {  // kept as they are, at the thread's own place
-            float w[E];
-            load_f<WD, E>(static_cast<const Bits<WD>*>(a.w) + c, w);
-            store_f<WD, E>(weights + c, w);
-        }
+        if (a.w != nullptr && c < a.h) keep_params<WD, E>(weights, a.w, c);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             dw[v][e] = 0.0f;
@@ -337,14 +444,7 @@ __global__ void __launch_bounds__(512, NV <= 2 ? 2 : 1) norm_backward_ring_kerne
 #pragma unroll
                 for (int e = 0; e < E; ++e) w[e] = 1.0f;
             } else {
-                constexpr int W = Vec<WD>::E;
-#pragma unroll
-                for (int i = 0; i < E / W; ++i) {
-                    float t[W];
-                    Vec<WD>::unpack(reinterpret_cast<const uint4*>(weights + col_of<E>(v, tx, g))[i], t);
-#pragma unroll
-                    for (int e = 0; e < W; ++e) w[i * W + e] = t[e];
-                }
+                read_params<WD, E>(weights, col_of<E>(v, tx, g), w);
             }
         };
         float2 s = make_float2(0.0f, 0.0f);
@@ -521,13 +621,18 @@ Shape forward_shape(long long h, int e) {
     }
     return {0, 0};
 }
+// Blocks of at most 512 threads, two on an SM, or one where a thread has four accesses.
+Shape ring_shape(long long h, int e) {
+    const long long n = ceil_div(h, e);
+    if (n <= 64 || n > 2048) return {0, 0};
+    return n <= 1024 ? Shape{2, round32(ceil_div(n, 2))} : Shape{4, round32(ceil_div(n, 4))};
+}
 Shape backward_shape(long long h, int e) {
     const long long n = ceil_div(h, e);
     if (e > 1) {
         for (int nv : {1, 2})
             if (n <= 32 * nv) return {nv, 32};
-        if (n <= 1024) return {2, round32(ceil_div(n, 2))};
-        if (n <= 2048) return {4, round32(ceil_div(n, 4))};
+        return ring_shape(h, e);
     } else {
         for (int nv : {4, 16})
             if (n <= 32 * nv) return {nv, 32};
@@ -563,8 +668,42 @@ cudaError_t forward(const NormForwardArgs& a, int threads, cudaStream_t s) {
     return cudaGetLastError();
 }
 
+// The deepest ring of 2 to 4 rows that leaves the SM room for `per_sm` blocks (228 KiB; a block takes
+// 1 KiB for the system and 512 bytes for its sums besides). Launches f(Int<stages>, bytes).
+template <typename F>
+cudaError_t with_ring(size_t row, size_t params, int per_sm, F&& f) {
+    const size_t room = std::min<size_t>(228 * 1024 / per_sm, 227 * 1024) - 1024 - 512;
+    if (params + 4 * row <= room) return f(Int<4>{}, params + 4 * row);
+    if (params + 3 * row <= room) return f(Int<3>{}, params + 3 * row);
+    return f(Int<2>{}, params + 2 * row);
+}
+
+template <int D, int WD, int NV, bool LAYER>
+cudaError_t forward_ring(const NormForwardArgs& a, int threads, cudaStream_t s) {
+    const int per_sm = std::min(8, (NV > 2 ? 512 : 1024) / threads);
+    const int grid = static_cast<int>(std::min<long long>(a.rows, static_cast<long long>(sm_count()) * per_sm));
+    const int vectors = (a.w != nullptr) + (a.b != nullptr);
+    return with_ring(static_cast<size_t>(NV) * threads * 16, static_cast<size_t>(vectors) * a.h * sizeof(Bits<WD>), per_sm,
+                     [&](auto S, size_t smem) {
+                         auto* kernel = &norm_forward_ring_kernel<D, WD, NV, LAYER, decltype(S)::value>;
+                         const cudaError_t e = cudaFuncSetAttribute(
+                             kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+                         if (e != cudaSuccess) return e;
+                         kernel<<<grid, threads, smem, s>>>(a);
+                         return cudaGetLastError();
+                     });
+}
+
 template <int D, int WD, int E, bool LAYER>
 cudaError_t forward_any(const NormForwardArgs& a, cudaStream_t s) {
+    if constexpr (E > 1) {
+        const Shape ring = ring_shape(a.h, E);
+        static const int mode = getenv("BCCL_X") ? atoi(getenv("BCCL_X")) : 0;
+        if (mode < 8 && ring.threads != 0 && a.rows > (mode ? 0 : 2ll * sm_count() * ((ring.nv > 2 ? 512 : 1024) / ring.threads))) {
+            if (ring.nv == 2) return forward_ring<D, WD, 2, LAYER>(a, ring.threads, s);
+            return forward_ring<D, WD, 4, LAYER>(a, ring.threads, s);
+        }
+    }
     const Shape sh = forward_shape(a.h, E);
     if constexpr (E > 1) {
         if (sh.nv == 1) return forward<D, WD, E, 1, LAYER>(a, sh.threads, s);
@@ -592,26 +731,18 @@ cudaError_t backward(const NormBackwardArgs& a, int threads, int grid, cudaStrea
     return cudaGetLastError();
 }
 
-template <int D, int WD, int NV, bool LAYER, int STAGES>
-cudaError_t backward_ring(const NormBackwardArgs& a, int threads, int grid, size_t smem, cudaStream_t s) {
-    auto* kernel = &norm_backward_ring_kernel<D, WD, NV, LAYER, STAGES>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(smem));
-    if (e != cudaSuccess) return e;
-    kernel<<<grid, threads, smem, s>>>(a);
-    return cudaGetLastError();
-}
-// The deepest ring of 2 to 4 rows that leaves the SM room for all the blocks it should hold (227 KiB,
-// 1 KiB of them per block for the system).
 template <int D, int WD, int NV, bool LAYER>
 cudaError_t backward_ring(const NormBackwardArgs& a, int threads, int grid, cudaStream_t s) {
-    const size_t row = static_cast<size_t>(2) * NV * threads * 16;
-    const size_t weights = a.w != nullptr ? static_cast<size_t>(a.h) * sizeof(Bits<WD>) : 0;
     const int per_sm = std::max(1, std::min(static_cast<int>(ceil_div(grid, sm_count())), (NV > 2 ? 512 : 1024) / threads));
-    const size_t room = static_cast<size_t>(227 * 1024) / per_sm - 2048;
-    if (weights + 4 * row <= room) return backward_ring<D, WD, NV, LAYER, 4>(a, threads, grid, weights + 4 * row, s);
-    if (weights + 3 * row <= room) return backward_ring<D, WD, NV, LAYER, 3>(a, threads, grid, weights + 3 * row, s);
-    return backward_ring<D, WD, NV, LAYER, 2>(a, threads, grid, weights + 2 * row, s);
+    return with_ring(static_cast<size_t>(2) * NV * threads * 16, a.w != nullptr ? a.h * sizeof(Bits<WD>) : 0, per_sm,
+                     [&](auto S, size_t smem) {
+                         auto* kernel = &norm_backward_ring_kernel<D, WD, NV, LAYER, decltype(S)::value>;
+                         const cudaError_t e = cudaFuncSetAttribute(
+                             kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+                         if (e != cudaSuccess) return e;
+                         kernel<<<grid, threads, smem, s>>>(a);
+                         return cudaGetLastError();
+                     });
 }
 
 // Rows of partial sums that the backward pass of this shape writes.

@@ -38,13 +38,24 @@ def cutlass_include() -> Path | None:
     return None
 
 
+def python_extension_flags() -> tuple[str, str] | None:
+    """Compile and link flags of the Python extension (csrc/python), or None where Python's or
+    PyTorch's headers are missing; the package then reads tensor lists in Python."""
+    py = Path(sysconfig.get_paths()["include"])
+    torch = _site_packages() / "torch"
+    if not (py / "Python.h").exists() or not (torch / "include" / "torch" / "csrc" / "autograd" / "python_variable.h").exists():
+        return None
+    return (f"-isystem {py} -isystem {torch / 'include'} -isystem {torch / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
+            f"-L{torch / 'lib'} -ltorch_python -ltorch_cpu -lc10")
+
+
 # Host sources whose inner loops must be vectorised (-O2's cost model leaves loops with a
 # run-time trip count scalar).
 VECTORIZED = {"host_reduce.cc"}
 
 
 def _sources() -> tuple[list[Path], list[Path]]:
-    cc = sorted(p for p in CSRC.rglob("*.cc") if not {"launcher", "examples"} & set(p.parts))
+    cc = sorted(p for p in CSRC.rglob("*.cc") if not {"launcher", "examples", "python"} & set(p.parts))
     cu = sorted(CSRC.rglob("*.cu"))
     return cc, cu
 
@@ -101,6 +112,15 @@ def _ninja_file() -> str:
         obj = BUILD / (str(src.relative_to(CSRC)).replace("/", "_") + ".o")
         lines.append(f"build {obj}: nvcc {src}")
         objs.append(obj)
+    ext = python_extension_flags()
+    if ext:
+        lines += ["rule pyext",
+                  f"  command = $cxx -MMD -MF $out.d -O2 -std=c++17 -fPIC -Wall -shared {ext[0]} $in -o $out.tmp {ext[1]} "
+                  "&& mv -f $out.tmp $out",
+                  "  depfile = $out.d",
+                  "  deps = gcc",
+                  "  description = PYEXT $out",
+                  f"build {LIBDIR / '_tensor_list.so'}: pyext {CSRC / 'python' / 'tensor_list.cc'}"]
     lines.append(f"build {LIBDIR / 'libbccl.so'}: link {' '.join(map(str, objs))}")
     launcher = CSRC / "launcher" / "bccl_run.cc"
     lobj = BUILD / "launcher_bccl_run.cc.o"

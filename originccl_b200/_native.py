@@ -145,3 +145,21 @@ def lib() -> ctypes.CDLL:
 def last_error() -> str:
     msg = lib().bcclGetLastError()
     return msg.decode() if msg else ""
+
+
+def tensor_list():
+    """The Python extension that reads lists of torch tensors (csrc/python/tensor_list.cc), or None where
+    it was not built (no PyTorch headers) or was built for another PyTorch."""
+    import importlib.machinery
+    import importlib.util
+    path = _LIB_PATH.parent / "_tensor_list.so"
+    if not path.exists():
+        return None
+    import torch  # noqa: F401  (its libraries hold the symbols)
+    loader = importlib.machinery.ExtensionFileLoader("_tensor_list", str(path))
+    try:
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_tensor_list", loader))
+        loader.exec_module(module)
+    except ImportError:
+        return None
+    return module

@@ -15,10 +15,11 @@ from __future__ import annotations
 
 from array import array
 from operator import attrgetter
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 
+from .. import _native
 from ._launch import FLOATS, Entry
 
 _squares, _clip = Entry("bcclGradSquares"), Entry("bcclGradClip")
@@ -36,26 +37,40 @@ def _dense(t) -> bool:
     return True
 
 
+def _apart_in_python(written, counts, size, read, read_counts, read_size) -> bool:
+    """No tensor written overlaps another one or any of the tensors read (arrays of 64-bit words)."""
+    ranges = [(p, p + n * size, True) for p, n in zip(array("Q", written), array("Q", counts)) if n]
+    ranges += [(p, p + n * read_size, False) for p, n in zip(array("Q", read), array("Q", read_counts)) if n]
+    any_end = written_end = 0
+    for start, end, w in sorted(ranges):
+        if start < (any_end if w else written_end):
+            return False
+        any_end = max(any_end, end)
+        written_end = max(written_end, end) if w else written_end
+    return True
+
+
 _T = torch.Tensor
 _dtype = attrgetter("dtype")
+_SIZES = {0: 4, 4: 2, 5: 2}  # of the type codes
+_lists = _native.tensor_list()
+_describe = _lists.describe if _lists else (lambda tensors: None)
+_apart = _lists.apart if _lists else _apart_in_python
 
 
-class _Group:
-    """Pointer and count arrays of the tensors of one type (and of their outputs)."""
-
-    def __init__(self, dtype, ptrs, counts, out_dtype=None, outs=None) -> None:
-        self.code, self.n = FLOATS[dtype], len(ptrs)
-        self.ptrs, self.counts = array("Q", ptrs), array("Q", counts)
-        self.outs, self.out_code = (self.ptrs, self.code) if outs is None else (array("Q", outs), FLOATS[out_dtype])
-
-    @property
-    def inputs(self):
-        return self.ptrs.buffer_info()[0], self.counts.buffer_info()[0]
+class _Group(NamedTuple):
+    """The tensors of one type: host arrays of their (and their outputs') pointers and element counts."""
+    n: int
+    code: int
+    ptrs: bytes
+    counts: bytes
+    total: int
+    out_code: int
+    outs: bytes
 
 
 def _check_list(op, tensors, device):
-    """Types, device and layout of a list; the lists may be long, so each property is read once per
-    tensor in a loop that runs in C. Returns the types and whether all are contiguous."""
+    """Checks types, device and layout of a list; returns the types and whether all are contiguous."""
     dtypes = set(map(_dtype, tensors))
     if not dtypes <= FLOATS.keys():
         raise TypeError(f"{op}: tensors must be float32, bfloat16 or float16, got {sorted(map(str, dtypes))}")
@@ -72,6 +87,20 @@ def _check_list(op, tensors, device):
 
 def _groups(op, grads, outs, device, written=True):
     """The tensors by type, checked."""
+    a = _describe(grads)
+    b = a if outs is None else _describe(outs)
+    if a is not None and b is not None and a[4] == b[4] == device and b[1] == a[1] and (b[3] == a[3] or b[3] == 0):
+        group = _Group(len(grads), a[3], a[0], a[1], a[2], b[3], b[0])
+        if written:
+            size = _SIZES[a[3]]
+            if outs is None or (b[0] == a[0] and b[3] == a[3]):
+                apart = _apart(a[0], a[1], size, b"", b"", 0)
+            else:
+                apart = _apart(b[0], a[1], _SIZES[b[3]], a[0], a[1], size)
+            if not apart:
+                raise ValueError(f"{op}: tensors to be written overlap")
+        return [group]
+    # Lists of mixed types or layouts, and whatever is to be refused.
     dtypes, plain = _check_list(op, grads, device)
     ptrs, counts = list(map(_T.data_ptr, grads)), list(map(_T.numel, grads))
     optrs, odtypes = ptrs, dtypes
@@ -85,10 +114,6 @@ def _groups(op, grads, outs, device, written=True):
                                 for t, o in zip(grads, outs))
         if not same:
             raise ValueError(f"{op}: each out must have its gradient's shape and layout")
-    if written and len(set(optrs)) != len(optrs):
-        live = [p for p, c in zip(optrs, counts) if c]  # empty tensors have no place of their own
-        if len(set(live)) != len(live):
-            raise ValueError(f"{op}: a tensor to be written is listed twice")
     if len(dtypes) == 1 and len(odtypes) == 1:
         kinds = {(*dtypes, *odtypes): None}
     else:
@@ -97,13 +122,21 @@ def _groups(op, grads, outs, device, written=True):
             kinds.setdefault((t.dtype, t.dtype if outs is None else outs[i].dtype), []).append(i)
     result = []
     for (dtype, odtype), idx in kinds.items():
-        if odtype != dtype:
-            if odtype != torch.float32:
-                raise TypeError(f"{op}: an out has its gradient's type or float32, got {odtype} for {dtype}")
-            if not set(ptrs).isdisjoint(p for p in optrs if p):
-                raise ValueError(f"{op}: an out in a gradient's place must have its type")
-        pick = (lambda v: v) if idx is None else (lambda v: [v[i] for i in idx])
-        result.append(_Group(dtype, pick(ptrs), pick(counts), odtype, None if outs is None else pick(optrs)))
+        if odtype != dtype and odtype != torch.float32:
+            raise TypeError(f"{op}: an out has its gradient's type or float32, got {odtype} for {dtype}")
+        idx = range(len(ptrs)) if idx is None else idx
+        pack = lambda v: array("Q", [v[i] for i in idx]).tobytes()  # noqa: E731
+        result.append(_Group(len(idx), FLOATS[dtype], pack(ptrs), pack(counts), sum(counts[i] for i in idx), FLOATS[odtype],
+                             pack(optrs)))
+    if written:  # in bytes, over all types at once
+        words = lambda v: array("Q", v).tobytes()  # noqa: E731
+        lists = [(words(ptrs), words(c * _SIZES[FLOATS[t.dtype]] for c, t in zip(counts, grads)), 1)]
+        if outs is not None:
+            lists.insert(0, (words(optrs), words(c * _SIZES[FLOATS[t.dtype]] for c, t in zip(counts, outs)), 1))
+        if len(lists) == 1 or lists[0] == lists[1]:
+            lists[1:] = [(b"", b"", 0)]
+        if not _apart(*lists[0], *lists[1]):
+            raise ValueError(f"{op}: tensors to be written overlap")
     return result
 
 
@@ -111,9 +144,9 @@ def _sum_of_squares(like, groups, device, comm):
     total = like.new_empty(1, dtype=torch.float64)
     for i, g in enumerate(groups):
         # A double per 32 KiB of gradients, two more per tensor for its ends (BCCL_GRAD_WORKSPACE).
-        size = 8 * (sum(g.counts) // 8192 + 2 * g.n + 1)
+        size = 8 * (g.total // 8192 + 2 * g.n + 1)
         ws = like.new_empty(size, dtype=torch.uint8)
-        _squares(device, *g.inputs, g.n, g.code, i > 0, total.data_ptr(), ws.data_ptr(), size)
+        _squares(device, g.ptrs, g.counts, g.n, g.code, i > 0, total.data_ptr(), ws.data_ptr(), size)
     if comm is not None and comm.world_size > 1:
         comm.all_reduce(total)
     return total
@@ -160,7 +193,7 @@ def grad_norm(grads: Sequence[torch.Tensor], *, comm=None):
 def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, *, eps: float = 1e-6,
                    outs: Optional[Sequence[torch.Tensor]] = None, comm=None):
     """Scales the gradients by ``min(1, max_norm / (norm + eps))`` in place, or into ``outs`` (same shapes; the
-    gradients' type or float32), and returns the norm from before."""
+    gradients' type or float32; memory of their own), and returns the norm from before."""
     op = "clip_grad_norm"
     grads, cuda = _list(op, grads)
     if not max_norm >= 0.0 or not eps >= 0.0:
@@ -181,7 +214,6 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, *, eps: float
     total = _sum_of_squares(grads[0], groups, device, comm)
     norm = grads[0].new_empty((), dtype=torch.float32)
     for i, g in enumerate(groups):
-        ptrs, counts = g.inputs
-        _clip(device, ptrs, g.outs.buffer_info()[0], counts, g.n, g.code, g.out_code, total.data_ptr(), max_norm, eps,
+        _clip(device, g.ptrs, g.outs, g.counts, g.n, g.code, g.out_code, total.data_ptr(), max_norm, eps,
               norm.data_ptr() if i == 0 else None)
     return norm
