@@ -6,7 +6,8 @@
 // writes each element to its place: equal digits keep their order, whatever the timing. Elements
 // between passes travel through global memory (L2); the barrier between passes is the hardware's
 // cluster barrier, so there is nothing to spin on. Bound by latency: a warp loads kBatch steps of
-// 32 keys at once, and stretches of one batch stay in registers for the second walk.
+// 32 keys at once, and stretches of one batch stay in registers for the second walk. Lanes with equal
+// digits are found by a vote per bit: match.any made 65536 keys of 7 bits take 23 us, votes @SORT@.
 #pragma once
 
 #include "kernels/ops_common.cuh"
@@ -35,6 +36,19 @@ struct KeySource {
     }
 };
 
+// The lanes of `valid` whose digit equals this lane's (which must be one of them).
+__device__ __forceinline__ unsigned int same_digit(unsigned int d, int bits, unsigned int valid) {
+    unsigned int same = valid;
+#pragma unroll
+    for (int b = 0; b < kSortMaxBits; ++b) {
+        if (b >= bits) break;
+        const bool set = (d >> b) & 1;
+        const unsigned int votes = __ballot_sync(0xffffffffu, set);
+        same &= set ? votes : ~votes;
+    }
+    return same;
+}
+
 // One pass over n elements by digit (key >> shift) & (2^bits - 1), blockDim.x == 1024. get(i) gives
 // {key, position}; put(place, key, position) stores it; totals(digit, first place) is called once
 // per digit by block 0. counters: shared memory, [warps][2^bits] and 2^bits + 32 words.
@@ -56,6 +70,7 @@ __device__ __forceinline__ void sort_pass(unsigned int* counters, long long n, i
     for (int i = threadIdx.x; i < kSortWarps * nbins / 2; i += blockDim.x)
         reinterpret_cast<uint2*>(counters)[i] = make_uint2(0, 0);
     uint2 held[kBatch];
+    unsigned int equal[kBatch];
     auto load = [&](long long i0) {
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
@@ -72,9 +87,9 @@ __device__ __forceinline__ void sort_pass(unsigned int* counters, long long n, i
             const long long base = i0 + b * 32;
             if (base >= hi) break;
             const bool in = base + lane < hi;
-            const unsigned int d = in ? (held[b].x >> shift) & mask : nbins;
-            const unsigned int same = __match_any_sync(0xffffffffu, d);
-            if (in && (same & lower) == 0) mine[d] += __popc(same);
+            const unsigned int d = (held[b].x >> shift) & mask;
+            equal[b] = same_digit(d, bits, __ballot_sync(0xffffffffu, in));
+            if (in && (equal[b] & lower) == 0) mine[d] += __popc(equal[b]);
             __syncwarp();
         }
     }
@@ -125,19 +140,20 @@ __device__ __forceinline__ void sort_pass(unsigned int* counters, long long n, i
     }
     __syncthreads();
     for (long long i0 = lo; i0 < hi; i0 += kBatch * 32) {
-        if (per > kBatch * 32) load(i0);
+        const bool again = per > kBatch * 32;
+        if (again) load(i0);
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
             const long long base = i0 + b * 32;
             if (base >= hi) break;
             const bool in = base + lane < hi;
-            const unsigned int dg = in ? (held[b].x >> shift) & mask : nbins;
-            const unsigned int same = __match_any_sync(0xffffffffu, dg);
-            const unsigned int at = in ? mine[dg] : 0;
+            const unsigned int dg = (held[b].x >> shift) & mask;
+            if (again) equal[b] = same_digit(dg, bits, __ballot_sync(0xffffffffu, in));
+            const unsigned int at = mine[dg];
             __syncwarp();
-            if (in && (same & lower) == 0) mine[dg] = at + __popc(same);
+            if (in && (equal[b] & lower) == 0) mine[dg] = at + __popc(equal[b]);
             __syncwarp();
-            if (in) put(at + __popc(same & lower), held[b].x, held[b].y);
+            if (in) put(at + __popc(equal[b] & lower), held[b].x, held[b].y);
         }
     }
     // The next pass reads what all blocks wrote; and no block may leave, or reuse its totals,

@@ -14,6 +14,7 @@
 #include "kernels/ops_common.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace bccl {
 namespace ops {
@@ -86,7 +87,7 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 512) norm_forward_kern
                 }
             }
         }
-        const float rstd = 1.0f / sqrtf(sum(s) * inv_h + a.eps);
+        const float rstd = inv_sqrt(sum(s) * inv_h + a.eps);
         if (tx == 0) {
             if (LAYER) a.mean[row] = mean;
             a.rstd[row] = rstd;
@@ -115,113 +116,128 @@ __device__ __forceinline__ void copy16_async(void* smem, const void* global) {
                  : "memory");
 }
 
-// Parameters of a thread's columns in shared memory (its own place, so no barrier), read back as floats.
+// The parameters of E columns in shared memory (the thread's own place, so no barrier), and back.
 template <int WD, int E>
-__device__ __forceinline__ void keep_params(Bits<WD>* smem, const void* params, long long c) {
-    float w[E];
-    load_f<WD, E>(static_cast<const Bits<WD>*>(params) + c, w);
-    store_f<WD, E>(smem + c, w);
+__device__ __forceinline__ void keep_params(Bits<WD>* smem, const void* params, int c) {
+#pragma unroll
+    for (int i = 0; i < E / Vec<WD>::E; ++i)
+        reinterpret_cast<uint4*>(smem + c)[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const Bits<WD>*>(params) + c) + i);
 }
 template <int WD, int E>
-__device__ __forceinline__ void read_params(const Bits<WD>* smem, long long c, float (&w)[E]) {
+__device__ __forceinline__ void read_params(const Bits<WD>* smem, int c, F2 (&w)[E / 2]) {
     constexpr int W = Vec<WD>::E;
 #pragma unroll
     for (int i = 0; i < E / W; ++i) {
-        float t[W];
-        Vec<WD>::unpack(reinterpret_cast<const uint4*>(smem + c)[i], t);
+        F2 t[W / 2];
+        unpack2<WD>(reinterpret_cast<const uint4*>(smem + c)[i], t);
 #pragma unroll
-        for (int e = 0; e < W; ++e) w[i * W + e] = t[e];
+        for (int e = 0; e < W / 2; ++e) w[i * (W / 2) + e] = t[e];
     }
 }
 
-// Many rows of 16-byte accesses too long for a warp. Every thread copies its own columns of the next
-// STAGES - 1 rows into shared memory with cp.async and only reads what it copied itself, so the copies
-// need no barrier and stay in flight whatever the row at hand waits for; a row costs one barrier
-// per sum.
-template <int D, int WD, int NV, bool LAYER, int STAGES>
-__global__ void __launch_bounds__(512, NV <= 2 ? 2 : 1) norm_forward_ring_kernel(const NormForwardArgs a) {
-    constexpr int E = Vec<D>::E;
+// Many rows of 16-byte accesses, too long for a warp. Blocks are persistent. Every thread copies its
+// own columns of the next STAGES - 1 rows into shared memory with cp.async and only reads what it
+// copied itself, so the copies need no barrier and stay in flight whatever the row at hand waits for;
+// a row costs one barrier per sum. A thread takes two accesses and 64 registers, so that an SM holds
+// 1024 threads (of rows too long for that, four and 128): measured on the backward pass of 8192 x 8192
+// bf16, one access per thread took 132 us, two 97, four 96 to 102; f32 rows of 4096 77, 77 and 91.
+template <int D> constexpr int ring_max_threads() { return D == kF32 ? 1024 : 512; }
+
+template <int D, int WD, bool LAYER, int STAGES, int NV>
+__global__ void __launch_bounds__(ring_max_threads<D>(), NV == 2 && D != kF32 ? 2 : 1) norm_forward_ring_kernel(const NormForwardArgs a) {
+    constexpr int E = Vec<D>::E, P = E / 2;
     extern __shared__ uint4 ring[];  // [STAGES][NV][threads], then the parameters
     __shared__ float buf[2][32];
-    const int tx = threadIdx.x, g = blockDim.x, warps = g >> 5;
-    const float inv_h = 1.0f / static_cast<float>(a.h);
-    const Bits<D>* x = static_cast<const Bits<D>*>(a.x);
-    Bits<WD>* w_smem = reinterpret_cast<Bits<WD>*>(ring + static_cast<size_t>(STAGES) * NV * g);
-    Bits<WD>* b_smem = w_smem + a.h;
-    auto issue = [&](long long row, int slot) {
-        if (row < a.rows) {
+    const int tx = threadIdx.x, g = blockDim.x, warps = g >> 5, h = static_cast<int>(a.h);
+    const float inv_h = 1.0f / static_cast<float>(h);
+    const int c0 = tx * E, dc = g * E;  // columns of access v: c0 + v * dc
+    Bits<WD>* w_smem = reinterpret_cast<Bits<WD>*>(ring + STAGES * NV * g);
+    Bits<WD>* b_smem = w_smem + h;
+    const long long x_step = static_cast<long long>(gridDim.x) * a.x_stride, y_step = static_cast<long long>(gridDim.x) * a.y_stride;
+    const Bits<D>* x = static_cast<const Bits<D>*>(a.x) + blockIdx.x * a.x_stride + c0;  // of the next row to copy
+    Bits<D>* y = static_cast<Bits<D>*>(a.y) + blockIdx.x * a.y_stride + c0;
+    int left = static_cast<int>((a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x);  // rows to copy
+    int todo = left;
+    auto issue = [&](int slot) {
+        if (left > 0) {
 #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                const long long c = col_of<E>(v, tx, g);
-                if (c < a.h) copy16_async(ring + (static_cast<size_t>(slot) * NV + v) * g + tx, x + row * a.x_stride + c);
-            }
+            for (int v = 0; v < NV; ++v)
+                if (c0 + v * dc < h) copy16_async(ring + (slot * NV + v) * g + tx, x + v * dc);
+            x += x_step;
+            --left;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) issue(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
+    for (int s = 0; s < STAGES - 1; ++s) issue(s);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-        const long long c = col_of<E>(v, tx, g);
-        if (c >= a.h) continue;
+        const int c = c0 + v * dc;
+        if (c >= h) continue;
         if (a.w != nullptr) keep_params<WD, E>(w_smem, a.w, c);
         if (LAYER && a.b != nullptr) keep_params<WD, E>(b_smem, a.b, c);
     }
     int slot = 0, parity = 0;
-    auto sum = [&](float v) {
-        const float s = block_sum(v, buf, parity, tx, warps);
+    auto sum = [&](F2 v) {
+        const float2 t = split(v);
+        const float s = block_sum(t.x + t.y, buf, parity, tx, warps);
         parity ^= 1;
         return s;
     };
-    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        issue(row + static_cast<long long>(STAGES - 1) * gridDim.x, slot == 0 ? STAGES - 1 : slot - 1);
+    for (long long row = blockIdx.x; todo > 0; --todo, row += gridDim.x) {
+        issue(slot == 0 ? STAGES - 1 : slot - 1);
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-        float f[NV][E], s = 0.0f, mean = 0.0f;
+        F2 f[NV][P], s = f2(0.0f, 0.0f);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            if (col_of<E>(v, tx, g) >= a.h) continue;
-            Vec<D>::unpack(ring[(static_cast<size_t>(slot) * NV + v) * g + tx], f[v]);
+            if (c0 + v * dc >= h) continue;
+            unpack2<D>(ring[(slot * NV + v) * g + tx], f[v]);
 #pragma unroll
-            for (int e = 0; e < E; ++e) s += LAYER ? f[v][e] : f[v][e] * f[v][e];
+            for (int e = 0; e < P; ++e) s = LAYER ? add2(f[v][e], s) : fma2(f[v][e], f[v][e], s);
         }
+        float mean = 0.0f;
         if constexpr (LAYER) {
             mean = sum(s) * inv_h;
-            s = 0.0f;
+            const F2 minus = f2(-mean, -mean);
+            s = f2(0.0f, 0.0f);
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
-                if (col_of<E>(v, tx, g) >= a.h) continue;
+                if (c0 + v * dc >= h) continue;
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    f[v][e] -= mean;
-                    s = fmaf(f[v][e], f[v][e], s);
+                for (int e = 0; e < P; ++e) {
+                    f[v][e] = add2(f[v][e], minus);
+                    s = fma2(f[v][e], f[v][e], s);
                 }
             }
         }
-        const float rstd = 1.0f / sqrtf(sum(s) * inv_h + a.eps);
+        const float rstd = inv_sqrt(sum(s) * inv_h + a.eps);
         if (tx == 0) {
             if (LAYER) a.mean[row] = mean;
             a.rstd[row] = rstd;
         }
-        Bits<D>* y = static_cast<Bits<D>*>(a.y) + row * a.y_stride;
+        const F2 scale = f2(rstd, rstd);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const long long c = col_of<E>(v, tx, g);
-            if (c >= a.h) continue;
-            float p[E];
+            const int c = c0 + v * dc;
+            if (c >= h) continue;
+            F2 w[P];
 #pragma unroll
-            for (int e = 0; e < E; ++e) f[v][e] *= rstd;
+            for (int e = 0; e < P; ++e) f[v][e] = mul2(f[v][e], scale);
             if (a.w != nullptr) {
-                read_params<WD, E>(w_smem, c, p);
+                read_params<WD, E>(w_smem, c, w);
+                if (LAYER && a.b != nullptr) {
+                    F2 b[P];
+                    read_params<WD, E>(b_smem, c, b);
 #pragma unroll
-                for (int e = 0; e < E; ++e) f[v][e] *= p[e];
-            }
-            if (LAYER && a.b != nullptr) {
-                read_params<WD, E>(b_smem, c, p);
+                    for (int e = 0; e < P; ++e) f[v][e] = fma2(f[v][e], w[e], b[e]);
+                } else {
 #pragma unroll
-                for (int e = 0; e < E; ++e) f[v][e] += p[e];
+                    for (int e = 0; e < P; ++e) f[v][e] = mul2(f[v][e], w[e]);
+                }
             }
-            store_f_cs<D, E>(y + c, f[v]);
+            __stcs(reinterpret_cast<uint4*>(y + v * dc), pack2<D>(f[v]));
         }
+        y += y_step;
         slot = slot == STAGES - 1 ? 0 : slot + 1;
     }
 }
@@ -254,7 +270,7 @@ __global__ void __launch_bounds__(1024) norm_forward_long_kernel(const NormForwa
 #pragma unroll
             for (int e = 0; e < E; ++e) s = fmaf(f[e] - mean, f[e] - mean, s);
         }
-        const float rstd = 1.0f / sqrtf(block_sum(s, buf, 1, tx, blockDim.x >> 5) * inv_h + a.eps);
+        const float rstd = inv_sqrt(block_sum(s, buf, 1, tx, blockDim.x >> 5) * inv_h + a.eps);
         __syncthreads();  // RMS norm sums once per row: its buffer is free only now
         if (tx == 0) {
             if (LAYER) a.mean[row] = mean;
@@ -386,108 +402,143 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 512) norm_backward_ker
     }
 }
 
-// Rows of 16-byte accesses too long for a warp. Every thread copies its own columns of the next
-// STAGES - 1 rows of x and dy into shared memory with cp.async, and only reads what it copied
-// itself, so the copies need no barrier and keep 2 blocks' rings of up to 112 KiB in flight per SM; a
-// row costs one barrier, for its sums. The second use of a row reads it from shared memory again
-// instead of holding it in registers.
-template <int D, int WD, int NV, bool LAYER, int STAGES>
-__global__ void __launch_bounds__(512, NV <= 2 ? 2 : 1) norm_backward_ring_kernel(const NormBackwardArgs a) {
-    constexpr int E = Vec<D>::E;
-    extern __shared__ uint4 ring[];  // [STAGES][x, dy][NV][threads], then the weights' accesses
-    __shared__ float2 buf[2][32];
-    const int tx = threadIdx.x, g = blockDim.x, warps = g >> 5;
-    const float inv_h = 1.0f / static_cast<float>(a.h);
-    const Bits<D>* x = static_cast<const Bits<D>*>(a.x);
-    const Bits<D>* dy = static_cast<const Bits<D>*>(a.dy);
-    Bits<WD>* weights = reinterpret_cast<Bits<WD>*>(ring + static_cast<size_t>(STAGES) * 2 * NV * g);
-    auto issue = [&](long long row, int slot) {
-        if (row < a.rows) {
-            uint4* to = ring + static_cast<size_t>(slot) * 2 * NV * g + tx;
+// As norm_forward_ring_kernel, with x and dy in the ring. With g = dy * w:
+//   sums g and g * (x - mean);  dx = rstd * (g - m1) - (x - mean) * (rstd^2 * m2),  m2 = mean(g (x - mean)) * rstd
+// The second use of a row reads it from shared memory again; RMS norm, which has registers left where
+// layer norm adds up db, keeps g (8192 x 8192 bf16: 81 us, 86 without; floor 61). Pairs of floats share an
+// instruction: issuing them fills 70% of the slots, the rest waits for the barrier and shared memory.
+template <int D, int WD, bool LAYER, int STAGES, int NV>
+__global__ void __launch_bounds__(ring_max_threads<D>(), NV == 2 && D != kF32 ? 2 : 1) norm_backward_ring_kernel(const NormBackwardArgs a) {
+    constexpr int E = Vec<D>::E, P = E / 2;
+    using Sum = typename std::conditional<LAYER, float2, float>::type;
+    extern __shared__ uint4 ring[];  // [STAGES][x, dy][NV][threads], then the weights
+    __shared__ Sum buf[2][32];
+    const int tx = threadIdx.x, g = blockDim.x, warps = g >> 5, h = static_cast<int>(a.h);
+    const float inv_h = 1.0f / static_cast<float>(h);
+    const int c0 = tx * E, dc = g * E;
+    Bits<WD>* w_smem = reinterpret_cast<Bits<WD>*>(ring + STAGES * 2 * NV * g);
+    const Bits<D>* x = static_cast<const Bits<D>*>(a.x) + blockIdx.x * a.x_stride + c0;  // of the next row to copy
+    const Bits<D>* dy = static_cast<const Bits<D>*>(a.dy) + blockIdx.x * a.dy_stride + c0;
+    Bits<D>* dx = static_cast<Bits<D>*>(a.dx) + blockIdx.x * a.dx_stride + c0;
+    int left = static_cast<int>((a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x);  // rows to copy
+    int todo = left;
+    auto issue = [&](int slot) {
+        if (left > 0) {
+            uint4* to = ring + slot * 2 * NV * g + tx;
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
-                const long long c = col_of<E>(v, tx, g);
-                if (c < a.h) {
-                    copy16_async(to + v * g, x + row * a.x_stride + c);
-                    copy16_async(to + (NV + v) * g, dy + row * a.dy_stride + c);
+                if (c0 + v * dc < h) {
+                    copy16_async(to + v * g, x + v * dc);
+                    copy16_async(to + (NV + v) * g, dy + v * dc);
                 }
             }
+            x += gridDim.x * a.x_stride;
+            dy += gridDim.x * a.dy_stride;
+            --left;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) issue(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
-    float dw[NV][E], db[LAYER ? NV : 1][E];
+    for (int s = 0; s < STAGES - 1; ++s) issue(s);
+    const F2 zero = f2(0.0f, 0.0f);
+    F2 dw[NV][P], db[LAYER ? NV : 1][P];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-        const long long c = col_of<E>(v, tx, g);
-        if (a.w != nullptr && c < a.h) keep_params<WD, E>(weights, a.w, c);
+        const int c = c0 + v * dc;
+        if (a.w != nullptr && c < h) keep_params<WD, E>(w_smem, a.w, c);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            dw[v][e] = 0.0f;
-            if constexpr (LAYER) db[v][e] = 0.0f;
+        for (int e = 0; e < P; ++e) {
+            dw[v][e] = zero;
+            if constexpr (LAYER) db[v][e] = zero;
         }
     }
     int slot = 0, parity = 0;
-    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        issue(row + static_cast<long long>(STAGES - 1) * gridDim.x, slot == 0 ? STAGES - 1 : slot - 1);
-        const float mean = LAYER ? __ldg(a.mean + row) : 0.0f;
-        const float rstd = __ldg(a.rstd + row);
+    float next_mean = LAYER ? __ldg(a.mean + blockIdx.x) : 0.0f, next_rstd = __ldg(a.rstd + blockIdx.x);
+    for (long long row = blockIdx.x; todo > 0; --todo) {
+        issue(slot == 0 ? STAGES - 1 : slot - 1);
+        const float mean = next_mean, rstd = next_rstd;
+        row += gridDim.x;
+        if (todo > 1) {  // a row ahead, like the row itself
+            if (LAYER) next_mean = __ldg(a.mean + row);
+            next_rstd = __ldg(a.rstd + row);
+        }
+        const F2 scale = f2(rstd, rstd), minus = f2(-mean, -mean);
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-        const uint4* from = ring + static_cast<size_t>(slot) * 2 * NV * g + tx;
-        auto load = [&](int v, float (&xh)[E], float (&gr)[E], float (&w)[E]) {
-            Vec<D>::unpack(from[v * g], xh);
-            Vec<D>::unpack(from[(NV + v) * g], gr);
-#pragma unroll
-            for (int e = 0; e < E; ++e) xh[e] = (xh[e] - mean) * rstd;
-            if (a.w == nullptr) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) w[e] = 1.0f;
-            } else {
-                read_params<WD, E>(weights, col_of<E>(v, tx, g), w);
-            }
-        };
-        float2 s = make_float2(0.0f, 0.0f);
+        const uint4* from = ring + slot * 2 * NV * g + tx;
+        F2 s1 = zero, s2 = zero, gw[LAYER ? 1 : NV][P];
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            if (col_of<E>(v, tx, g) >= a.h) continue;
-            float xh[E], gr[E], w[E];
-            load(v, xh, gr, w);
+            if (c0 + v * dc >= h) continue;
+            F2 xc[P], gr[P], w[P];
+            unpack2<D>(from[v * g], xc);
+            unpack2<D>(from[(NV + v) * g], gr);
+            if (a.w != nullptr) read_params<WD, E>(w_smem, c0 + v * dc, w);
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                dw[v][e] = fmaf(gr[e], xh[e], dw[v][e]);
-                if constexpr (LAYER) db[v][e] += gr[e];
-                const float gw = gr[e] * w[e];
-                if (LAYER) s.x += gw;
-                s.y = fmaf(gw, xh[e], s.y);
+            for (int e = 0; e < P; ++e) {
+                if (LAYER) xc[e] = add2(xc[e], minus);
+                dw[v][e] = fma2(gr[e], mul2(xc[e], scale), dw[v][e]);
+                if constexpr (LAYER) db[v][e] = add2(gr[e], db[v][e]);
+                if (a.w != nullptr) gr[e] = mul2(gr[e], w[e]);
+                if (LAYER) s1 = add2(gr[e], s1);
+                else gw[v][e] = gr[e];
+                s2 = fma2(gr[e], xc[e], s2);
             }
         }
-        s = block_sum(s, buf, parity, tx, warps);
+        float m1 = 0.0f, m2;
+        const float2 t2 = split(s2);
+        if constexpr (LAYER) {
+            const float2 t1 = split(s1);
+            const float2 t = block_sum(make_float2(t1.x + t1.y, t2.x + t2.y), buf, parity, tx, warps);
+            m1 = t.x * inv_h;
+            m2 = t.y * inv_h * rstd;
+        } else {
+            m2 = block_sum(t2.x + t2.y, buf, parity, tx, warps) * inv_h * rstd;
+        }
         parity ^= 1;
-        const float m1 = LAYER ? s.x * inv_h : 0.0f, m2 = s.y * inv_h;
-        Bits<D>* dx = static_cast<Bits<D>*>(a.dx) + row * a.dx_stride;
+        const float k1 = -m1 * rstd, k2 = -m2 * rstd * rstd;
+        const F2 c1 = f2(k1, k1), c2 = f2(k2, k2);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const long long c = col_of<E>(v, tx, g);
-            if (c >= a.h) continue;
-            float xh[E], gr[E], w[E];
-            load(v, xh, gr, w);
+            if (c0 + v * dc >= h) continue;
+            F2 xc[P], gr[P], w[P];
+            unpack2<D>(from[v * g], xc);
+            if constexpr (LAYER) {
+                unpack2<D>(from[(NV + v) * g], gr);
+                if (a.w != nullptr) read_params<WD, E>(w_smem, c0 + v * dc, w);
+            }
 #pragma unroll
-            for (int e = 0; e < E; ++e) gr[e] = rstd * (gr[e] * w[e] - m1 - xh[e] * m2);
-            store_f_cs<D, E>(dx + c, gr);
+            for (int e = 0; e < P; ++e) {
+                if constexpr (LAYER) {
+                    xc[e] = add2(xc[e], minus);
+                    if (a.w != nullptr) gr[e] = mul2(gr[e], w[e]);
+                    gr[e] = fma2(gr[e], scale, c1);
+                } else {
+                    gr[e] = mul2(gw[v][e], scale);
+                }
+                gr[e] = fma2(xc[e], c2, gr[e]);
+            }
+            __stcs(reinterpret_cast<uint4*>(dx + v * dc), pack2<D>(gr));
         }
+        dx += gridDim.x * a.dx_stride;
         slot = slot == STAGES - 1 ? 0 : slot + 1;
     }
     if (a.partials == nullptr) return;
     float* pw = a.partials + blockIdx.x * a.h;
     float* pb = a.partials + (static_cast<long long>(gridDim.x) + blockIdx.x) * a.h;
+    auto put = [&](float* to, const F2 (&sum)[P]) {
+#pragma unroll
+        for (int e = 0; e < P; e += 2) {
+            const float2 lo = split(sum[e]), hi = split(sum[e + 1]);
+            reinterpret_cast<float4*>(to)[e / 2] = make_float4(lo.x, lo.y, hi.x, hi.y);
+        }
+    };
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-        const long long c = col_of<E>(v, tx, g);
-        if (c >= a.h) continue;
-        if (a.dw != nullptr) store_f<kF32, E>(reinterpret_cast<Bits<kF32>*>(pw + c), dw[v]);
+        const int c = c0 + v * dc;
+        if (c >= h) continue;
+        if (a.dw != nullptr) put(pw + c, dw[v]);
         if constexpr (LAYER) {
-            if (a.db != nullptr) store_f<kF32, E>(reinterpret_cast<Bits<kF32>*>(pb + c), db[v]);
+            if (a.db != nullptr) put(pb + c, db[v]);
         }
     }
 }
@@ -617,39 +668,40 @@ Shape forward_shape(long long h, int e) {
     } else {
         for (int nv : {4, 16})
             if (n <= 32 * nv) return {nv, 32};
+        if (n <= 2048) return {4, round32(ceil_div(n, 4))};
         if (n <= 8192) return {16, round32(ceil_div(n, 16))};
     }
     return {0, 0};
 }
-// Blocks of at most 512 threads, two on an SM, or one where a thread has four accesses.
-Shape ring_shape(long long h, int e) {
+// Accesses per thread of the ring kernels: 0 where a row is short enough for a warp's registers, or
+// so long that two rows of x and dy and the weights do not fit in shared memory.
+int ring_accesses(long long h, int e) {
     const long long n = ceil_div(h, e);
-    if (n <= 64 || n > 2048) return {0, 0};
-    return n <= 1024 ? Shape{2, round32(ceil_div(n, 2))} : Shape{4, round32(ceil_div(n, 4))};
+    const int most = e == 4 ? 1024 : 512;
+    if (n <= 64) return 0;
+    return n <= 2 * most ? 2 : n <= 4 * most && e != 4 ? 4 : 0;
 }
+int ring_threads(long long h, int e, int nv) { return round32(ceil_div(h, e * nv)); }
+int ring_blocks(int threads, int nv) { return std::min(16, std::max(1, (nv == 2 ? 1024 : 512) / threads)); }
 Shape backward_shape(long long h, int e) {
     const long long n = ceil_div(h, e);
     if (e > 1) {
         for (int nv : {1, 2})
             if (n <= 32 * nv) return {nv, 32};
-        return ring_shape(h, e);
     } else {
         for (int nv : {4, 16})
             if (n <= 32 * nv) return {nv, 32};
+        if (n <= 2048) return {4, round32(ceil_div(n, 4))};
         if (n <= 4096) return {8, round32(ceil_div(n, 8))};
         if (n <= 8192) return {16, round32(ceil_div(n, 16))};
     }
     return {0, 0};
 }
 
-// Backward blocks that are resident at once: 1024 threads per SM at 64 registers (512 where a
-// thread holds 4 accesses), but 8 rows each where that still fills the SMs, since each block costs
-// a row of partial sums.
-int row_blocks(long long rows, int threads, int nv, int e) {
-    const bool warp = threads == 32;
-    const int block = warp ? 32 * kWarpRows : threads;
-    const int per_sm = std::max(1, std::min(8, (e > 1 && nv > 2 ? 512 : 1024) / block));
-    const long long work = warp ? ceil_div(rows, kWarpRows) : rows;
+// Backward blocks: what is resident at once, but 8 rows each where that still fills the SMs, since
+// each block costs a row of partial sums.
+int row_blocks(long long rows, int rows_per_block, int per_sm) {
+    const long long work = ceil_div(rows, rows_per_block);
     return static_cast<int>(std::min(std::min(work, static_cast<long long>(sm_count()) * per_sm),
                                      std::max<long long>(sm_count(), ceil_div(work, 8))));
 }
@@ -660,7 +712,7 @@ template <int D, int WD, int E, int NV, bool LAYER>
 cudaError_t forward(const NormForwardArgs& a, int threads, cudaStream_t s) {
     // A row per block (or warp) and no persistent grid: with all SMs' blocks resident the rows in
     // flight hide each other's latency.
-    const int grid = static_cast<int>(std::min<long long>(threads == 32 ? ceil_div(a.rows, kWarpRows) : a.rows, 1 << 20));
+    const int grid = static_cast<int>(std::min<long long>(threads == 32 ? ceil_div(a.rows, kWarpRows) : a.rows, E == 1 && threads != 32 ? sm_count() * std::max(1, 2048 / threads) : 1 << 20));
     if (threads == 32)
         norm_forward_kernel<D, WD, E, NV, LAYER, true><<<grid, dim3(32, kWarpRows), 0, s>>>(a);
     else
@@ -678,14 +730,14 @@ cudaError_t with_ring(size_t row, size_t params, int per_sm, F&& f) {
     return f(Int<2>{}, params + 2 * row);
 }
 
-template <int D, int WD, int NV, bool LAYER>
-cudaError_t forward_ring(const NormForwardArgs& a, int threads, cudaStream_t s) {
-    const int per_sm = std::min(8, (NV > 2 ? 512 : 1024) / threads);
+template <int D, int WD, bool LAYER, int NV>
+cudaError_t forward_ring(const NormForwardArgs& a, cudaStream_t s) {
+    const int threads = ring_threads(a.h, Vec<D>::E, NV), per_sm = ring_blocks(threads, NV);
     const int grid = static_cast<int>(std::min<long long>(a.rows, static_cast<long long>(sm_count()) * per_sm));
     const int vectors = (a.w != nullptr) + (a.b != nullptr);
-    return with_ring(static_cast<size_t>(NV) * threads * 16, static_cast<size_t>(vectors) * a.h * sizeof(Bits<WD>), per_sm,
+    return with_ring(static_cast<size_t>(NV) * 16 * threads, static_cast<size_t>(vectors) * a.h * sizeof(Bits<WD>), per_sm,
                      [&](auto S, size_t smem) {
-                         auto* kernel = &norm_forward_ring_kernel<D, WD, NV, LAYER, decltype(S)::value>;
+                         auto* kernel = &norm_forward_ring_kernel<D, WD, LAYER, decltype(S)::value, NV>;
                          const cudaError_t e = cudaFuncSetAttribute(
                              kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
                          if (e != cudaSuccess) return e;
@@ -697,11 +749,11 @@ cudaError_t forward_ring(const NormForwardArgs& a, int threads, cudaStream_t s) 
 template <int D, int WD, int E, bool LAYER>
 cudaError_t forward_any(const NormForwardArgs& a, cudaStream_t s) {
     if constexpr (E > 1) {
-        const Shape ring = ring_shape(a.h, E);
-        static const int mode = getenv("BCCL_X") ? atoi(getenv("BCCL_X")) : 0;
-        if (mode < 8 && ring.threads != 0 && a.rows > (mode ? 0 : 2ll * sm_count() * ((ring.nv > 2 ? 512 : 1024) / ring.threads))) {
-            if (ring.nv == 2) return forward_ring<D, WD, 2, LAYER>(a, ring.threads, s);
-            return forward_ring<D, WD, 4, LAYER>(a, ring.threads, s);
+        // Blocks that walk several rows: below that a row per block fills the SMs sooner.
+        const int nv = ring_accesses(a.h, E);
+        if (nv != 0 && a.rows > static_cast<long long>(sm_count()) * ring_blocks(ring_threads(a.h, E, nv), nv)) {
+            if (nv == 2) return forward_ring<D, WD, LAYER, 2>(a, s);
+            if constexpr (E == 8) return forward_ring<D, WD, LAYER, 4>(a, s);
         }
     }
     const Shape sh = forward_shape(a.h, E);
@@ -731,12 +783,13 @@ cudaError_t backward(const NormBackwardArgs& a, int threads, int grid, cudaStrea
     return cudaGetLastError();
 }
 
-template <int D, int WD, int NV, bool LAYER>
-cudaError_t backward_ring(const NormBackwardArgs& a, int threads, int grid, cudaStream_t s) {
-    const int per_sm = std::max(1, std::min(static_cast<int>(ceil_div(grid, sm_count())), (NV > 2 ? 512 : 1024) / threads));
-    return with_ring(static_cast<size_t>(2) * NV * threads * 16, a.w != nullptr ? a.h * sizeof(Bits<WD>) : 0, per_sm,
+template <int D, int WD, bool LAYER, int NV>
+cudaError_t backward_ring(const NormBackwardArgs& a, int grid, cudaStream_t s) {
+    const int threads = ring_threads(a.h, Vec<D>::E, NV);
+    const int per_sm = std::max(1, std::min(static_cast<int>(ceil_div(grid, sm_count())), ring_blocks(threads, NV)));
+    return with_ring(static_cast<size_t>(2) * NV * 16 * threads, a.w != nullptr ? a.h * sizeof(Bits<WD>) : 0, per_sm,
                      [&](auto S, size_t smem) {
-                         auto* kernel = &norm_backward_ring_kernel<D, WD, NV, LAYER, decltype(S)::value>;
+                         auto* kernel = &norm_backward_ring_kernel<D, WD, LAYER, decltype(S)::value, NV>;
                          const cudaError_t e = cudaFuncSetAttribute(
                              kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
                          if (e != cudaSuccess) return e;
@@ -747,8 +800,11 @@ cudaError_t backward_ring(const NormBackwardArgs& a, int threads, int grid, cuda
 
 // Rows of partial sums that the backward pass of this shape writes.
 int partial_rows(long long rows, long long h, int e) {
+    const int nv = e > 1 ? ring_accesses(h, e) : 0;
+    if (nv != 0) return row_blocks(rows, 1, ring_blocks(ring_threads(h, e, nv), nv));
     const Shape sh = backward_shape(h, e);
-    if (sh.threads != 0) return row_blocks(rows, sh.threads, sh.nv, e);
+    if (sh.threads == 32) return row_blocks(rows, kWarpRows, 1024 / (32 * kWarpRows));
+    if (sh.threads != 0) return row_blocks(rows, 1, std::max(1, std::min(8, 1024 / sh.threads)));
     return static_cast<int>(std::max(1ll, std::min<long long>(ceil_div(rows, 8), kColumnChunks)));
 }
 
@@ -757,21 +813,24 @@ cudaError_t backward_any(const NormBackwardArgs& a, cudaStream_t s) {
     const Shape sh = backward_shape(a.h, E);
     const int parts = partial_rows(a.rows, a.h, E);
     cudaError_t e = cudaSuccess;
-    if (sh.threads != 0) {
+    const int nv = E > 1 ? ring_accesses(a.h, E) : 0;
+    if (nv != 0) {
+        if constexpr (E == 8)
+            e = nv == 2 ? backward_ring<D, WD, LAYER, 2>(a, parts, s) : backward_ring<D, WD, LAYER, 4>(a, parts, s);
+        else if constexpr (E == 4)
+            e = backward_ring<D, WD, LAYER, 2>(a, parts, s);
+    } else if (sh.threads != 0) {
         if constexpr (E > 1) {
-            if (sh.threads == 32)
-                e = sh.nv == 1 ? backward<D, WD, E, 1, LAYER, true>(a, sh.threads, parts, s)
-                               : backward<D, WD, E, 2, LAYER, true>(a, sh.threads, parts, s);
-            else
-                e = sh.nv == 2 ? backward_ring<D, WD, 2, LAYER>(a, sh.threads, parts, s)
-                               : backward_ring<D, WD, 4, LAYER>(a, sh.threads, parts, s);
+            e = sh.nv == 1 ? backward<D, WD, E, 1, LAYER, true>(a, sh.threads, parts, s)
+                           : backward<D, WD, E, 2, LAYER, true>(a, sh.threads, parts, s);
         } else {
             if (sh.threads == 32)
                 e = sh.nv == 4 ? backward<D, WD, E, 4, LAYER, true>(a, sh.threads, parts, s)
                                : backward<D, WD, E, 16, LAYER, true>(a, sh.threads, parts, s);
             else
-                e = sh.nv == 8 ? backward<D, WD, E, 8, LAYER, false>(a, sh.threads, parts, s)
-                               : backward<D, WD, E, 16, LAYER, false>(a, sh.threads, parts, s);
+                e = sh.nv == 4   ? backward<D, WD, E, 4, LAYER, false>(a, sh.threads, parts, s)
+                    : sh.nv == 8 ? backward<D, WD, E, 8, LAYER, false>(a, sh.threads, parts, s)
+                                 : backward<D, WD, E, 16, LAYER, false>(a, sh.threads, parts, s);
         }
     } else {
         norm_backward_long_kernel<D, WD, E, LAYER>

@@ -111,6 +111,55 @@ __device__ __forceinline__ void store_raw_cs(Bits<D>* p, const Raw<D, E>& r) {
     else __stcs(reinterpret_cast<uint4*>(p), r.v);
 }
 
+// Two floats in one register pair: sm_100 multiplies and adds both in one instruction.
+struct F2 {
+    unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 split(F2 a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+    return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+// 16 bytes as pairs of floats, and back.
+template <int D>
+__device__ __forceinline__ void unpack2(const uint4& u, F2 (&a)[Vec<D>::E / 2]) {
+    float f[Vec<D>::E];
+    Vec<D>::unpack(u, f);
+#pragma unroll
+    for (int i = 0; i < Vec<D>::E / 2; ++i) a[i] = f2(f[2 * i], f[2 * i + 1]);
+}
+template <int D>
+__device__ __forceinline__ uint4 pack2(const F2 (&a)[Vec<D>::E / 2]) {
+    float f[Vec<D>::E];
+#pragma unroll
+    for (int i = 0; i < Vec<D>::E / 2; ++i) {
+        const float2 t = split(a[i]);
+        f[2 * i] = t.x;
+        f[2 * i + 1] = t.y;
+    }
+    return Vec<D>::pack(f);
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -128,17 +177,31 @@ __device__ __forceinline__ float2 warp_sum(float2 v) {
 // Sums over all threads of a block (a multiple of 32, at most 1024) in a fixed order, result in
 // every thread. `parity` alternates between calls: a call's buffer is written again only two
 // calls later, after the barrier of the call between, so one barrier per sum is enough.
-__device__ __forceinline__ float block_sum(float v, float (&buf)[2][32], int parity, int tid, int warps) {
+__device__ __forceinline__ float plus(float a, float b) { return a + b; }
+__device__ __forceinline__ float2 plus(float2 a, float2 b) { return make_float2(a.x + b.x, a.y + b.y); }
+template <typename T>
+__device__ __forceinline__ T block_sum(T v, T (&buf)[2][32], int parity, int tid, int warps) {
     v = warp_sum(v);
+    if (warps == 1) return v;
     if ((tid & 31) == 0) buf[parity][tid >> 5] = v;
     __syncthreads();
-    return warp_sum((tid & 31) < warps ? buf[parity][tid & 31] : 0.0f);
+    if (warps <= 8) {  // a few broadcast loads instead of another tree of shuffles
+        T s = buf[parity][0];
+#pragma unroll
+        for (int w = 1; w < 8; ++w)
+            if (w < warps) s = plus(s, buf[parity][w]);
+        return s;
+    }
+    return warp_sum((tid & 31) < warps ? buf[parity][tid & 31] : T{});
 }
-__device__ __forceinline__ float2 block_sum(float2 v, float2 (&buf)[2][32], int parity, int tid, int warps) {
-    v = warp_sum(v);
-    if ((tid & 31) == 0) buf[parity][tid >> 5] = v;
-    __syncthreads();
-    return warp_sum((tid & 31) < warps ? buf[parity][tid & 31] : make_float2(0.0f, 0.0f));
+
+// 1 / sqrt(v) to within an ulp or two: the hardware's approximation and a Newton step, in 6
+// instructions where the correctly rounded root and quotient take some 50 in every thread of a row.
+__device__ __forceinline__ float inv_sqrt(float v) {
+    const float r = rsqrtf(v);
+    const float d = fmaf(-v * r, r, 1.0f);
+    // Zero, infinity and NaN as they come out of the approximation.
+    return fabsf(d) < 1.0f ? fmaf(0.5f * r, d, r) : r;
 }
 
 inline bool float_type(int d) { return d == kF32 || d == kBF16 || d == kF16; }
