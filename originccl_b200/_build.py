@@ -40,13 +40,16 @@ def cutlass_include() -> Path | None:
 
 def python_extension_flags() -> tuple[str, str] | None:
     """Compile and link flags of the Python extension (csrc/python), or None where Python's or
-    PyTorch's headers are missing; the package then reads tensor lists in Python."""
+    PyTorch's CUDA headers are missing; the compute operators then refuse to load."""
     py = Path(sysconfig.get_paths()["include"])
     torch = _site_packages() / "torch"
-    if not (py / "Python.h").exists() or not (torch / "include" / "torch" / "csrc" / "autograd" / "python_variable.h").exists():
+    inc = torch / "include"
+    if not (py / "Python.h").exists() or not (inc / "torch" / "csrc" / "autograd" / "python_variable.h").exists() or \
+            not (torch / "lib" / "libc10_cuda.so").exists():
         return None
-    return (f"-isystem {py} -isystem {torch / 'include'} -isystem {torch / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
-            f"-L{torch / 'lib'} -ltorch_python -ltorch_cpu -lc10")
+    return (f"-I{CSRC / 'include'} -isystem {py} -isystem {inc} -isystem {inc / 'torch' / 'csrc' / 'api' / 'include'} "
+            f"-isystem {CUDA_HOME / 'include'}",
+            f"-L{torch / 'lib'} -ltorch_python -ltorch_cpu -lc10 -lc10_cuda -L{LIBDIR} -lbccl -Wl,-rpath,'$$ORIGIN'")
 
 
 # Host sources whose inner loops must be vectorised (-O2's cost model leaves loops with a
@@ -120,7 +123,7 @@ def _ninja_file() -> str:
                   "  depfile = $out.d",
                   "  deps = gcc",
                   "  description = PYEXT $out",
-                  f"build {LIBDIR / '_tensor_list.so'}: pyext {CSRC / 'python' / 'tensor_list.cc'}"]
+                  f"build {LIBDIR / '_ops.so'}: pyext {CSRC / 'python' / 'ops_module.cc'} | {LIBDIR / 'libbccl.so'}"]
     lines.append(f"build {LIBDIR / 'libbccl.so'}: link {' '.join(map(str, objs))}")
     launcher = CSRC / "launcher" / "bccl_run.cc"
     lobj = BUILD / "launcher_bccl_run.cc.o"

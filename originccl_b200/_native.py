@@ -147,19 +147,25 @@ def last_error() -> str:
     return msg.decode() if msg else ""
 
 
-def tensor_list():
-    """The Python extension that reads lists of torch tensors (csrc/python/tensor_list.cc), or None where
-    it was not built (no PyTorch headers) or was built for another PyTorch."""
-    import importlib.machinery
-    import importlib.util
-    path = _LIB_PATH.parent / "_tensor_list.so"
-    if not path.exists():
-        return None
-    import torch  # noqa: F401  (its libraries hold the symbols)
-    loader = importlib.machinery.ExtensionFileLoader("_tensor_list", str(path))
-    try:
-        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_tensor_list", loader))
+
+_OPS = None
+
+
+def ops():
+    """The Python extension of the compute operators (csrc/python/ops_module.cc), built against the
+    installed PyTorch."""
+    global _OPS
+    if _OPS is None:
+        import importlib.machinery
+        import importlib.util
+        import torch  # noqa: F401  (its libraries hold the symbols)
+        path = _LIB_PATH.parent / "_ops.so"
+        if not path.exists():
+            raise ImportError(f"{path} is missing: build the native library with Python's and PyTorch's CUDA headers "
+                              "installed (python -m originccl_b200._build)")
+        lib()
+        loader = importlib.machinery.ExtensionFileLoader("_ops", str(path))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_ops", loader))
         loader.exec_module(module)
-    except ImportError:
-        return None
-    return module
+        _OPS = module
+    return _OPS

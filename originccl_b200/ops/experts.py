@@ -20,13 +20,12 @@ from typing import Optional, Tuple
 
 import torch
 
-from ._launch import Entry, float_code, int_code, like_or_f32, one_device, ptr, rows as _rows
+from .. import _native
 
 MAX_EXPERTS = 1023
 MAX_TOP = 64
 
-_sort, _dispatch = Entry("bcclExpertSort"), Entry("bcclExpertDispatch")
-_combine, _combine_backward = Entry("bcclExpertCombine"), Entry("bcclExpertCombineBackward")
+_ops = _native.ops()
 
 
 class ExpertOrder:
@@ -36,18 +35,20 @@ class ExpertOrder:
     assignment of each sorted row, -1 behind the last. ``offsets`` [num_experts + 1] int32: the first row of
     each expert; the last entry counts the kept rows."""
 
-    __slots__ = ("slots", "sources", "offsets", "tokens", "top", "num_experts", "device")
+    __slots__ = ("slots", "sources", "offsets")
 
     def __init__(self, slots, sources, offsets) -> None:
         for t, dim in ((slots, 2), (sources, 1), (offsets, 1)):
             if t.dtype is not torch.int32 or t.dim() != dim or not t.is_contiguous():
                 raise ValueError("ExpertOrder: slots, sources and offsets must come from sort_by_expert")
-        self.slots, self.sources, self.offsets = slots, sources, offsets
-        self.tokens, self.top = slots.shape
-        self.num_experts = offsets.shape[0] - 1
-        if not 1 <= self.top <= MAX_TOP or not 1 <= self.num_experts <= MAX_EXPERTS or sources.shape[0] != slots.numel():
+        if not 1 <= slots.shape[1] <= MAX_TOP or not 2 <= offsets.shape[0] <= MAX_EXPERTS + 1 or \
+                sources.shape[0] != slots.numel() or slots.device != offsets.device or slots.device != sources.device:
             raise ValueError("ExpertOrder: slots, sources and offsets must come from sort_by_expert")
-        self.device = one_device("ExpertOrder", slots, sources, offsets)
+        self.slots, self.sources, self.offsets = slots, sources, offsets
+
+    @property
+    def num_experts(self) -> int:
+        return self.offsets.shape[0] - 1
 
     def rank_counts(self, world: int) -> torch.Tensor:
         """Rows for each of ``world`` ranks that hold equal, consecutive shares of the experts (the
@@ -59,100 +60,31 @@ class ExpertOrder:
 
 def sort_by_expert(expert_ids, num_experts: int) -> ExpertOrder:
     """expert_ids [tokens, top] (or [tokens]) int32 or int64 -> :class:`ExpertOrder`."""
-    op = "sort_by_expert"
-    icode = int_code(op, "expert_ids", expert_ids.dtype)
-    shape = expert_ids.shape
-    if len(shape) not in (1, 2):
-        raise ValueError(f"{op}: expert_ids must be [tokens, top], got shape {tuple(shape)}")
-    tokens, top = shape if len(shape) == 2 else (shape[0], 1)
-    if not 1 <= top <= MAX_TOP:
-        raise ValueError(f"{op}: 1 to {MAX_TOP} experts per token, got {top}")
-    if not 1 <= num_experts <= MAX_EXPERTS:
-        raise ValueError(f"{op}: 1 to {MAX_EXPERTS} experts, got {num_experts}")
-    device = one_device(op, expert_ids)
-    ids = expert_ids.contiguous()
-    slots = ids.new_empty((tokens, top), dtype=torch.int32)
-    sources = ids.new_empty(tokens * top, dtype=torch.int32)
-    offsets = ids.new_empty(num_experts + 1, dtype=torch.int32)
-    _sort(device, ids.data_ptr(), icode, tokens, top, num_experts, slots.data_ptr(), sources.data_ptr(), offsets.data_ptr())
-    return ExpertOrder(slots, sources, offsets)
-
-
-def _rows_of(op, what, t, n, order):
-    """Width of ``t``, which must be [n, h] beside the order."""
-    shape = t.shape
-    if len(shape) != 2 or shape[0] != n or shape[1] < 1:
-        raise ValueError(f"{op}: {what} must be [{n}, h], got shape {tuple(shape)}")
-    if t.get_device() != order.device:
-        raise ValueError(f"{op}: {what} must be a CUDA tensor on the order's device, got {t.device}")
-    return shape[1]
-
-
-def _weights(op, weights, order, dtype, code):
-    if weights is None:
-        return None, code
-    wcode = like_or_f32(op, "weights", weights.dtype, dtype)
-    if weights.shape != (order.tokens, order.top) or weights.get_device() != order.device:
-        raise ValueError(f"{op}: weights must be ({order.tokens}, {order.top}) on the order's device, got "
-                         f"{tuple(weights.shape)} on {weights.device}")
-    return weights.contiguous(), wcode
+    order = ExpertOrder.__new__(ExpertOrder)
+    order.slots, order.sources, order.offsets = _ops.expert_sort(expert_ids, num_experts)
+    return order
 
 
 def dispatch_forward(x, order: ExpertOrder, out=None):
     """x [tokens, h] -> rows [tokens * top, h] sorted by expert (``out``, contiguous, receives them, e.g. a
     registered send buffer)."""
-    op = "dispatch"
-    code = float_code(op, "input", x.dtype)
-    h = _rows_of(op, "input", x, order.tokens, order)
-    n = order.tokens * order.top
-    if out is None:
-        out = x.new_empty((n, h))
-    elif out.dtype is not x.dtype or _rows_of(op, "out", out, n, order) != h or not out.is_contiguous():
-        raise ValueError(f"{op}: out must be a contiguous {x.dtype} tensor of shape ({n}, {h})")
-    xr, stride = _rows(x, h)
-    _dispatch(order.device, xr.data_ptr(), stride, order.slots.data_ptr(), order.offsets.data_ptr(), order.tokens, order.top,
-              order.num_experts, h, out.data_ptr(), code)
-    return out
-
-
-def _combine_rows(op, rows, order, weights):
-    code = float_code(op, "rows", rows.dtype)
-    h = _rows_of(op, "rows", rows, order.tokens * order.top, order)
-    w, wcode = _weights(op, weights, order, rows.dtype, code)
-    rows = rows.contiguous()
-    y = rows.new_empty((order.tokens, h))
-    _combine(order.device, rows.data_ptr(), order.slots.data_ptr(), ptr(w), wcode, order.tokens, order.top, h, y.data_ptr(),
-             h, code)
-    return y
+    return _ops.dispatch(x, order.slots, order.offsets, out)
 
 
 def dispatch_backward(drows, order: ExpertOrder):
     """The gradient of x: each token's sum over its kept assignments' rows of drows."""
-    return _combine_rows("dispatch_backward", drows, order, None)
+    return _ops.combine(drows, order.slots, order.offsets, None)
 
 
 def combine_forward(rows, order: ExpertOrder, weights=None):
     """rows [tokens * top, h] in sorted order, weights [tokens, top] (None: ones) -> y [tokens, h]."""
-    return _combine_rows("combine", rows, order, weights)
+    return _ops.combine(rows, order.slots, order.offsets, weights)
 
 
 def combine_backward(dy, rows, order: ExpertOrder, weights=None, *, weight_grad: bool = True) -> Tuple:
     """(drows, dweights) of :func:`combine_forward`; dweights is None without weights or where it is not
     asked for."""
-    op = "combine_backward"
-    code = float_code(op, "dy", dy.dtype)
-    h = _rows_of(op, "dy", dy, order.tokens, order)
-    n = order.tokens * order.top
-    if _rows_of(op, "rows", rows, n, order) != h or rows.dtype is not dy.dtype:
-        raise ValueError(f"{op}: rows must be {dy.dtype} of width {h}, got {rows.dtype} {tuple(rows.shape)}")
-    w, wcode = _weights(op, weights, order, dy.dtype, code)
-    rows = rows.contiguous()
-    d, stride = _rows(dy, h)
-    drows = dy.new_empty((n, h))
-    dw = torch.empty_like(w) if w is not None and weight_grad else None
-    _combine_backward(order.device, d.data_ptr(), stride, rows.data_ptr(), order.slots.data_ptr(), order.offsets.data_ptr(),
-                      ptr(w), wcode, order.tokens, order.top, order.num_experts, h, drows.data_ptr(), ptr(dw), code)
-    return drows, dw
+    return _ops.combine_backward(dy, rows, order.slots, order.offsets, weights, weight_grad)
 
 
 class _Dispatch(torch.autograd.Function):

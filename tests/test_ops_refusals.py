@@ -67,6 +67,10 @@ def test_embedding_refuses():
         embedding.embedding_backward(dy, ids, -1)
     with pytest.raises(ValueError, match="accumulate"):
         embedding.embedding_backward(dy, ids, 6, accumulate=True)
+    with pytest.raises(TypeError, match="tensor"):
+        embedding.embedding_forward([1, 2], w)
+    with pytest.raises(TypeError):
+        embedding.embedding_forward(ids, w, scale="2")
 
 
 def test_experts_refuse():
@@ -89,8 +93,22 @@ def test_experts_refuse():
                   (ids, ids.reshape(-1), ids.reshape(-1)[:1])):
         with pytest.raises(ValueError, match="sort_by_expert"):
             experts.ExpertOrder(*parts)
+    order = experts.ExpertOrder(ids, ids.reshape(-1), ids.reshape(-1)[:5])
+    assert order.num_experts == 4
+    with pytest.raises(ValueError, match="split"):
+        order.rank_counts(3)
     with pytest.raises(ValueError, match="CUDA"):
-        experts.ExpertOrder(ids, ids.reshape(-1), ids.reshape(-1)[:5])
+        experts.dispatch_forward(torch.zeros(5, 8), order)
+    with pytest.raises(ValueError, match=r"\[5, h\]"):
+        experts.dispatch_forward(torch.zeros(4, 8), order)
+    with pytest.raises(ValueError, match=r"\[10, h\]"):
+        experts.combine_forward(torch.zeros(5, 8), order)
+    with pytest.raises(ValueError, match="weights"):
+        experts.combine_forward(torch.zeros(10, 8), order, torch.zeros(5, 3))
+    with pytest.raises(TypeError, match="weights"):
+        experts.combine_forward(torch.zeros(10, 8), order, torch.zeros(5, 2).half())
+    with pytest.raises(ValueError, match="rows"):
+        experts.combine_backward(torch.zeros(5, 8), torch.zeros(10, 9), order)
 
 
 def test_clipping_refuses():
