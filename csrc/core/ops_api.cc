@@ -135,7 +135,7 @@ int bcclEmbeddingForward(const void* ids, int ids_dtype, int64_t n, const void* 
 
 size_t bcclEmbeddingBackwardWorkspace(int64_t n, int64_t rows, int64_t h) {
     if (n < 1 || n > INT32_MAX || rows < 0 || rows > INT32_MAX - 1 || h < 1 || h > kMaxWidth) return 0;
-    return bccl::EmbeddingBackwardWorkspace(n, rows, h);
+    return bccl::EmbeddingBackwardWorkspace(n, h);
 }
 
 int bcclEmbeddingBackward(const void* dy, int64_t dy_stride, const void* ids, int ids_dtype, int64_t n, void* dtable,
@@ -151,7 +151,7 @@ int bcclEmbeddingBackward(const void* dy, int64_t dy_stride, const void* ids, in
         return Bad(op, "invalid gradient");
     if (n > 0 && rows > 0 &&
         (workspace == nullptr || !Aligned(workspace, 16) ||
-         workspace_bytes < bccl::EmbeddingBackwardWorkspace(n, rows, h)))
+         workspace_bytes < bccl::EmbeddingBackwardWorkspace(n, h)))
         return Bad(op, "workspace too small or misaligned");
     const bccl::EmbeddingArgs a{ids, ids_dtype == kI64, n, rows, h, first_row};
     return Launched(op, bccl::LaunchEmbeddingBackward(a, dy, dy_stride, dtable, scale, skip_id, has_skip != 0,

@@ -2,8 +2,7 @@
 //
 //   out[i] = scale * table[ids[i] - first],  dtable[v] = scale * sum of dy[i] over ids[i] == first + v
 //
-// Gradient, three launches. (1) One cluster sorts the positions by token (key_sort.cuh) and marks
-// the rows that occur. (2) The sorted positions are cut into windows of equal length, so a token
+// Gradient, three launches. (1) One cluster sorts the positions by token (key_sort.cuh). (2) The sorted positions are cut into windows of equal length, so a token
 // that is everywhere is summed by many blocks: a block adds the rows of its window in order and
 // writes every token that lies wholly in it; the part of a token that runs over the window's
 // edge goes to a 32-bit partial row. The same launch writes zeros to the rows that do not occur.
@@ -55,33 +54,20 @@ __global__ void __launch_bounds__(kThreads) lookup_kernel(const KeySource key, l
     }
 }
 
-// sorted: {row, position} of the n positions, by row; a and b are the buffers between passes
-// (the last pass writes b). present (rows bytes) marks the rows that occur.
-__global__ void __launch_bounds__(1024) position_sort_kernel(const KeySource key, long long n, int bits, int passes,
-                                                             uint2* a, uint2* b, unsigned char* present) {
+// Writes {row, position} of the n positions to b, by row; a is the other buffer between passes.
+template <int BITS>
+__global__ void __launch_bounds__(1024) position_sort_kernel(const KeySource key, long long n, int passes, uint2* a, uint2* b) {
     extern __shared__ unsigned int counters[];
-    namespace cg = cooperative_groups;
-    if (present != nullptr) {
-        // Cleared by all blocks; the first pass's cluster barriers come before the last pass marks.
-        const long long threads = static_cast<long long>(gridDim.x) * blockDim.x;
-        const long long me = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-        for (long long i = me; i < (key.bins + 15) / 16; i += threads)
-            reinterpret_cast<uint4*>(present)[i] = make_uint4(0, 0, 0, 0);
-    }
     for (int p = 0; p < passes; ++p) {
         // Buffers alternate so that the last pass writes b.
         uint2* to = ((passes - 1 - p) & 1) ? a : b;
         const uint2* from = to == a ? b : a;
-        const bool last = p == passes - 1;
-        sort_pass(
-            counters, n, p * bits, bits,
+        sort_pass<BITS>(
+            counters, n, p * BITS, p == passes - 1,
             [&](long long i) {
                 return p == 0 ? make_uint2(key(i), static_cast<unsigned int>(i)) : __ldcg(from + i);
             },
-            [&](unsigned int place, unsigned int k, unsigned int pos) {
-                to[place] = make_uint2(k, pos);
-                if (last && present != nullptr && k < key.bins) present[k] = 1;
-            },
+            [&](unsigned int place, unsigned int k, unsigned int pos) { to[place] = make_uint2(k, pos); },
             [](unsigned int, unsigned int) {});
     }
 }
@@ -121,10 +107,54 @@ struct WindowArgs {
     int window;
     long long windows;
     float* partial;  // [windows][2][h]: a token that came from the left; one that goes on to the right
-    const unsigned char* present;
     float scale;
     int accumulate;
+    int tile;  // rows that a block clears at a time
 };
+
+constexpr int kMaxTile = 4096;
+
+// First of the n sorted positions whose row is at least `row`.
+__device__ __forceinline__ long long first_of(const uint2* sorted, long long n, long long row) {
+    long long lo = 0, hi = n;
+    while (lo < hi) {
+        const long long mid = (lo + hi) >> 1;
+        if (__ldg(&sorted[mid].x) < row) lo = mid + 1; else hi = mid;
+    }
+    return lo;
+}
+
+// Zeros for the rows of the table that do not occur among the sorted positions. The positions of a
+// tile's rows set bits in shared memory. (Marking rows while sorting took longer than the sort: thousands
+// of stores to the byte of a frequent token.)
+template <int OD, int E>
+__device__ __forceinline__ void clear_absent(const WindowArgs& a, long long c, Bits<OD>* dtable) {
+    __shared__ unsigned int present[kMaxTile / 32];
+    __shared__ long long range[2];
+    float zero[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) zero[e] = 0.0f;
+    const long long tiles = (a.rows + a.tile - 1) / a.tile;
+    for (long long t = blockIdx.x - a.windows; t < tiles; t += gridDim.x - a.windows) {
+        const long long r0 = t * a.tile;
+        const int count = static_cast<int>(min(static_cast<long long>(a.tile), a.rows - r0));
+        for (int i = threadIdx.x; i < (count + 31) / 32; i += blockDim.x) present[i] = 0;
+        if (threadIdx.x < 2) range[threadIdx.x] = first_of(a.sorted, a.n, threadIdx.x == 0 ? r0 : r0 + count);
+        __syncthreads();
+        for (long long i = range[0] + threadIdx.x; i < range[1]; i += blockDim.x) {
+            const unsigned int row = __ldg(&a.sorted[i].x);
+            // A token's first position is enough.
+            if (i == range[0] || __ldg(&a.sorted[i - 1].x) != row)
+                atomicOr(&present[(row - r0) >> 5], 1u << ((row - r0) & 31));
+        }
+        __syncthreads();
+        if (c < a.h) {
+            for (int r = 0; r < count; ++r)
+                if (!(present[r >> 5] >> (r & 31) & 1)) store_f_cs<OD, E>(dtable + (r0 + r) * a.h + c, zero);
+        }
+        __syncthreads();
+    }
+}
 
 // blockIdx.x < windows: a window of sorted positions; beyond: rows to clear. blockIdx.y: columns.
 template <int D, int OD, int E>
@@ -133,12 +163,7 @@ __global__ void __launch_bounds__(kThreads) window_kernel(const WindowArgs a, co
     __shared__ uint2 item[kMaxWindow + 2];  // the window and its neighbours on either side
     const long long c = (static_cast<long long>(blockIdx.y) * blockDim.x + threadIdx.x) * E;
     if (blockIdx.x >= a.windows) {
-        if (c >= a.h) return;
-        float zero[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) zero[e] = 0.0f;
-        for (long long r = blockIdx.x - a.windows; r < a.rows; r += gridDim.x - a.windows)
-            if (__ldg(a.present + r) == 0) store_f_cs<OD, E>(dtable + r * a.h + c, zero);
+        clear_absent<OD, E>(a, c, dtable);
         return;
     }
     const long long w0 = static_cast<long long>(blockIdx.x) * a.window;
@@ -262,10 +287,10 @@ cudaError_t LaunchEmbeddingForward(const EmbeddingArgs& a, const void* table, lo
     });
 }
 
-size_t EmbeddingBackwardWorkspace(long long n, long long rows, long long h) {
+size_t EmbeddingBackwardWorkspace(long long n, long long h) {
     using namespace ops;
     const long long windows = ceil_div(n, window_of(n));
-    return 2 * align16(sizeof(uint2) * static_cast<size_t>(n)) + align16(static_cast<size_t>(rows)) +
+    return 2 * align16(sizeof(uint2) * static_cast<size_t>(n)) +
            align16(sizeof(float) * 2 * static_cast<size_t>(windows) * static_cast<size_t>(h));
 }
 
@@ -283,8 +308,6 @@ cudaError_t LaunchEmbeddingBackward(const EmbeddingArgs& a, const void* dy, long
     ws += align16(sizeof(uint2) * static_cast<size_t>(a.n));
     uint2* buf_b = reinterpret_cast<uint2*>(ws);
     ws += align16(sizeof(uint2) * static_cast<size_t>(a.n));
-    unsigned char* present = reinterpret_cast<unsigned char*>(ws);
-    ws += align16(static_cast<size_t>(a.rows));
     float* partial = reinterpret_cast<float*>(ws);
 
     int key_bits = 1;
@@ -292,21 +315,22 @@ cudaError_t LaunchEmbeddingBackward(const EmbeddingArgs& a, const void* dy, long
     const int passes = static_cast<int>(ceil_div(key_bits, kSortMaxBits));
     const int bits = static_cast<int>(ceil_div(key_bits, passes));
     const KeySource key{a.ids, a.ids64, a.first, a.rows, skip, has_skip ? 1 : 0};
-    const cudaError_t e = launch_sort(position_sort_kernel, a.n, bits, stream, key, a.n, bits, passes, buf_a, buf_b,
-                                      accumulate ? static_cast<unsigned char*>(nullptr) : present);
+    const cudaError_t e = with_bits(bits, [&](auto B) {
+        constexpr int kB = decltype(B)::value;
+        return launch_sort(position_sort_kernel<kB>, a.n, kB, stream, key, a.n, passes, buf_a, buf_b);
+    });
     if (e != cudaSuccess) return e;
 
-    WindowArgs w{};
-    w.sorted = buf_b;
-    w.n = a.n;
-    w.rows = a.rows;
-    w.h = a.h;
-    w.window = window_of(a.n);
-    w.windows = ceil_div(a.n, w.window);
-    w.partial = partial;
-    w.present = present;
-    w.scale = scale;
-    w.accumulate = accumulate ? 1 : 0;
+    WindowArgs args{};
+    args.sorted = buf_b;
+    args.n = a.n;
+    args.rows = a.rows;
+    args.h = a.h;
+    args.window = window_of(a.n);
+    args.windows = ceil_div(a.n, args.window);
+    args.partial = partial;
+    args.scale = scale;
+    args.accumulate = accumulate ? 1 : 0;
     const bool wide = rows16(dy, dy_stride, a.h, size_of(dtype)) && rows16(dtable, a.h, a.h, size_of(out_dtype));
     return with_types(dtype, out_dtype, [&](auto D, auto O) {
         constexpr int kD = decltype(D)::value, kO = decltype(O)::value, kE = Vec<kD>::E;
@@ -314,8 +338,11 @@ cudaError_t LaunchEmbeddingBackward(const EmbeddingArgs& a, const void* dy, long
             constexpr int E = decltype(EE)::value;
             const int threads = static_cast<int>(std::min<long long>(kThreads, round32(ceil_div(a.h, E))));
             const unsigned cols = static_cast<unsigned>(ceil_div(a.h, static_cast<long long>(threads) * E));
-            const long long clear =
-                accumulate ? 0 : std::max(1ll, std::min<long long>(a.rows, static_cast<long long>(sm_count()) * 8 / cols));
+            // Rows to clear in tiles, as many as there are blocks for up to 8 per SM.
+            WindowArgs w = args;
+            const long long most = std::max(1ll, static_cast<long long>(sm_count()) * 8 / cols);
+            w.tile = static_cast<int>(std::min<long long>(kMaxTile, std::max(1ll, ceil_div(a.rows, most))));
+            const long long clear = accumulate ? 0 : std::min(most, ceil_div(a.rows, w.tile));
             window_kernel<kD, kO, E><<<dim3(static_cast<unsigned>(w.windows + clear), cols), threads, 0, stream>>>(
                 w, static_cast<const Bits<kD>*>(dy), dy_stride, static_cast<Bits<kO>*>(dtable));
             cudaError_t err = cudaGetLastError();

@@ -19,12 +19,13 @@ namespace ops {
 namespace {
 
 // One pass: the digits are the experts themselves and `experts` for dropped assignments.
-__global__ void __launch_bounds__(1024) expert_sort_kernel(const KeySource key, long long n, int bits, int* slots,
-                                                           int* sources, int* offsets) {
+template <int BITS>
+__global__ void __launch_bounds__(1024) expert_sort_kernel(const KeySource key, long long n, int* slots, int* sources,
+                                                           int* offsets) {
     extern __shared__ unsigned int counters[];
     const unsigned int experts = static_cast<unsigned int>(key.bins);
-    sort_pass(
-        counters, n, 0, bits, [&](long long i) { return make_uint2(key(i), static_cast<unsigned int>(i)); },
+    sort_pass<BITS>(
+        counters, n, 0, true, [&](long long i) { return make_uint2(key(i), static_cast<unsigned int>(i)); },
         [&](unsigned int place, unsigned int k, unsigned int a) {
             slots[a] = k < experts ? static_cast<int>(place) : -1;
             sources[place] = k < experts ? static_cast<int>(a) : -1;
@@ -170,7 +171,10 @@ cudaError_t LaunchExpertSort(const void* ids, int ids64, long long n, int expert
     int bits = 1;
     while ((1 << bits) < experts + 1) ++bits;
     const KeySource key{ids, ids64, 0, experts, 0, 0};
-    return launch_sort(expert_sort_kernel, n, bits, stream, key, n, bits, slots, sources, offsets);
+    return with_bits(bits, [&](auto B) {
+        constexpr int kB = decltype(B)::value;
+        return launch_sort(expert_sort_kernel<kB>, n, kB, stream, key, n, slots, sources, offsets);
+    });
 }
 
 cudaError_t LaunchExpertDispatch(const void* x, long long x_stride, const int* slots, const int* offsets,

@@ -128,21 +128,24 @@ constexpr int kFoldThreads = 1024;
 __global__ void __launch_bounds__(kFoldThreads) fold_kernel(const double* __restrict__ partials, unsigned int n,
                                                             int accumulate, double* sum) {
     double s = 0.0;
-#pragma unroll 16
+#pragma unroll 8
     for (unsigned int i = threadIdx.x; i < n; i += kFoldThreads) s += partials[i];
     s = block_sum_f64<kFoldThreads>(s);
     if (threadIdx.x == 0) *sum = accumulate ? *sum + s : s;
 }
 
 // The blocks take the chunks from the last to the first: what the squares read last is still in
-// L2 (126 MB) and is read from there.
+// L2 (126 MB) and is read from there. A block takes kInPlace chunks in place and one otherwise: in place
+// most launches find nothing to do, and then starting the warps is all they cost (1.5 GB: 37 us with
+// a block per chunk).
+constexpr int kInPlace = 4;
+
 template <int D, int O, int N>
 __global__ void __launch_bounds__(kThreads, 4) clip_kernel(const __grid_constant__ Table<N> t, int in_place,
                                                            const double* __restrict__ sum, float max_norm, float eps,
                                                            float* norm_out) {
     constexpr int E = Vec<D>::E;
-    // In place, a norm below the bound by more than rounding moves nothing: most steps. Their blocks
-    // (45000 for 1.5 GB) only look at the sum; with the root and the quotient that took 37 us.
+    // In place, a norm below the bound by more than rounding moves nothing: most steps.
     const double free_norm = static_cast<double>(max_norm) - eps;
     if (in_place && free_norm > 0.0 && *sum < free_norm * free_norm * (1.0 - 1e-6) && (blockIdx.x != 0 || norm_out == nullptr))
         return;
@@ -151,36 +154,39 @@ __global__ void __launch_bounds__(kThreads, 4) clip_kernel(const __grid_constant
     const float q = max_norm / (norm + eps);
     const float c = q > 1.0f ? 1.0f : q;  // a NaN stays
     if ((in_place && c == 1.0f) || t.n == 0) return;
-    const unsigned int chunk = gridDim.x - 1 - blockIdx.x;
-    const int i = tensor_of(t, chunk);
-    const ChunkView<D> view(t.in[i], t.count[i], chunk - t.start[i]);
-    Bits<O>* out = static_cast<Bits<O>*>(t.out[i]) - view.first;  // indexed like base
-    const bool wide = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-    Raw<D, E> r[kUnroll];
+    const unsigned int chunks = t.start[t.n];
+    for (unsigned int k = blockIdx.x; k < chunks; k += gridDim.x) {
+        const unsigned int chunk = chunks - 1 - k;
+        const int i = tensor_of(t, chunk);
+        const ChunkView<D> view(t.in[i], t.count[i], chunk - t.start[i]);
+        Bits<O>* out = static_cast<Bits<O>*>(t.out[i]) - view.first;  // indexed like base
+        const bool wide = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+        Raw<D, E> r[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-        const long long v = view.lo + u * kThreads + threadIdx.x;
-        if (v < view.hi && view.whole(v)) r[u].v = __ldcs(reinterpret_cast<const uint4*>(view.base + v * E));
-    }
-    if (threadIdx.x < 2) {
-        const long long v = threadIdx.x == 0 ? view.lo : view.hi - 1;
-        if (!view.whole(v) && (threadIdx.x == 0 || v != view.lo))
-            for (long long k = max(view.first, v * E); k < min(view.last, (v + 1) * E); ++k)
-                out[k] = Ty<O>::store(Ty<D>::load(view.base[k]) * c);
-    }
+        for (int u = 0; u < kUnroll; ++u) {
+            const long long v = view.lo + u * kThreads + threadIdx.x;
+            if (v < view.hi && view.whole(v)) r[u].v = __ldcs(reinterpret_cast<const uint4*>(view.base + v * E));
+        }
+        if (threadIdx.x < 2) {
+            const long long v = threadIdx.x == 0 ? view.lo : view.hi - 1;
+            if (!view.whole(v) && (threadIdx.x == 0 || v != view.lo))
+                for (long long j = max(view.first, v * E); j < min(view.last, (v + 1) * E); ++j)
+                    out[j] = Ty<O>::store(Ty<D>::load(view.base[j]) * c);
+        }
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-        const long long v = view.lo + u * kThreads + threadIdx.x;
-        if (v < view.hi && view.whole(v)) {
-            float a[E];
-            unpack<D, E>(r[u], a);
+        for (int u = 0; u < kUnroll; ++u) {
+            const long long v = view.lo + u * kThreads + threadIdx.x;
+            if (v < view.hi && view.whole(v)) {
+                float a[E];
+                unpack<D, E>(r[u], a);
 #pragma unroll
-            for (int e = 0; e < E; ++e) a[e] *= c;
-            if (wide) {
-                store_f_cs<O, E>(out + v * E, a);
-            } else {
+                for (int e = 0; e < E; ++e) a[e] *= c;
+                if (wide) {
+                    store_f_cs<O, E>(out + v * E, a);
+                } else {
 #pragma unroll
-                for (int e = 0; e < E; ++e) out[v * E + e] = Ty<O>::store(a[e]);
+                    for (int e = 0; e < E; ++e) out[v * E + e] = Ty<O>::store(a[e]);
+                }
             }
         }
     }
@@ -243,7 +249,7 @@ cudaError_t clip(const void* const* in, void* const* out, const size_t* counts, 
         i = fill(t, in, out, counts, i, n, size_of(dtype));
         if (i < 0) return cudaErrorInvalidValue;
         if (t.n == 0 && norm == nullptr) continue;
-        const unsigned int grid = std::max(1u, t.start[t.n]);
+        const unsigned int grid = std::max(1u, in_place ? (t.start[t.n] + kInPlace - 1) / kInPlace : t.start[t.n]);
         const cudaError_t e = with_types(dtype, out_dtype, [&](auto D, auto O) {
             clip_kernel<decltype(D)::value, decltype(O)::value, N>
                 <<<grid, kThreads, 0, s>>>(t, in_place, sum, max_norm, eps, norm);

@@ -7,7 +7,8 @@
 // between passes travel through global memory (L2); the barrier between passes is the hardware's
 // cluster barrier, so there is nothing to spin on. Bound by latency: a warp loads kBatch steps of
 // 32 keys at once, and stretches of one batch stay in registers for the second walk. Lanes with equal
-// digits are found by a vote per bit: match.any made 65536 keys of 7 bits take 23 us, votes @SORT@.
+// digits are found by a vote per bit, all in flight together (65536 keys of 7 bits: 23 us with
+// match.any, 19 with votes in a loop, @SORT@ unrolled).
 #pragma once
 
 #include "kernels/ops_common.cuh"
@@ -36,39 +37,40 @@ struct KeySource {
     }
 };
 
-// The lanes of `valid` whose digit equals this lane's (which must be one of them).
-__device__ __forceinline__ unsigned int same_digit(unsigned int d, int bits, unsigned int valid) {
-    unsigned int same = valid;
+// The lanes of `valid` whose BITS-bit digit equals this lane's (which must be one of them).
+template <int BITS>
+__device__ __forceinline__ unsigned int same_digit(unsigned int d, unsigned int valid) {
+    unsigned int votes[BITS];
 #pragma unroll
-    for (int b = 0; b < kSortMaxBits; ++b) {
-        if (b >= bits) break;
-        const bool set = (d >> b) & 1;
-        const unsigned int votes = __ballot_sync(0xffffffffu, set);
-        same &= set ? votes : ~votes;
-    }
-    return same;
+    for (int b = 0; b < BITS; ++b) votes[b] = __ballot_sync(0xffffffffu, (d >> b) & 1);
+#pragma unroll
+    for (int b = 0; b < BITS; ++b) valid &= (d >> b) & 1 ? votes[b] : ~votes[b];
+    return valid;
 }
 
-// One pass over n elements by digit (key >> shift) & (2^bits - 1), blockDim.x == 1024. get(i) gives
-// {key, position}; put(place, key, position) stores it; totals(digit, first place) is called once
-// per digit by block 0. counters: shared memory, [warps][2^bits] and 2^bits + 32 words.
-template <typename Get, typename Put, typename Totals>
-__device__ __forceinline__ void sort_pass(unsigned int* counters, long long n, int shift, int bits, Get get, Put put,
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
+// One pass over n elements by digit (key >> shift) & (2^BITS - 1), blockDim.x == 1024. get(i) gives
+// {key, position}; put(place, key, position) stores it; totals(digit, first place) is called once per digit by block 0. counters: shared memory
+// of sort_smem(BITS) bytes. After the last pass other blocks' elements may still be on their way.
+template <int BITS, typename Get, typename Put, typename Totals>
+__device__ __forceinline__ void sort_pass(unsigned int* counters, long long n, int shift, bool last, Get get, Put put,
                                           Totals totals) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
-    const int nbins = 1 << bits, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int kBins = 1 << BITS;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rank = static_cast<int>(cluster.block_rank()), blocks = static_cast<int>(cluster.num_blocks());
-    const unsigned int mask = nbins - 1, lower = (1u << lane) - 1;
-    unsigned int* mine = counters + warp * nbins;
-    unsigned int* block_total = counters + kSortWarps * nbins;  // read by the other blocks
-    unsigned int* warp_total = block_total + nbins;
+    const unsigned int lower = (1u << lane) - 1;
+    unsigned int* mine = counters + warp * kBins;
+    unsigned int* block_total = counters + kSortWarps * kBins;  // read by the other blocks
+    unsigned int* start = block_total + kBins;                  // where this block's elements of a digit go
+    unsigned int* warp_total = start + kBins;
     const long long share = static_cast<long long>(kSortWarps) * blocks * 32;
     const long long per = (n + share - 1) / share * 32;
     const long long lo = min(n, (static_cast<long long>(rank) * kSortWarps + warp) * per), hi = min(n, lo + per);
 
-    for (int i = threadIdx.x; i < kSortWarps * nbins / 2; i += blockDim.x)
-        reinterpret_cast<uint2*>(counters)[i] = make_uint2(0, 0);
     uint2 held[kBatch];
     unsigned int equal[kBatch];
     auto load = [&](long long i0) {
@@ -79,16 +81,17 @@ __device__ __forceinline__ void sort_pass(unsigned int* counters, long long n, i
         }
     };
     load(lo);
+    for (int i = threadIdx.x; i < kSortWarps * kBins / 4; i += blockDim.x)
+        reinterpret_cast<uint4*>(counters)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     for (long long i0 = lo; i0 < hi; i0 += kBatch * 32) {
         if (i0 != lo) load(i0);
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
-            const long long base = i0 + b * 32;
-            if (base >= hi) break;
-            const bool in = base + lane < hi;
-            const unsigned int d = (held[b].x >> shift) & mask;
-            equal[b] = same_digit(d, bits, __ballot_sync(0xffffffffu, in));
+            if (i0 + b * 32 >= hi) break;
+            const bool in = i0 + b * 32 + lane < hi;
+            const unsigned int d = (held[b].x >> shift) & (kBins - 1);
+            equal[b] = same_digit<BITS>(d, __ballot_sync(0xffffffffu, in));
             if (in && (equal[b] & lower) == 0) mine[d] += __popc(equal[b]);
             __syncwarp();
         }
@@ -97,13 +100,13 @@ __device__ __forceinline__ void sort_pass(unsigned int* counters, long long n, i
     // A thread per digit: counts of the warps before each warp, the block's total, the blocks' totals.
     const int d = threadIdx.x;
     unsigned int before = 0, all = 0;
-    if (d < nbins) {
+    if (d < kBins) {
         unsigned int c[kSortWarps];
 #pragma unroll
-        for (int w = 0; w < kSortWarps; ++w) c[w] = counters[w * nbins + d];
+        for (int w = 0; w < kSortWarps; ++w) c[w] = counters[w * kBins + d];
 #pragma unroll
         for (int w = 0; w < kSortWarps; ++w) {
-            counters[w * nbins + d] = all;
+            counters[w * kBins + d] = all;
             all += c[w];
         }
         block_total[d] = all;
@@ -111,7 +114,7 @@ __device__ __forceinline__ void sort_pass(unsigned int* counters, long long n, i
     if (blocks > 1) {
         cluster.sync();
         all = 0;
-        if (d < nbins) {
+        if (d < kBins) {
 #pragma unroll 8
             for (int b = 0; b < blocks; ++b) {
                 const unsigned int c = cluster.map_shared_rank(block_total, b)[d];
@@ -119,6 +122,7 @@ __device__ __forceinline__ void sort_pass(unsigned int* counters, long long n, i
                 all += c;
             }
         }
+        cluster_arrive_relaxed();  // done with the other blocks' totals
     }
     // Exclusive sum over the digits.
     unsigned int incl = all;
@@ -133,10 +137,9 @@ __device__ __forceinline__ void sort_pass(unsigned int* counters, long long n, i
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) first += __shfl_xor_sync(0xffffffffu, first, o);
     first += incl - all;
-    if (d < nbins) {
+    if (d < kBins) {
         if (rank == 0) totals(static_cast<unsigned int>(d), first);
-#pragma unroll
-        for (int w = 0; w < kSortWarps; ++w) counters[w * nbins + d] += first + before;
+        start[d] = first + before;
     }
     __syncthreads();
     for (long long i0 = lo; i0 < hi; i0 += kBatch * 32) {
@@ -144,26 +147,36 @@ __device__ __forceinline__ void sort_pass(unsigned int* counters, long long n, i
         if (again) load(i0);
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
-            const long long base = i0 + b * 32;
-            if (base >= hi) break;
-            const bool in = base + lane < hi;
-            const unsigned int dg = (held[b].x >> shift) & mask;
-            if (again) equal[b] = same_digit(dg, bits, __ballot_sync(0xffffffffu, in));
+            if (i0 + b * 32 >= hi) break;
+            const bool in = i0 + b * 32 + lane < hi;
+            const unsigned int dg = (held[b].x >> shift) & (kBins - 1);
+            if (again) equal[b] = same_digit<BITS>(dg, __ballot_sync(0xffffffffu, in));
             const unsigned int at = mine[dg];
             __syncwarp();
             if (in && (equal[b] & lower) == 0) mine[dg] = at + __popc(equal[b]);
             __syncwarp();
-            if (in) put(at + __popc(equal[b] & lower), held[b].x, held[b].y);
+            if (in) put(start[dg] + at + __popc(equal[b] & lower), held[b].x, held[b].y);
         }
     }
-    // The next pass reads what all blocks wrote; and no block may leave, or reuse its totals,
-    // while another reads them.
-    if (blocks > 1) cluster.sync();
-    else __syncthreads();
+    if (blocks > 1) {
+        cluster_wait();             // nobody reads this block's totals any more
+        if (!last) cluster.sync();  // the next pass reads what all blocks wrote
+    } else if (!last) {
+        __syncthreads();
+    }
 }
 
 inline size_t sort_smem(int bits) {
-    return sizeof(unsigned int) * (static_cast<size_t>(kSortWarps + 1) * (1u << bits) + kSortWarps);
+    return sizeof(unsigned int) * (static_cast<size_t>(kSortWarps + 2) * (1u << bits) + kSortWarps);
+}
+
+// Digit widths that kernels exist for (votes are unrolled), and the one to use for `bits`.
+template <typename F>
+cudaError_t with_bits(int bits, F&& f) {
+    if (bits <= 4) return f(Int<4>{});
+    if (bits <= 7) return f(Int<7>{});
+    if (bits <= 9) return f(Int<9>{});
+    return f(Int<10>{});
 }
 
 // Launches a kernel that sorts n elements by sort_pass: one block while it holds them in registers,

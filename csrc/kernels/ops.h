@@ -53,7 +53,7 @@ struct EmbeddingArgs {
 };
 cudaError_t LaunchEmbeddingForward(const EmbeddingArgs& a, const void* table, long long table_stride, float scale,
                                    void* out, long long out_stride, int dtype, cudaStream_t stream);
-size_t EmbeddingBackwardWorkspace(long long n, long long rows, long long h);
+size_t EmbeddingBackwardWorkspace(long long n, long long h);
 cudaError_t LaunchEmbeddingBackward(const EmbeddingArgs& a, const void* dy, long long dy_stride, void* dtable,
                                     float scale, long long skip, bool has_skip, bool accumulate, int dtype,
                                     int out_dtype, void* workspace, cudaStream_t stream);
