@@ -165,16 +165,23 @@ bool ExpertShape(int64_t tokens, int top) {
 bool Experts(int experts) { return experts >= 1 && experts <= BCCL_MAX_EXPERTS; }
 }  // namespace
 
+size_t bcclExpertSortWorkspace(int64_t tokens, int top) {
+    return ExpertShape(tokens, top) ? bccl::ExpertSortWorkspace(tokens * top) : 0;
+}
+
 int bcclExpertSort(const void* ids, int ids_dtype, int64_t tokens, int top, int experts, int32_t* slots, int32_t* sources,
-                   int32_t* offsets, void* stream) {
+                   int32_t* offsets, void* workspace, size_t workspace_bytes, void* stream) {
     const char* op = "expert sort";
     if (!IndexType(ids_dtype)) return Bad(op, "ids are int32 or int64");
     if (!ExpertShape(tokens, top) || !Experts(experts)) return Bad(op, "invalid shape (top <= 64, experts <= 1023)");
     if (offsets == nullptr || (tokens > 0 && (ids == nullptr || slots == nullptr || sources == nullptr ||
                                               !Aligned(ids, SizeOf(ids_dtype)))))
         return Bad(op, "null or misaligned array");
+    const size_t need = bccl::ExpertSortWorkspace(tokens * top);
+    if (need > 0 && (workspace == nullptr || !Aligned(workspace, 16) || workspace_bytes < need))
+        return Bad(op, "workspace too small or misaligned");
     return Launched(op, bccl::LaunchExpertSort(ids, ids_dtype == kI64, tokens * top, experts, slots, sources, offsets,
-                                               Stream(stream)));
+                                               workspace, Stream(stream)));
 }
 
 int bcclExpertDispatch(const void* x, int64_t x_stride, const int32_t* slots, const int32_t* offsets, int64_t tokens,

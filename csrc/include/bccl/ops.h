@@ -76,8 +76,9 @@ int bcclEmbeddingBackward(const void* dy, int64_t dy_stride, const void* ids, in
  * (0: dropped). The gradient of dispatch is a combine without weights. */
 #define BCCL_MAX_EXPERTS 1023
 #define BCCL_MAX_TOP 64
+size_t bcclExpertSortWorkspace(int64_t tokens, int top);
 int bcclExpertSort(const void* ids, int ids_dtype, int64_t tokens, int top, int experts, int32_t* slots, int32_t* sources,
-                   int32_t* offsets, void* stream);
+                   int32_t* offsets, void* workspace, size_t workspace_bytes, void* stream);
 int bcclExpertDispatch(const void* x, int64_t x_stride, const int32_t* slots, const int32_t* offsets, int64_t tokens,
                        int top, int experts, int64_t h, void* rows, int dtype, void* stream);
 int bcclExpertCombine(const void* rows, const int32_t* slots, const void* weights, int wdtype, int64_t tokens, int top,

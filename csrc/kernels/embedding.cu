@@ -2,7 +2,8 @@
 //
 //   out[i] = scale * table[ids[i] - first],  dtable[v] = scale * sum of dy[i] over ids[i] == first + v
 //
-// Gradient, three launches. (1) One cluster sorts the positions by token (key_sort.cuh). (2) The sorted positions are cut into windows of equal length, so a token
+// Gradient, three launches. (1) The positions are sorted by token (key_sort.cuh; more launches for
+// more than 32768). (2) The sorted positions are cut into windows of equal length, so a token
 // that is everywhere is summed by many blocks: a block adds the rows of its window in order and
 // writes every token that lies wholly in it; the part of a token that runs over the window's
 // edge goes to a 32-bit partial row. The same launch writes zeros to the rows that do not occur.
@@ -54,16 +55,19 @@ __global__ void __launch_bounds__(kThreads) lookup_kernel(const KeySource key, l
     }
 }
 
-// Writes {row, position} of the n positions to b, by row; a is the other buffer between passes.
-template <int BITS>
-__global__ void __launch_bounds__(1024) position_sort_kernel(const KeySource key, long long n, int passes, uint2* a, uint2* b) {
+// Writes {row, position} of the n positions to b, by row; a is the other buffer between passes. A
+// cluster does all passes; kCount and kPlace launches do pass `first` only.
+template <int BITS, SortMode MODE>
+__global__ void __launch_bounds__(1024) position_sort_kernel(const KeySource key, long long n, int first, int passes,
+                                                             unsigned int* grid_totals, uint2* a, uint2* b) {
     extern __shared__ unsigned int counters[];
-    for (int p = 0; p < passes; ++p) {
+    const int end = MODE == kCluster ? passes : first + 1;
+    for (int p = first; p < end; ++p) {
         // Buffers alternate so that the last pass writes b.
         uint2* to = ((passes - 1 - p) & 1) ? a : b;
         const uint2* from = to == a ? b : a;
-        sort_pass<BITS>(
-            counters, n, p * BITS, p == passes - 1,
+        sort_pass<BITS, MODE>(
+            counters, grid_totals, n, p * BITS, p == passes - 1,
             [&](long long i) {
                 return p == 0 ? make_uint2(key(i), static_cast<unsigned int>(i)) : __ldcg(from + i);
             },
@@ -237,12 +241,18 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const WindowArgs a, Bits
     if (c >= a.h) return;
     float sum[E];
     load_f<kF32, E>(reinterpret_cast<const Bits<kF32>*>(a.partial + (w * 2 + 1) * a.h + c), sum);
-#pragma unroll 4
-    for (long long k = w + 1; k <= lo; ++k) {
-        float f[E];
-        load_f<kF32, E>(reinterpret_cast<const Bits<kF32>*>(a.partial + k * 2 * a.h + c), f);
+    for (long long k0 = w + 1; k0 <= lo; k0 += kFlight) {
+        float f[kFlight][E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) sum[e] += f[e];
+        for (int u = 0; u < kFlight; ++u)
+            if (k0 + u <= lo)
+                load_f<kF32, E>(reinterpret_cast<const Bits<kF32>*>(a.partial + (k0 + u) * 2 * a.h + c), f[u]);
+#pragma unroll
+        for (int u = 0; u < kFlight; ++u) {
+            if (k0 + u > lo) break;
+#pragma unroll
+            for (int e = 0; e < E; ++e) sum[e] += f[u][e];
+        }
     }
     write_row<OD, E>(dtable + row * a.h + c, sum, a.scale, a.accumulate != 0);
 }
@@ -290,7 +300,7 @@ cudaError_t LaunchEmbeddingForward(const EmbeddingArgs& a, const void* table, lo
 size_t EmbeddingBackwardWorkspace(long long n, long long h) {
     using namespace ops;
     const long long windows = ceil_div(n, window_of(n));
-    return 2 * align16(sizeof(uint2) * static_cast<size_t>(n)) +
+    return 2 * align16(sizeof(uint2) * static_cast<size_t>(n)) + align16(sizeof(unsigned int) * sort_totals(n)) +
            align16(sizeof(float) * 2 * static_cast<size_t>(windows) * static_cast<size_t>(h));
 }
 
@@ -308,6 +318,8 @@ cudaError_t LaunchEmbeddingBackward(const EmbeddingArgs& a, const void* dy, long
     ws += align16(sizeof(uint2) * static_cast<size_t>(a.n));
     uint2* buf_b = reinterpret_cast<uint2*>(ws);
     ws += align16(sizeof(uint2) * static_cast<size_t>(a.n));
+    unsigned int* totals = reinterpret_cast<unsigned int*>(ws);
+    ws += align16(sizeof(unsigned int) * sort_totals(a.n));
     float* partial = reinterpret_cast<float*>(ws);
 
     int key_bits = 1;
@@ -317,7 +329,18 @@ cudaError_t LaunchEmbeddingBackward(const EmbeddingArgs& a, const void* dy, long
     const KeySource key{a.ids, a.ids64, a.first, a.rows, skip, has_skip ? 1 : 0};
     const cudaError_t e = with_bits(bits, [&](auto B) {
         constexpr int kB = decltype(B)::value;
-        return launch_sort(position_sort_kernel<kB>, a.n, kB, stream, key, a.n, passes, buf_a, buf_b);
+        if (a.n <= kClusterSort)
+            return launch_sort(position_sort_kernel<kB, kCluster>, true, a.n, kB, stream, key, a.n, 0, passes, totals, buf_a,
+                               buf_b);
+        for (int p = 0; p < passes; ++p) {
+            cudaError_t err = launch_sort(position_sort_kernel<kB, kCount>, false, a.n, kB, stream, key, a.n, p, passes, totals,
+                                          buf_a, buf_b);
+            if (err == cudaSuccess)
+                err = launch_sort(position_sort_kernel<kB, kPlace>, false, a.n, kB, stream, key, a.n, p, passes, totals, buf_a,
+                                  buf_b);
+            if (err != cudaSuccess) return err;
+        }
+        return cudaSuccess;
     });
     if (e != cudaSuccess) return e;
 

@@ -19,13 +19,13 @@ namespace ops {
 namespace {
 
 // One pass: the digits are the experts themselves and `experts` for dropped assignments.
-template <int BITS>
-__global__ void __launch_bounds__(1024) expert_sort_kernel(const KeySource key, long long n, int* slots, int* sources,
-                                                           int* offsets) {
+template <int BITS, SortMode MODE>
+__global__ void __launch_bounds__(1024) expert_sort_kernel(const KeySource key, long long n, unsigned int* grid_totals,
+                                                           int* slots, int* sources, int* offsets) {
     extern __shared__ unsigned int counters[];
     const unsigned int experts = static_cast<unsigned int>(key.bins);
-    sort_pass<BITS>(
-        counters, n, 0, true, [&](long long i) { return make_uint2(key(i), static_cast<unsigned int>(i)); },
+    sort_pass<BITS, MODE>(
+        counters, grid_totals, n, 0, true, [&](long long i) { return make_uint2(key(i), static_cast<unsigned int>(i)); },
         [&](unsigned int place, unsigned int k, unsigned int a) {
             slots[a] = k < experts ? static_cast<int>(place) : -1;
             sources[place] = k < experts ? static_cast<int>(a) : -1;
@@ -164,8 +164,10 @@ int token_threads(long long h, int e, int most) {
 }  // namespace
 }  // namespace ops
 
+size_t ExpertSortWorkspace(long long n) { return sizeof(unsigned int) * ops::sort_totals(n); }
+
 cudaError_t LaunchExpertSort(const void* ids, int ids64, long long n, int experts, int* slots, int* sources,
-                             int* offsets, cudaStream_t stream) {
+                             int* offsets, void* workspace, cudaStream_t stream) {
     using namespace ops;
     if (n == 0) return cudaMemsetAsync(offsets, 0, sizeof(int) * (experts + 1), stream);
     int bits = 1;
@@ -173,7 +175,13 @@ cudaError_t LaunchExpertSort(const void* ids, int ids64, long long n, int expert
     const KeySource key{ids, ids64, 0, experts, 0, 0};
     return with_bits(bits, [&](auto B) {
         constexpr int kB = decltype(B)::value;
-        return launch_sort(expert_sort_kernel<kB>, n, kB, stream, key, n, slots, sources, offsets);
+        unsigned int* totals = static_cast<unsigned int*>(workspace);
+        if (n <= kClusterSort)
+            return launch_sort(expert_sort_kernel<kB, kCluster>, true, n, kB, stream, key, n, totals, slots, sources, offsets);
+        const cudaError_t e =
+            launch_sort(expert_sort_kernel<kB, kCount>, false, n, kB, stream, key, n, totals, slots, sources, offsets);
+        if (e != cudaSuccess) return e;
+        return launch_sort(expert_sort_kernel<kB, kPlace>, false, n, kB, stream, key, n, totals, slots, sources, offsets);
     });
 }
 

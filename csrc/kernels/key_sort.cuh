@@ -1,19 +1,27 @@
-// Stable sort of small integer keys by one thread-block cluster, one launch.
+// Stable sort of small integer keys.
 //
-// Radix sort from the lowest digit. The cluster's warps own consecutive stretches of the input. A
-// pass counts each warp's digits in shared memory, adds the counts up over warps, blocks (through
-// distributed shared memory) and digits, and then every warp walks its stretch in order again and
-// writes each element to its place: equal digits keep their order, whatever the timing. Elements
-// between passes travel through global memory (L2); the barrier between passes is the hardware's
-// cluster barrier, so there is nothing to spin on. Bound by latency: a warp loads kBatch steps of
-// 32 keys at once, and stretches of one batch stay in registers for the second walk. Lanes with equal
-// digits are found by a vote per bit, all in flight together (65536 keys of 7 bits: 23 us with
-// match.any, 19 with votes in a loop, 16 us unrolled).
+// Radix sort from the lowest digit. Warps own consecutive stretches of the input. A pass counts each
+// warp's digits in shared memory, adds the counts up over warps, blocks and digits, and then every
+// warp walks its stretch in order again and writes each element to its place: equal digits keep their
+// order, whatever the timing. Elements between passes travel through global memory (L2).
+//
+// Up to 32768 elements one thread-block cluster does all passes in one launch: blocks read each other's
+// totals through distributed shared memory, and the barrier between passes is the hardware's cluster
+// barrier, so there is nothing to spin on. More elements get two launches per pass over up to 128 blocks
+// (count, then place), with the totals in global memory: 800000 keys of 4 bits take @BIG@ that way and 144 us
+// on a cluster.
+//
+// Bound by latency: a warp loads kBatch steps of 32 keys at once, and stretches of one batch stay in
+// registers for the second walk. Lanes with equal digits are found by a vote per bit, all in flight
+// together (65536 keys of 7 bits on a cluster: 23 us with match.any, 19 with votes in a loop, 16 unrolled);
+// the votes are two thirds of the counting.
 #pragma once
 
 #include "kernels/ops_common.cuh"
 
 #include <cooperative_groups.h>
+
+#include <algorithm>
 
 namespace bccl {
 namespace ops {
@@ -48,20 +56,26 @@ __device__ __forceinline__ unsigned int same_digit(unsigned int d, unsigned int 
     return valid;
 }
 
+// How the blocks of a pass learn of each other's totals. kCount ends a pass after writing them to
+// global memory, kPlace takes them from there.
+enum SortMode { kCluster, kCount, kPlace };
+
 __device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 
 // One pass over n elements by digit (key >> shift) & (2^BITS - 1), blockDim.x == 1024. get(i) gives
-// {key, position}; put(place, key, position) stores it; totals(digit, first place) is called once per digit by block 0. counters: shared memory
-// of sort_smem(BITS) bytes. After the last pass other blocks' elements may still be on their way.
-template <int BITS, typename Get, typename Put, typename Totals>
-__device__ __forceinline__ void sort_pass(unsigned int* counters, long long n, int shift, bool last, Get get, Put put,
-                                          Totals totals) {
+// {key, position}; put(place, key, position) stores it; totals(digit, first place) is called once
+// per digit by block 0. counters: shared memory of sort_smem(BITS) bytes. grid_totals ([blocks][2^BITS], not
+// for kCluster). After the last pass other blocks' elements may still be on their way.
+template <int BITS, SortMode MODE, typename Get, typename Put, typename Totals>
+__device__ __forceinline__ void sort_pass(unsigned int* counters, unsigned int* grid_totals, long long n, int shift,
+                                          bool last, Get get, Put put, Totals totals) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     constexpr int kBins = 1 << BITS;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int rank = static_cast<int>(cluster.block_rank()), blocks = static_cast<int>(cluster.num_blocks());
+    const int rank = MODE == kCluster ? static_cast<int>(cluster.block_rank()) : static_cast<int>(blockIdx.x);
+    const int blocks = MODE == kCluster ? static_cast<int>(cluster.num_blocks()) : static_cast<int>(gridDim.x);
     const unsigned int lower = (1u << lane) - 1;
     unsigned int* mine = counters + warp * kBins;
     unsigned int* block_total = counters + kSortWarps * kBins;  // read by the other blocks
@@ -110,8 +124,20 @@ __device__ __forceinline__ void sort_pass(unsigned int* counters, long long n, i
             all += c[w];
         }
         block_total[d] = all;
+        if constexpr (MODE == kCount) grid_totals[rank * kBins + d] = all;
     }
-    if (blocks > 1) {
+    if constexpr (MODE == kCount) return;
+    if constexpr (MODE == kPlace) {
+        all = 0;
+        if (d < kBins) {
+#pragma unroll 16
+            for (int b = 0; b < blocks; ++b) {
+                const unsigned int c = __ldg(grid_totals + b * kBins + d);
+                if (b < rank) before += c;
+                all += c;
+            }
+        }
+    } else if (blocks > 1) {
         cluster.sync();
         all = 0;
         if (d < kBins) {
@@ -158,6 +184,7 @@ __device__ __forceinline__ void sort_pass(unsigned int* counters, long long n, i
             if (in) put(start[dg] + at + __popc(equal[b] & lower), held[b].x, held[b].y);
         }
     }
+    if (MODE == kPlace) return;
     if (blocks > 1) {
         cluster_wait();             // nobody reads this block's totals any more
         if (!last) cluster.sync();  // the next pass reads what all blocks wrote
@@ -179,16 +206,25 @@ cudaError_t with_bits(int bits, F&& f) {
     return f(Int<10>{});
 }
 
-// Launches a kernel that sorts n elements by sort_pass: one block while a warp has at most two steps,
-// else a cluster of 8 (the largest that every GPU guarantees).
+constexpr long long kClusterSort = 32768;  // elements that a cluster sorts in one launch
+
+// Blocks of the launches for more elements: 2048 each while that is no more than 128.
+inline int sort_grid(long long n) { return static_cast<int>(std::min(128ll, ceil_div(n, 2048))); }
+// Words of grid_totals that sorting n elements needs.
+inline size_t sort_totals(long long n) {
+    return n <= kClusterSort ? 0 : static_cast<size_t>(sort_grid(n)) << kSortMaxBits;
+}
+
+// Launches a kernel of sort passes: by a cluster (one block while a warp has at most two steps, else 8,
+// the most that every GPU guarantees), or by the blocks of sort_grid.
 template <typename... Params, typename... Args>
-cudaError_t launch_sort(void (*kernel)(Params...), long long n, int bits, cudaStream_t stream, Args... args) {
+cudaError_t launch_sort(void (*kernel)(Params...), bool by_cluster, long long n, int bits, cudaStream_t stream, Args... args) {
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = n <= kSortWarps * 2 * 32 ? 1 : 8;
+    attr[0].val.clusterDim.x = !by_cluster || n <= kSortWarps * 2 * 32 ? 1 : 8;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(attr[0].val.clusterDim.x);
+    cfg.gridDim = dim3(by_cluster ? attr[0].val.clusterDim.x : sort_grid(n));
     cfg.blockDim = dim3(kSortWarps * 32);
     cfg.dynamicSmemBytes = sort_smem(bits);
     cfg.stream = stream;

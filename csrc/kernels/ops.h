@@ -58,8 +58,9 @@ cudaError_t LaunchEmbeddingBackward(const EmbeddingArgs& a, const void* dy, long
                                     float scale, long long skip, bool has_skip, bool accumulate, int dtype,
                                     int out_dtype, void* workspace, cudaStream_t stream);
 
+size_t ExpertSortWorkspace(long long n);
 cudaError_t LaunchExpertSort(const void* ids, int ids64, long long n, int experts, int* slots, int* sources,
-                             int* offsets, cudaStream_t stream);
+                             int* offsets, void* workspace, cudaStream_t stream);
 cudaError_t LaunchExpertDispatch(const void* x, long long x_stride, const int* slots, const int* offsets,
                                  long long tokens, int top, int experts, long long h, void* rows, int dtype,
                                  cudaStream_t stream);

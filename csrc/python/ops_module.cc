@@ -363,10 +363,12 @@ PyObject* ExpertSort(PyObject* const* a) {
     const auto i32 = ids.options().dtype(at::kInt);
     const Tensor slots = at::empty({tokens, top}, i32), sources = at::empty({tokens * top}, i32),
                  offsets = at::empty({experts + 1}, i32);
+    const size_t size = bcclExpertSortWorkspace(tokens, static_cast<int>(top));
+    const Optional ws = size > 0 ? Optional(bytes(ids, size)) : std::nullopt;
     launch(device, [&](void* s) {
         return bcclExpertSort(data(i), icode, tokens, static_cast<int>(top), static_cast<int>(experts),
                               static_cast<int32_t*>(data(slots)), static_cast<int32_t*>(data(sources)),
-                              static_cast<int32_t*>(data(offsets)), s);
+                              static_cast<int32_t*>(data(offsets)), data(ws), size, s);
     });
     return wrap_all(slots, sources, offsets);
 }

@@ -107,7 +107,8 @@ def load(path: Path | None = None) -> ctypes.CDLL:
         "bcclEmbeddingBackwardWorkspace": (c_size, [i64, i64, i64]),
         "bcclEmbeddingBackward": (c_int, [vp, i64, vp, c_int, i64, vp, i64, i64, i64, c_float, i64, c_int, c_int, c_int,
                                           c_int, vp, c_size, vp]),
-        "bcclExpertSort": (c_int, [vp, c_int, i64, c_int, c_int, vp, vp, vp, vp]),
+        "bcclExpertSortWorkspace": (c_size, [i64, c_int]),
+        "bcclExpertSort": (c_int, [vp, c_int, i64, c_int, c_int, vp, vp, vp, vp, c_size, vp]),
         "bcclExpertDispatch": (c_int, [vp, i64, vp, vp, i64, c_int, c_int, i64, vp, c_int, vp]),
         "bcclExpertCombine": (c_int, [vp, vp, vp, c_int, i64, c_int, i64, vp, i64, c_int, vp]),
         "bcclExpertCombineBackward": (c_int, [vp, i64, vp, vp, vp, vp, c_int, i64, c_int, c_int, i64, vp, vp, c_int, vp]),

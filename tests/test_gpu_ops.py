@@ -218,7 +218,7 @@ def some_ids(n, vocab, kind, seed, dtype=torch.int64):
     (1, 1, 1, "flat"), (1, 70000, 8, "flat"), (5, 3, 33, "flat"), (64, 1024, 256, "flat"), (777, 1023, 250, "skewed"),
     (4096, 1024, 64, "skewed"), (4097, 1025, 40, "skewed"), (9000, 128256, 16, "skewed"), (20000, 50, 24, "same"),
     (70001, 300, 9, "skewed"), (3000, 2000, 264, "far"), (300, 1100000, 8, "skewed"), (2049, 600, 3000, "skewed"),
-    (16, 10, 2 ** 15 + 8, "flat")])
+    (16, 10, 2 ** 15 + 8, "flat"), (32768, 3000, 8, "skewed"), (32769, 1 << 21, 8, "flat"), (300001, 70000, 4, "far")])
 def test_embedding(dtype, n, vocab, h, kind):
     from originccl_b200.ops import embedding
     for itype in (torch.int64, torch.int32):
@@ -333,7 +333,8 @@ def order64(ids, experts):
 
 @pytest.mark.parametrize("tokens,top,experts,kind", [
     (1, 1, 1, "flat"), (8, 2, 8, "flat"), (33, 3, 7, "far"), (1000, 1, 5, "skewed"), (4096, 1, 64, "skewed"),
-    (700, 64, 100, "flat"), (2049, 2, 1023, "skewed"), (9001, 8, 33, "far"), (3000, 2, 4, "none"), (500, 2, 9, "same")])
+    (700, 64, 100, "flat"), (2049, 2, 1023, "skewed"), (9001, 8, 33, "far"), (3000, 2, 4, "none"), (500, 2, 9, "same"),
+    (16384, 2, 64, "skewed"), (16385, 2, 1000, "far"), (100003, 3, 11, "skewed")])
 def test_expert_order(tokens, top, experts, kind):
     from originccl_b200.ops import experts as ex
     for itype in (torch.int32, torch.int64):

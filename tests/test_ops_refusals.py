@@ -215,10 +215,15 @@ def test_the_c_interface_refuses():
     refused(embb(od=5), "dtypes")
     refused(embb(n=-1), "shape")
 
-    refused(lib.bcclExpertSort(p(64), 2, 4, 65, 8, p(64), p(64), p(64), None), "shape")
-    refused(lib.bcclExpertSort(p(64), 2, 4, 2, 1024, p(64), p(64), p(64), None), "shape")
-    refused(lib.bcclExpertSort(p(64), 2, (1 << 31) // 2, 2, 8, p(64), p(64), p(64), None), "shape")
-    refused(lib.bcclExpertSort(p(64), 2, 4, 2, 8, p(0), p(64), p(64), None), "null")
+    def sort(tokens=4, top=2, experts=8, slots=64, ws=64, size=1 << 30):
+        return lib.bcclExpertSort(p(64), 2, tokens, top, experts, p(slots), p(64), p(64), p(ws), size, None)
+    refused(sort(top=65), "shape")
+    refused(sort(experts=1024), "shape")
+    refused(sort(tokens=1 << 30), "shape")
+    refused(sort(slots=0), "null")
+    assert lib.bcclExpertSortWorkspace(4, 2) == 0
+    refused(sort(tokens=1 << 20, size=lib.bcclExpertSortWorkspace(1 << 20, 2) - 1), "workspace")
+    refused(sort(tokens=1 << 20, ws=0), "workspace")
     refused(lib.bcclExpertDispatch(p(64), 8, p(64), p(64), 4, 2, 8, 0, p(64), 0, None), "shape")
     refused(lib.bcclExpertDispatch(p(66), 8, p(64), p(64), 4, 2, 8, 8, p(64), 0, None), "misaligned")
     refused(lib.bcclExpertCombine(p(64), p(64), p(64), 4, 4, 2, 8, p(64), 8, 0, None), "dtypes")
