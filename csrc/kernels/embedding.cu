@@ -21,35 +21,47 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// A block copies its columns of TOKENS rows, all in flight at once: a row cannot be asked for before
-// its id is there, so one row per block leaves the memory idle (32768 rows of 8 KiB: 97 us with one).
-template <int D, int E, int TOKENS>
-__global__ void __launch_bounds__(kThreads) lookup_kernel(const KeySource key, long long n, const Bits<D>* __restrict__ table,
-                                                          long long table_stride, long long h, float scale,
+// A thread copies its columns of TOKENS rows, all in flight at once: a row cannot be asked for before
+// its id is there, so one row at a time leaves the memory idle (32768 rows of 8 KiB: 97 us, with four 63).
+// blockDim (x, y): columns, groups of TOKENS rows.
+template <int D, bool ODD, int TOKENS>
+__global__ void __launch_bounds__(kThreads, ODD ? 3 : 6) lookup_kernel(const KeySource key, long long n, const Bits<D>* __restrict__ table,
+                                                          long long table_stride, int h, float scale,
                                                           Bits<D>* __restrict__ out, long long out_stride) {
-    const long long c = (static_cast<long long>(blockIdx.y) * blockDim.x + threadIdx.x) * E;
-    if (c >= h) return;
-    for (long long i0 = static_cast<long long>(blockIdx.x) * TOKENS; i0 < n; i0 += static_cast<long long>(gridDim.x) * TOKENS) {
+    constexpr int E = Vec<D>::E;
+    const int j = blockIdx.y * blockDim.x + threadIdx.x;
+    if (!ODD && j * E >= h) return;
+    const long long step = static_cast<long long>(gridDim.x) * blockDim.y * TOKENS;
+    for (long long i0 = (static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y) * TOKENS; i0 < n; i0 += step) {
         unsigned int row[TOKENS];
         Raw<D, E> r[TOKENS];
 #pragma unroll
         for (int t = 0; t < TOKENS; ++t)
             row[t] = i0 + t < n ? key(i0 + t) : static_cast<unsigned int>(key.bins);
 #pragma unroll
-        for (int t = 0; t < TOKENS; ++t)
-            r[t] = row[t] < key.bins ? load_raw<D, E>(table + row[t] * table_stride + c) : zero_raw<D, E>();
+        for (int t = 0; t < TOKENS; ++t) {
+            if constexpr (!ODD) {
+                r[t] = row[t] < key.bins ? load_raw<D, E>(table + row[t] * table_stride + j * E) : zero_raw<D, E>();
+            } else {
+                const int c = j * E - shift_of<ODD, D>(out + (i0 + t) * out_stride);
+                r[t] = zero_raw<D, E>();
+                if (row[t] < key.bins && c < h) r[t] = get_row<ODD, D>(table + row[t] * table_stride, c, h);
+            }
+        }
 #pragma unroll
         for (int t = 0; t < TOKENS; ++t) {
+            Bits<D>* to = out + (i0 + t) * out_stride;
+            const int c = j * E - shift_of<ODD, D>(to);
             if (i0 + t >= n) break;
-            Bits<D>* to = out + (i0 + t) * out_stride + c;
+            if (ODD && c >= h) continue;
             if (scale == 1.0f) {
-                store_raw_cs<D, E>(to, r[t]);
+                put_raw<ODD, D>(to, c, h, r[t]);
             } else {
                 float f[E];
                 unpack<D, E>(r[t], f);
 #pragma unroll
                 for (int e = 0; e < E; ++e) f[e] = row[t] < key.bins ? f[e] * scale : 0.0f;
-                store_f_cs<D, E>(to, f);
+                put_row<ODD, D, E>(to, c, h, f);
             }
         }
     }
@@ -76,30 +88,30 @@ __global__ void __launch_bounds__(1024) position_sort_kernel(const KeySource key
     }
 }
 
-template <int OD, int E>
-__device__ __forceinline__ void write_row(Bits<OD>* p, const float (&sum)[E], float scale, bool accumulate) {
+// Columns [c, c + E) of a row of the table's gradient.
+template <int OD, int E, bool ODD>
+__device__ __forceinline__ void write_row(Bits<OD>* row, int c, int h, const float (&sum)[E], float scale, bool accumulate) {
     float f[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] = sum[e] * scale;
     if (accumulate) {
         // Plain loads: this kernel writes the array they read.
-        if constexpr (E == 1) {
-            f[0] = Ty<OD>::load(*p);
-        } else {
+        if (!ODD || (c >= 0 && c + E <= h)) {
             constexpr int W = Vec<OD>::E;
 #pragma unroll
             for (int i = 0; i < E / W; ++i) {
                 float t[W];
-                Vec<OD>::unpack(*(reinterpret_cast<const uint4*>(p) + i), t);
+                Vec<OD>::unpack(*(reinterpret_cast<const uint4*>(row + c) + i), t);
 #pragma unroll
-                for (int e = 0; e < W; ++e) f[i * W + e] = t[e];
+                for (int e = 0; e < W; ++e) f[i * W + e] = fmaf(sum[i * W + e], scale, t[e]);
             }
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (c + e >= 0 && c + e < h) f[e] = fmaf(sum[e], scale, Ty<OD>::load(row[c + e]));
         }
-#pragma unroll
-        for (int e = 0; e < E; ++e) f[e] = fmaf(sum[e], scale, f[e]);
-    } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) f[e] = sum[e] * scale;
     }
-    store_f_cs<OD, E>(p, f);
+    put_row<ODD, OD, E>(row, c, h, f);
 }
 
 constexpr int kMaxWindow = 128;
@@ -107,13 +119,16 @@ constexpr int kFlight = 8;  // rows of dy in flight per thread
 
 struct WindowArgs {
     const uint2* sorted;
-    long long n, rows, h;
+    long long n, rows;
+    int h;
     int window;
     long long windows;
-    float* partial;  // [windows][2][h]: a token that came from the left; one that goes on to the right
+    float* partial;      // [windows][2][width]: a token that came from the left; one that goes on to the right
+    long long width;     // by accesses: columns of a row begin at its shift
     float scale;
     int accumulate;
-    int tile;  // rows that a block clears at a time
+    int tile;            // rows that a block clears at a time
+    int window_blocks;   // blocks of windows, the others clear
 };
 
 constexpr int kMaxTile = 4096;
@@ -131,65 +146,75 @@ __device__ __forceinline__ long long first_of(const uint2* sorted, long long n, 
 // Zeros for the rows of the table that do not occur among the sorted positions. The positions of a
 // tile's rows set bits in shared memory. (Marking rows while sorting took longer than the sort: thousands
 // of stores to the byte of a frequent token.)
-template <int OD, int E>
-__device__ __forceinline__ void clear_absent(const WindowArgs& a, long long c, Bits<OD>* dtable) {
+template <int OD, int E, bool ODD>
+__device__ __forceinline__ void clear_absent(const WindowArgs& a, int j, Bits<OD>* dtable) {
     __shared__ unsigned int present[kMaxTile / 32];
     __shared__ long long range[2];
+    const int id = threadIdx.y * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y;
     float zero[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) zero[e] = 0.0f;
     const long long tiles = (a.rows + a.tile - 1) / a.tile;
-    for (long long t = blockIdx.x - a.windows; t < tiles; t += gridDim.x - a.windows) {
+    for (long long t = static_cast<long long>(blockIdx.x) - a.window_blocks; t < tiles; t += gridDim.x - a.window_blocks) {
         const long long r0 = t * a.tile;
         const int count = static_cast<int>(min(static_cast<long long>(a.tile), a.rows - r0));
-        for (int i = threadIdx.x; i < (count + 31) / 32; i += blockDim.x) present[i] = 0;
-        if (threadIdx.x < 2) range[threadIdx.x] = first_of(a.sorted, a.n, threadIdx.x == 0 ? r0 : r0 + count);
+        for (int i = id; i < (count + 31) / 32; i += threads) present[i] = 0;
+        for (int i = id; i < 2; i += threads) range[i] = first_of(a.sorted, a.n, i == 0 ? r0 : r0 + count);
         __syncthreads();
-        for (long long i = range[0] + threadIdx.x; i < range[1]; i += blockDim.x) {
+        for (long long i = range[0] + id; i < range[1]; i += threads) {
             const unsigned int row = __ldg(&a.sorted[i].x);
             // A token's first position is enough.
             if (i == range[0] || __ldg(&a.sorted[i - 1].x) != row)
                 atomicOr(&present[(row - r0) >> 5], 1u << ((row - r0) & 31));
         }
         __syncthreads();
-        if (c < a.h) {
-            for (int r = 0; r < count; ++r)
-                if (!(present[r >> 5] >> (r & 31) & 1)) store_f_cs<OD, E>(dtable + (r0 + r) * a.h + c, zero);
+        for (int r = threadIdx.y; r < count; r += blockDim.y) {
+            if (present[r >> 5] >> (r & 31) & 1) continue;
+            Bits<OD>* row = dtable + (r0 + r) * a.h;
+            const int c = j * E - shift_of<ODD, OD>(row);
+            if (c < a.h) put_row<ODD, OD, E>(row, c, a.h, zero);
         }
         __syncthreads();
     }
 }
 
-// blockIdx.x < windows: a window of sorted positions; beyond: rows to clear. blockIdx.y: columns.
-template <int D, int OD, int E>
-__global__ void __launch_bounds__(kThreads) window_kernel(const WindowArgs a, const Bits<D>* __restrict__ dy,
+// blockDim (x, y): columns, windows. blockIdx.x < window_blocks: windows of sorted positions; beyond:
+// rows to clear. blockIdx.y: columns.
+template <int D, int OD, bool ODD>
+__global__ void __launch_bounds__(kThreads, ODD ? 3 : 4) window_kernel(const WindowArgs a, const Bits<D>* __restrict__ dy,
                                                           long long dy_stride, Bits<OD>* __restrict__ dtable) {
-    __shared__ uint2 item[kMaxWindow + 2];  // the window and its neighbours on either side
-    const long long c = (static_cast<long long>(blockIdx.y) * blockDim.x + threadIdx.x) * E;
-    if (blockIdx.x >= a.windows) {
-        clear_absent<OD, E>(a, c, dtable);
+    constexpr int E = Vec<D>::E;
+    extern __shared__ uint2 items[];  // [blockDim.y][window + 2]: the windows and their neighbours on either side
+    const int j = blockIdx.y * blockDim.x + threadIdx.x, h = a.h;
+    if (static_cast<int>(blockIdx.x) >= a.window_blocks) {
+        clear_absent<OD, E, ODD>(a, j, dtable);
         return;
     }
-    const long long w0 = static_cast<long long>(blockIdx.x) * a.window;
-    const int count = static_cast<int>(a.n - w0 < a.window ? a.n - w0 : a.window);
+    const long long w = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y, w0 = w * a.window;
+    const int count = static_cast<int>(max(0ll, min(a.n - w0, static_cast<long long>(a.window))));
+    uint2* it = items + threadIdx.y * (a.window + 2) + 1;
     for (int i = threadIdx.x; i < count + 2; i += blockDim.x) {
-        const long long j = w0 + i - 1;
-        item[i] = j >= 0 && j < a.n ? __ldg(a.sorted + j) : make_uint2(0xffffffffu, 0);
+        const long long k = w0 + i - 1;
+        it[i - 1] = k >= 0 && k < a.n ? __ldg(a.sorted + k) : make_uint2(0xffffffffu, 0);
     }
     __syncthreads();
-    if (c >= a.h) return;
-    const uint2* it = item + 1;
+    if (!ODD && j * E >= h) return;
     float sum[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) sum[e] = 0.0f;
-    bool from_left = it[-1].x == it[0].x;
+    bool from_left = count > 0 && it[-1].x == it[0].x;
     for (int i0 = 0; i0 < count; i0 += kFlight) {
         Raw<D, E> r[kFlight];
 #pragma unroll
         for (int u = 0; u < kFlight; ++u) {
+            const bool in = i0 + u < count && it[i0 + u].x < a.rows;
             r[u] = zero_raw<D, E>();
-            if (i0 + u < count && it[i0 + u].x < a.rows)
-                r[u] = load_raw_cs<D, E>(dy + static_cast<long long>(it[i0 + u].y) * dy_stride + c);
+            if constexpr (!ODD) {
+                if (in) r[u] = load_raw_cs<D, E>(dy + static_cast<long long>(it[i0 + u].y) * dy_stride + j * E);
+            } else if (in) {
+                const int c = j * E - shift_of<ODD, OD>(dtable + static_cast<long long>(it[i0 + u].x) * h);
+                if (c < h) r[u] = get_row<ODD, D>(dy + static_cast<long long>(it[i0 + u].y) * dy_stride, c, h);
+            }
         }
 #pragma unroll
         for (int u = 0; u < kFlight; ++u) {
@@ -203,11 +228,15 @@ __global__ void __launch_bounds__(kThreads) window_kernel(const WindowArgs a, co
             for (int e = 0; e < E; ++e) sum[e] += f[e];
             if (it[i + 1].x == row && i + 1 < count) continue;
             const bool to_right = it[i + 1].x == row;
-            if (from_left || to_right) {
-                float* p = a.partial + (static_cast<long long>(blockIdx.x) * 2 + (from_left ? 0 : 1)) * a.h + c;
+            Bits<OD>* to = dtable + static_cast<long long>(row) * h;
+            const int c = j * E - shift_of<ODD, OD>(to);
+            if (ODD && c >= h) {
+                // nothing of this row in this thread
+            } else if (from_left || to_right) {
+                float* p = a.partial + (w * 2 + (from_left ? 0 : 1)) * a.width + j * E;
                 store_f<kF32, E>(reinterpret_cast<Bits<kF32>*>(p), sum);
             } else {
-                write_row<OD, E>(dtable + row * a.h + c, sum, a.scale, a.accumulate != 0);
+                write_row<OD, E, ODD>(to, c, h, sum, a.scale, a.accumulate != 0);
             }
             from_left = false;
 #pragma unroll
@@ -217,15 +246,19 @@ __global__ void __launch_bounds__(kThreads) window_kernel(const WindowArgs a, co
 }
 
 // The window in which a token begins that runs over its right edge adds the token's partial rows.
-template <int OD, int E>
+template <int OD, int E, bool ODD>
 __global__ void __launch_bounds__(kThreads) join_kernel(const WindowArgs a, Bits<OD>* __restrict__ dtable) {
-    const long long w = blockIdx.x;
+    const long long w = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y;
     const long long end = (w + 1) * a.window;  // windows but the last are full
     if (end >= a.n) return;
     const unsigned int row = __ldg(&a.sorted[end - 1].x);
     if (row >= a.rows || __ldg(&a.sorted[end].x) != row) return;
     const long long begin = w * a.window;
     if (begin > 0 && __ldg(&a.sorted[begin - 1].x) == row) return;  // it began in an earlier window
+    const int j = blockIdx.y * blockDim.x + threadIdx.x;
+    Bits<OD>* to = dtable + static_cast<long long>(row) * a.h;
+    const int c = j * E - shift_of<ODD, OD>(to);
+    if (c >= a.h) return;
     // The last window that holds the token, which is the last whose first position has it: mostly the
     // next one, so search in growing steps.
     long long lo = w + 1, step = 1;
@@ -237,16 +270,14 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const WindowArgs a, Bits
         const long long mid = lo + step / 2;
         if (mid < a.windows && __ldg(&a.sorted[mid * a.window].x) == row) lo = mid;
     }
-    const long long c = (static_cast<long long>(blockIdx.y) * blockDim.x + threadIdx.x) * E;
-    if (c >= a.h) return;
     float sum[E];
-    load_f<kF32, E>(reinterpret_cast<const Bits<kF32>*>(a.partial + (w * 2 + 1) * a.h + c), sum);
+    load_f<kF32, E>(reinterpret_cast<const Bits<kF32>*>(a.partial + (w * 2 + 1) * a.width + j * E), sum);
     for (long long k0 = w + 1; k0 <= lo; k0 += kFlight) {
         float f[kFlight][E];
 #pragma unroll
         for (int u = 0; u < kFlight; ++u)
             if (k0 + u <= lo)
-                load_f<kF32, E>(reinterpret_cast<const Bits<kF32>*>(a.partial + (k0 + u) * 2 * a.h + c), f[u]);
+                load_f<kF32, E>(reinterpret_cast<const Bits<kF32>*>(a.partial + (k0 + u) * 2 * a.width + j * E), f[u]);
 #pragma unroll
         for (int u = 0; u < kFlight; ++u) {
             if (k0 + u > lo) break;
@@ -254,17 +285,19 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const WindowArgs a, Bits
             for (int e = 0; e < E; ++e) sum[e] += f[u][e];
         }
     }
-    write_row<OD, E>(dtable + row * a.h + c, sum, a.scale, a.accumulate != 0);
+    write_row<OD, E, ODD>(to, c, a.h, sum, a.scale, a.accumulate != 0);
 }
 
-// Positions per window: long ones make fewer partial rows, short ones more blocks.
-int window_of(long long n) {
-    int w = 16;
-    while (w < kMaxWindow && ceil_div(n, 2 * w) >= 512) w *= 2;
+// Positions per window: long ones make fewer partial rows, short ones more threads (150000 fill the
+// GPU's SMs by half).
+int window_of(long long n, long long h) {
+    int w = 8;
+    while (w < kMaxWindow && n / (2 * w) * ceil_div(h, 8) >= 150000) w *= 2;
     return w;
 }
 
 size_t align16(size_t v) { return (v + 15) / 16 * 16; }
+long long partial_width(long long h) { return (h + 14) / 8 * 8; }  // accesses of 4 or 8 columns at any shift
 
 }  // namespace
 }  // namespace ops
@@ -274,34 +307,34 @@ cudaError_t LaunchEmbeddingForward(const EmbeddingArgs& a, const void* table, lo
     using namespace ops;
     if (a.n == 0 || a.h == 0) return cudaSuccess;
     const int size = size_of(dtype);
-    const bool wide = rows16(table, table_stride, a.h, size) && rows16(out, out_stride, a.h, size);
+    const bool odd = !rows16(table, table_stride, a.h, size) || !rows16(out, out_stride, a.h, size);
     const KeySource key{a.ids, a.ids64, a.first, a.rows, 0, 0};
     return with_type(dtype, [&](auto D) {
-        constexpr int kD = decltype(D)::value, kE = Vec<kD>::E;
-        auto go = [&](auto EE) {
-            constexpr int E = decltype(EE)::value;
-            const int threads = static_cast<int>(std::min<long long>(kThreads, round32(ceil_div(a.h, E))));
-            const unsigned cols = static_cast<unsigned>(ceil_div(a.h, static_cast<long long>(threads) * E));
-            auto launch = [&](auto TT) {
-                constexpr int T = decltype(TT)::value;
-                const dim3 grid(static_cast<unsigned>(std::min<long long>(ceil_div(a.n, T), 1 << 20)), cols);
-                lookup_kernel<kD, E, T><<<grid, threads, 0, stream>>>(key, a.n, static_cast<const Bits<kD>*>(table),
-                                                                      table_stride, a.h, scale,
-                                                                      static_cast<Bits<kD>*>(out), out_stride);
-                return cudaGetLastError();
-            };
-            // Few rows: one each, on as many SMs as there are.
-            return a.n * cols >= 16 * sm_count() ? launch(Int<4>{}) : launch(Int<1>{});
+        constexpr int kD = decltype(D)::value;
+        auto go = [&](auto O, auto TT) {
+            constexpr bool ODD = decltype(O)::value != 0;
+            constexpr int T = decltype(TT)::value;
+            const long long wide = accesses<ODD>(a.h, Vec<kD>::E);
+            const BlockShape b = block_shape(wide, kThreads);
+            const dim3 grid(static_cast<unsigned>(std::min<long long>(ceil_div(a.n, T * b.y), 1 << 20)),
+                            static_cast<unsigned>(ceil_div(wide, b.x)));
+            lookup_kernel<kD, ODD, T><<<grid, dim3(b.x, b.y), 0, stream>>>(
+                key, a.n, static_cast<const Bits<kD>*>(table), table_stride, static_cast<int>(a.h), scale,
+                static_cast<Bits<kD>*>(out), out_stride);
+            return cudaGetLastError();
         };
-        return wide ? go(Int<kE>{}) : go(Int<1>{});
+        // Few accesses: one row each, on as many SMs as there are.
+        if (a.n * ceil_div(a.h, Vec<kD>::E) < 16ll * kThreads * sm_count())
+            return odd ? go(Int<1>{}, Int<1>{}) : go(Int<0>{}, Int<1>{});
+        return odd ? go(Int<1>{}, Int<4>{}) : go(Int<0>{}, Int<4>{});
     });
 }
 
 size_t EmbeddingBackwardWorkspace(long long n, long long h) {
     using namespace ops;
-    const long long windows = ceil_div(n, window_of(n));
+    const long long windows = ceil_div(n, window_of(n, h));
     return 2 * align16(sizeof(uint2) * static_cast<size_t>(n)) + align16(sizeof(unsigned int) * sort_totals(n)) +
-           align16(sizeof(float) * 2 * static_cast<size_t>(windows) * static_cast<size_t>(h));
+           align16(sizeof(float) * 2 * static_cast<size_t>(windows) * static_cast<size_t>(partial_width(h)));
 }
 
 cudaError_t LaunchEmbeddingBackward(const EmbeddingArgs& a, const void* dy, long long dy_stride, void* dtable,
@@ -348,37 +381,43 @@ cudaError_t LaunchEmbeddingBackward(const EmbeddingArgs& a, const void* dy, long
     args.sorted = buf_b;
     args.n = a.n;
     args.rows = a.rows;
-    args.h = a.h;
-    args.window = window_of(a.n);
+    args.h = static_cast<int>(a.h);
+    args.window = window_of(a.n, a.h);
     args.windows = ceil_div(a.n, args.window);
     args.partial = partial;
+    args.width = partial_width(a.h);
     args.scale = scale;
     args.accumulate = accumulate ? 1 : 0;
-    const bool wide = rows16(dy, dy_stride, a.h, size_of(dtype)) && rows16(dtable, a.h, a.h, size_of(out_dtype));
+    const bool odd = !rows16(dy, dy_stride, a.h, size_of(dtype)) || !rows16(dtable, a.h, a.h, size_of(out_dtype));
     return with_types(dtype, out_dtype, [&](auto D, auto O) {
-        constexpr int kD = decltype(D)::value, kO = decltype(O)::value, kE = Vec<kD>::E;
-        auto go = [&](auto EE) {
-            constexpr int E = decltype(EE)::value;
-            const int threads = static_cast<int>(std::min<long long>(kThreads, round32(ceil_div(a.h, E))));
-            const unsigned cols = static_cast<unsigned>(ceil_div(a.h, static_cast<long long>(threads) * E));
+        constexpr int kD = decltype(D)::value, kO = decltype(O)::value, E = Vec<kD>::E;
+        auto go = [&](auto OO) {
+            constexpr bool ODD = decltype(OO)::value != 0;
+            const long long wide = accesses<ODD>(a.h, E);
+            BlockShape b = block_shape(wide, kThreads);
+            b.y = std::min<int>(b.y, 40 * 1024 / (sizeof(uint2) * (args.window + 2)));  // windows in shared memory
+            const unsigned cols = static_cast<unsigned>(ceil_div(wide, b.x));
             // Tiles of about 128 KiB, a block each, so that blocks whose rows mostly occur make room
             // for others (8 persistent blocks per SM with equal shares: 228 us for 32768 tokens, 128256
             // rows of 8 KiB; tiles 196 us), but two blocks per SM at least.
             WindowArgs w = args;
-            const long long bytes = std::min<long long>(a.h, static_cast<long long>(threads) * E) * sizeof(Bits<kO>);
+            const long long bytes = std::min<long long>(a.h, static_cast<long long>(b.x) * E) * sizeof(Bits<kO>);
             const long long tile = std::min(std::max(32ll, 128 * 1024 / bytes),
                                             ceil_div(a.rows, std::max(1ll, static_cast<long long>(sm_count()) * 2 / cols)));
             w.tile = static_cast<int>(std::min<long long>(kMaxTile, std::max(1ll, tile)));
             const long long clear = accumulate ? 0 : std::min(1ll << 20, ceil_div(a.rows, w.tile));
-            window_kernel<kD, kO, E><<<dim3(static_cast<unsigned>(w.windows + clear), cols), threads, 0, stream>>>(
-                w, static_cast<const Bits<kD>*>(dy), dy_stride, static_cast<Bits<kO>*>(dtable));
+            w.window_blocks = static_cast<int>(ceil_div(w.windows, b.y));
+            const size_t smem = sizeof(uint2) * b.y * (w.window + 2);
+            window_kernel<kD, kO, ODD>
+                <<<dim3(static_cast<unsigned>(w.window_blocks + clear), cols), dim3(b.x, b.y), smem, stream>>>(
+                    w, static_cast<const Bits<kD>*>(dy), dy_stride, static_cast<Bits<kO>*>(dtable));
             cudaError_t err = cudaGetLastError();
             if (err != cudaSuccess || w.windows == 1) return err;
-            join_kernel<kO, E><<<dim3(static_cast<unsigned>(w.windows - 1), cols), threads, 0, stream>>>(
+            join_kernel<kO, E, ODD><<<dim3(static_cast<unsigned>(w.window_blocks), cols), dim3(b.x, b.y), 0, stream>>>(
                 w, static_cast<Bits<kO>*>(dtable));
             return cudaGetLastError();
         };
-        return wide ? go(Int<kE>{}) : go(Int<1>{});
+        return odd ? go(Int<1>{}) : go(Int<0>{});
     });
 }
 

@@ -40,48 +40,73 @@ constexpr int kTokenThreads = 256;
 // Dropped assignments have slot -1; nothing outside the rows is touched whatever the slots hold.
 __device__ __forceinline__ bool in_rows(int slot, long long n) { return static_cast<unsigned int>(slot) < n; }
 
-// blockIdx.x walks tokens and then, past them, the rows behind the last kept one; blockIdx.y columns.
-template <int D, int E>
+// Zeros for the rows behind the last kept one, by all blocks of a kernel: row `first`, first + step, ...
+template <int D, bool ODD>
+__device__ __forceinline__ void clear_tail(Bits<D>* rows, long long kept, long long n, int h, int j0, int dj, long long first,
+                                           long long step) {
+    constexpr int E = Vec<D>::E;
+    for (long long i = kept + first; i < n; i += step) {
+        Bits<D>* row = rows + i * h;
+        const int shift = shift_of<ODD, D>(row);
+        for (int c = j0 * E - shift; c < h; c += dj * E) put_raw<ODD, D>(row, c, h, zero_raw<D, E>());
+    }
+}
+
+// blockDim (x, y): columns, tokens. blockIdx.x walks tokens, blockIdx.y columns.
+template <int D, bool ODD>
 __global__ void __launch_bounds__(kTokenThreads) dispatch_kernel(const Bits<D>* __restrict__ x, long long x_stride,
                                                                  const int* __restrict__ slots,
                                                                  const int* __restrict__ kept, long long tokens, int top,
-                                                                 long long h, Bits<D>* __restrict__ rows) {
-    const long long c = (static_cast<long long>(blockIdx.y) * blockDim.x + threadIdx.x) * E;
-    if (c >= h) return;
-    for (long long t = blockIdx.x; t < tokens; t += gridDim.x) {
-        const Raw<D, E> r = load_raw_cs<D, E>(x + t * x_stride + c);
-        const int* s = slots + t * top;
-        for (int j = 0; j < top; ++j) {
-            const int slot = __ldg(s + j);
-            if (in_rows(slot, tokens * top)) store_raw_cs<D, E>(rows + static_cast<long long>(slot) * h + c, r);
+                                                                 int h, Bits<D>* __restrict__ rows) {
+    constexpr int E = Vec<D>::E;
+    const int j = blockIdx.y * blockDim.x + threadIdx.x;
+    const long long first = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y;
+    const long long step = static_cast<long long>(gridDim.x) * blockDim.y, n = tokens * top;
+    if (!ODD && j * E >= h) return;
+    for (long long t = first; t < tokens; t += step) {
+        const Bits<D>* from = x + t * x_stride;
+        Raw<D, E> r;
+        if constexpr (!ODD) r = get_row<false, D>(from, j * E, h);
+        for (int k = 0; k < top; ++k) {
+            const int slot = __ldg(slots + t * top + k);
+            if (!in_rows(slot, n)) continue;
+            Bits<D>* to = rows + static_cast<long long>(slot) * h;
+            const int c = j * E - shift_of<ODD, D>(to);
+            if (ODD && c >= h) continue;
+            if constexpr (ODD) r = get_row<true, D>(from, c, h);
+            put_raw<ODD, D>(to, c, h, r);
         }
     }
-    for (long long i = __ldg(kept) + static_cast<long long>(blockIdx.x); i < tokens * top; i += gridDim.x)
-        store_raw_cs<D, E>(rows + i * h + c, zero_raw<D, E>());
+    clear_tail<D, ODD>(rows, __ldg(kept), n, h, j, gridDim.y * blockDim.x, first, step);
 }
 
-// U rows are in flight per thread; each token's sum runs over j in order.
-template <int D, int WD, int E, int U>
+// U rows are in flight per thread; each token's sum runs over its assignments in order.
+template <int D, int WD, bool ODD, int U>
 __global__ void __launch_bounds__(kTokenThreads) combine_kernel(const Bits<D>* __restrict__ rows,
                                                                 const int* __restrict__ slots,
                                                                 const Bits<WD>* __restrict__ weights, long long tokens,
-                                                                int top, long long h, Bits<D>* __restrict__ y,
+                                                                int top, int h, Bits<D>* __restrict__ y,
                                                                 long long y_stride) {
-    const long long c = (static_cast<long long>(blockIdx.y) * blockDim.x + threadIdx.x) * E;
-    if (c >= h) return;
-    for (long long t = blockIdx.x; t < tokens; t += gridDim.x) {
+    constexpr int E = Vec<D>::E;
+    const int j = blockIdx.y * blockDim.x + threadIdx.x;
+    const long long n = tokens * top;
+    for (long long t = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y; t < tokens;
+         t += static_cast<long long>(gridDim.x) * blockDim.y) {
+        Bits<D>* to = y + t * y_stride;
+        const int c = j * E - shift_of<ODD, D>(to);
+        if (c >= h) continue;
         float acc[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-        for (int j0 = 0; j0 < top; j0 += U) {
+        for (int k0 = 0; k0 < top; k0 += U) {
             Raw<D, E> r[U];
             float w[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int slot = j0 + u < top ? __ldg(slots + t * top + j0 + u) : -1;
-                const bool kept = in_rows(slot, tokens * top);
-                r[u] = kept ? load_raw_cs<D, E>(rows + static_cast<long long>(slot) * h + c) : zero_raw<D, E>();
-                w[u] = !kept ? 0.0f : weights == nullptr ? 1.0f : Ty<WD>::load(__ldg(weights + t * top + j0 + u));
+                const int slot = k0 + u < top ? __ldg(slots + t * top + k0 + u) : -1;
+                const bool kept = in_rows(slot, n);
+                r[u] = kept ? get_row<ODD, D>(rows + static_cast<long long>(slot) * h, c, h) : zero_raw<D, E>();
+                w[u] = !kept ? 0.0f : weights == nullptr ? 1.0f : Ty<WD>::load(__ldg(weights + t * top + k0 + u));
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -91,75 +116,69 @@ __global__ void __launch_bounds__(kTokenThreads) combine_kernel(const Bits<D>* _
                 for (int e = 0; e < E; ++e) acc[e] = fmaf(w[u], f[e], acc[e]);
             }
         }
-        store_f_cs<D, E>(y + t * y_stride + c, acc);
+        put_row<ODD, D, E>(to, c, h, acc);
     }
 }
 
-// A warp per assignment: a dot product needs no barrier, and a warp reads its row of `rows` in kFlight
-// accesses at a time; the token's row, which the block's other warps read too, comes from L1. (A
-// block per token with 4 or 8 rows in flight and block-wide sums took 199 and 241 us for 8192 tokens of
-// 8 x 4096 bf16; this takes 177 us.) A lane adds every kFlight-th of its products in the same register, the
-// registers and the lanes are added by trees.
+// A warp, or a part of one where a row is short (LANES), per assignment: a dot
+// product needs no barrier, and the lanes read their row of `rows` in kFlight accesses at a time; the
+// token's row, which the block's other warps read too, comes from L1. (A block per token with 4 or 8 rows
+// in flight and block-wide sums took 199 and 241 us for 8192 tokens of 8 x 4096 bf16; this takes 177.) A
+// lane adds every kFlight-th of its products in the same register, the registers and the lanes are added
+// by trees.
 constexpr int kFlight = 4;
 
-template <int D, int WD, int E>
+template <int D, int WD, bool ODD, int LANES>
 __global__ void __launch_bounds__(kTokenThreads) combine_backward_kernel(
     const Bits<D>* __restrict__ dy, long long dy_stride, const Bits<D>* __restrict__ rows, const int* __restrict__ slots,
-    const int* __restrict__ kept, const Bits<WD>* __restrict__ weights, long long tokens, int top, long long h,
+    const int* __restrict__ kept, const Bits<WD>* __restrict__ weights, long long tokens, int top, int h,
     Bits<D>* __restrict__ drows, Bits<WD>* __restrict__ dweights) {
-    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    const long long n = tokens * top, first = static_cast<long long>(blockIdx.x) * warps + (threadIdx.x >> 5);
-    const long long step = static_cast<long long>(gridDim.x) * warps;
-    for (long long a = first; a < n; a += step) {
-        const int slot = __ldg(slots + a);
-        if (!in_rows(slot, n)) {
-            if (dweights != nullptr && lane == 0) dweights[a] = Ty<WD>::store(0.0f);
-            continue;
-        }
-        const float w = weights == nullptr ? 1.0f : Ty<WD>::load(__ldg(weights + a));
-        const Bits<D>* g = dy + a / top * dy_stride;
-        const long long at = static_cast<long long>(slot) * h;
+    constexpr int E = Vec<D>::E;
+    constexpr int kRows = kTokenThreads / LANES;
+    const int lane = threadIdx.x & (LANES - 1), group = threadIdx.x / LANES;
+    const long long n = tokens * top, first = static_cast<long long>(blockIdx.x) * kRows + group;
+    const long long step = static_cast<long long>(gridDim.x) * kRows;
+    for (long long a0 = first - group; a0 < n; a0 += step) {  // the same trips for a whole warp
+        const long long a = a0 + group;
+        const int slot = a < n ? __ldg(slots + a) : -1;
         float dot[kFlight] = {};
-        for (long long c0 = lane * E; c0 < h; c0 += 32 * kFlight * E) {
-            Raw<D, E> r[kFlight], t[kFlight];
+        if (in_rows(slot, n)) {
+            const float w = weights == nullptr ? 1.0f : Ty<WD>::load(__ldg(weights + a));
+            const Bits<D>* g = dy + a / top * dy_stride;
+            const long long at = static_cast<long long>(slot) * h;
+            const int shift = drows != nullptr ? shift_of<ODD, D>(drows + at) : 0;
+            for (int c0 = lane * E - shift; c0 < h; c0 += LANES * kFlight * E) {
+                Raw<D, E> r[kFlight], t[kFlight];
 #pragma unroll
-            for (int u = 0; u < kFlight; ++u) {
-                const long long c = c0 + u * 32 * E;
-                r[u] = c < h && dweights != nullptr ? load_raw_cs<D, E>(rows + at + c) : zero_raw<D, E>();
-                t[u] = c < h ? load_raw<D, E>(g + c) : zero_raw<D, E>();
-            }
-#pragma unroll
-            for (int u = 0; u < kFlight; ++u) {
-                const long long c = c0 + u * 32 * E;
-                float f[E], d[E];
-                unpack<D, E>(r[u], f);
-                unpack<D, E>(t[u], d);
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    dot[u] = fmaf(d[e], f[e], dot[u]);
-                    d[e] *= w;
+                for (int u = 0; u < kFlight; ++u) {
+                    const int c = c0 + u * LANES * E;
+                    r[u] = c < h && dweights != nullptr ? get_row<ODD, D>(rows + at, c, h) : zero_raw<D, E>();
+                    t[u] = c >= h ? zero_raw<D, E>() : ODD ? get_row<ODD, D>(g, c, h) : load_raw<D, E>(g + c);
                 }
-                if (c < h && drows != nullptr) store_f_cs<D, E>(drows + at + c, d);
+#pragma unroll
+                for (int u = 0; u < kFlight; ++u) {
+                    const int c = c0 + u * LANES * E;
+                    float f[E], d[E];
+                    unpack<D, E>(r[u], f);
+                    unpack<D, E>(t[u], d);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        dot[u] = fmaf(d[e], f[e], dot[u]);
+                        d[e] *= w;
+                    }
+                    if (c < h && drows != nullptr) put_row<ODD, D, E>(drows + at, c, h, d);
+                }
             }
         }
         if (dweights == nullptr) continue;
-        const float s = warp_sum((dot[0] + dot[1]) + (dot[2] + dot[3]));
-        if (lane == 0) dweights[a] = Ty<WD>::store(s);
+        float s = (dot[0] + dot[1]) + (dot[2] + dot[3]);
+        for (int o = LANES / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (lane == 0 && a < n) dweights[a] = Ty<WD>::store(s);  // 0 for a dropped assignment
     }
-    if (drows == nullptr) return;
-    for (long long i = __ldg(kept) + first; i < n; i += step)
-        for (long long c = lane * E; c < h; c += 32 * E) store_raw_cs<D, E>(drows + i * h + c, zero_raw<D, E>());
+    if (drows != nullptr) clear_tail<D, ODD>(drows, __ldg(kept), n, h, lane, LANES, first, step);
 }
 
 constexpr long long kMaxBlocks = 1 << 20;
-
-dim3 token_grid(long long tokens, long long h, int e, int threads) {
-    return dim3(static_cast<unsigned>(std::min(tokens, kMaxBlocks)),
-                static_cast<unsigned>(ceil_div(h, static_cast<long long>(threads) * e)));
-}
-int token_threads(long long h, int e, int most) {
-    return static_cast<int>(std::min<long long>(most, round32(ceil_div(h, e))));
-}
 
 }  // namespace
 }  // namespace ops
@@ -191,18 +210,21 @@ cudaError_t LaunchExpertDispatch(const void* x, long long x_stride, const int* s
     using namespace ops;
     if (tokens == 0 || top == 0) return cudaSuccess;
     const int size = size_of(dtype);
-    const bool wide = rows16(x, x_stride, h, size) && on16(rows);
+    const bool odd = !rows16(x, x_stride, h, size) || !on16(rows);
     return with_type(dtype, [&](auto D) {
-        constexpr int kD = decltype(D)::value, kE = Vec<kD>::E;
-        auto go = [&](auto EE) {
-            constexpr int E = decltype(EE)::value;
-            const int threads = token_threads(h, E, kTokenThreads);
-            dispatch_kernel<kD, E><<<token_grid(tokens, h, E, threads), threads, 0, stream>>>(
-                static_cast<const Bits<kD>*>(x), x_stride, slots, offsets + experts, tokens, top, h,
+        constexpr int kD = decltype(D)::value;
+        auto go = [&](auto O) {
+            constexpr bool ODD = decltype(O)::value != 0;
+            const long long wide = accesses<ODD>(h, Vec<kD>::E);
+            const BlockShape b = block_shape(wide, kTokenThreads);
+            const dim3 grid(static_cast<unsigned>(std::min(ceil_div(tokens, b.y), kMaxBlocks)),
+                            static_cast<unsigned>(ceil_div(wide, b.x)));
+            dispatch_kernel<kD, ODD><<<grid, dim3(b.x, b.y), 0, stream>>>(
+                static_cast<const Bits<kD>*>(x), x_stride, slots, offsets + experts, tokens, top, static_cast<int>(h),
                 static_cast<Bits<kD>*>(rows));
             return cudaGetLastError();
         };
-        return wide ? go(Int<kE>{}) : go(Int<1>{});
+        return odd ? go(Int<1>{}) : go(Int<0>{});
     });
 }
 
@@ -211,19 +233,23 @@ cudaError_t LaunchExpertCombine(const void* rows, const int* slots, const void* 
     using namespace ops;
     if (tokens == 0) return cudaSuccess;
     const int size = size_of(dtype);
-    const bool wide = rows16(y, y_stride, h, size) && on16(rows);
+    const bool odd = !rows16(y, y_stride, h, size) || !on16(rows);
     return with_types(dtype, wdtype, [&](auto D, auto W) {
-        constexpr int kD = decltype(D)::value, kW = decltype(W)::value, kE = Vec<kD>::E;
-        auto go = [&](auto EE, auto UU) {
-            constexpr int E = decltype(EE)::value, U = decltype(UU)::value;
-            const int threads = token_threads(h, E, kTokenThreads);
-            combine_kernel<kD, kW, E, U><<<token_grid(tokens, h, E, threads), threads, 0, stream>>>(
-                static_cast<const Bits<kD>*>(rows), slots, static_cast<const Bits<kW>*>(weights), tokens, top, h,
-                static_cast<Bits<kD>*>(y), y_stride);
+        constexpr int kD = decltype(D)::value, kW = decltype(W)::value;
+        auto go = [&](auto O, auto UU) {
+            constexpr bool ODD = decltype(O)::value != 0;
+            constexpr int U = decltype(UU)::value;
+            const long long wide = accesses<ODD>(h, Vec<kD>::E);
+            const BlockShape b = block_shape(wide, kTokenThreads);
+            const dim3 grid(static_cast<unsigned>(std::min(ceil_div(tokens, b.y), kMaxBlocks)),
+                            static_cast<unsigned>(ceil_div(wide, b.x)));
+            combine_kernel<kD, kW, ODD, U><<<grid, dim3(b.x, b.y), 0, stream>>>(
+                static_cast<const Bits<kD>*>(rows), slots, static_cast<const Bits<kW>*>(weights), tokens, top,
+                static_cast<int>(h), static_cast<Bits<kD>*>(y), y_stride);
             return cudaGetLastError();
         };
-        if (top <= 2) return wide ? go(Int<kE>{}, Int<2>{}) : go(Int<1>{}, Int<2>{});
-        return wide ? go(Int<kE>{}, Int<8>{}) : go(Int<1>{}, Int<8>{});
+        if (top <= 2) return odd ? go(Int<1>{}, Int<2>{}) : go(Int<0>{}, Int<2>{});
+        return odd ? go(Int<1>{}, Int<4>{}) : go(Int<0>{}, Int<8>{});
     });
 }
 
@@ -234,20 +260,25 @@ cudaError_t LaunchExpertCombineBackward(const void* dy, long long dy_stride, con
     using namespace ops;
     if (tokens == 0 || top == 0) return cudaSuccess;
     const int size = size_of(dtype);
-    const bool wide = rows16(dy, dy_stride, h, size) && on16(rows) && (drows == nullptr || on16(drows));
+    const bool odd = !rows16(dy, dy_stride, h, size) || !on16(rows) || (drows != nullptr && !on16(drows));
     return with_types(dtype, wdtype, [&](auto D, auto W) {
-        constexpr int kD = decltype(D)::value, kW = decltype(W)::value, kE = Vec<kD>::E;
-        auto go = [&](auto EE) {
-            constexpr int E = decltype(EE)::value;
-            const long long blocks = ceil_div(tokens * top, kTokenThreads / 32);
-            combine_backward_kernel<kD, kW, E>
-                <<<static_cast<unsigned>(std::min(blocks, kMaxBlocks)), kTokenThreads, 0, stream>>>(
-                    static_cast<const Bits<kD>*>(dy), dy_stride, static_cast<const Bits<kD>*>(rows), slots,
-                    offsets + experts, static_cast<const Bits<kW>*>(weights), tokens, top, h,
-                    static_cast<Bits<kD>*>(drows), static_cast<Bits<kW>*>(dweights));
-            return cudaGetLastError();
+        constexpr int kD = decltype(D)::value, kW = decltype(W)::value;
+        auto go = [&](auto O) {
+            constexpr bool ODD = decltype(O)::value != 0;
+            auto launch = [&](auto L) {
+                constexpr int kLanes = decltype(L)::value;
+                const long long blocks = ceil_div(tokens * top, kTokenThreads / kLanes);
+                combine_backward_kernel<kD, kW, ODD, kLanes>
+                    <<<static_cast<unsigned>(std::min(blocks, kMaxBlocks)), kTokenThreads, 0, stream>>>(
+                        static_cast<const Bits<kD>*>(dy), dy_stride, static_cast<const Bits<kD>*>(rows), slots,
+                        offsets + experts, static_cast<const Bits<kW>*>(weights), tokens, top, static_cast<int>(h),
+                        static_cast<Bits<kD>*>(drows), static_cast<Bits<kW>*>(dweights));
+                return cudaGetLastError();
+            };
+            const long long n = accesses<ODD>(h, Vec<kD>::E);
+            return n <= 4 ? launch(Int<4>{}) : n <= 16 ? launch(Int<16>{}) : launch(Int<32>{});
         };
-        return wide ? go(Int<kE>{}) : go(Int<1>{});
+        return odd ? go(Int<1>{}) : go(Int<0>{});
     });
 }
 

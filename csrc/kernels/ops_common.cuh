@@ -1,13 +1,17 @@
 // Shared by the compute operators (grad_norm.cu, norms.cu, embedding.cu, experts.cu): loads and
 // stores of E adjacent elements as floats, reductions over a block, launch helpers.
 //
-// Each kernel exists in two widths: E elements that fill 16 bytes, where every row starts on a
-// 16-byte boundary (base pointers and row strides), and E = 1 for every other layout. A warp's
-// 16-byte accesses cover 512 adjacent bytes; element accesses of 2 or 4 bytes 64 or 128.
+// Kernels access E elements that fill 16 bytes. Where every row starts on a 16-byte boundary (base
+// pointers and row strides) an access covers the columns from a multiple of E on. For all other layouts
+// each kernel has an ODD form: accesses start on the 16-byte boundaries of the row that is written,
+// `shift` columns before multiples of E; a row read at another alignment is put together from two
+// 16-byte groups, and the first and last access of a row go element by element. (Element accesses
+// throughout were bound by issuing loads: norms over 16384 x 4097 bf16 took @ODD1@ us instead of @ODD8@.)
 #pragma once
 
 #include "kernels/common.cuh"
 
+#include <algorithm>
 #include <climits>
 
 namespace bccl {
@@ -109,6 +113,98 @@ template <int D, int E>
 __device__ __forceinline__ void store_raw_cs(Bits<D>* p, const Raw<D, E>& r) {
     if constexpr (E == 1) __stcs(p, r.v);
     else __stcs(reinterpret_cast<uint4*>(p), r.v);
+}
+
+// ---------------------------------------------------------------- rows of any alignment
+// 16 bytes from any element boundary, by 16-byte groups that each hold some of them (so they lie in the
+// allocation that holds the row, whatever comes before and behind it).
+template <int D>
+__device__ __forceinline__ uint4 load_unaligned(const Bits<D>* p) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+    const unsigned int k = a & 15;
+    const uint4* group = reinterpret_cast<const uint4*>(a - k);
+    const uint4 lo = __ldg(group);
+    if (k == 0) return lo;
+    const uint4 hi = __ldg(group + 1);
+    unsigned int w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    if (k & 4) {
+#pragma unroll
+        for (int i = 0; i < 7; ++i) w[i] = w[i + 1];
+    }
+    if (k & 8) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = w[i + 2];
+    }
+    const unsigned int bits = (k & 3) * 8;
+    return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                      __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+// Columns by which the row's first access starts before its first element.
+template <bool ODD, int D>
+__device__ __forceinline__ int shift_of(const Bits<D>* row) {
+    return ODD ? static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(Bits<D>)) : 0;
+}
+// Columns [c, c + E) of a row of h; zeros outside it. Not ODD: c is a multiple of E below h.
+template <bool ODD, int D>
+__device__ __forceinline__ Raw<D, Vec<D>::E> get_row(const Bits<D>* row, int c, int h) {
+    constexpr int E = Vec<D>::E;
+    if constexpr (!ODD) {
+        return load_raw_cs<D, E>(row + c);
+    } else {
+        Raw<D, E> r;
+        if (c >= 0 && c + E <= h) {
+            r.v = load_unaligned<D>(row + c);
+        } else {
+            dev::V16<D> v;
+#pragma unroll
+            for (int e = 0; e < E; ++e) v.b[e] = c + e >= 0 && c + e < h ? __ldg(row + c + e) : 0;
+            r.v = v.u;
+        }
+        return r;
+    }
+}
+// The same as floats, of a type that may be wider (parameters next to 16-bit rows).
+template <bool ODD, int D, int E>
+__device__ __forceinline__ void get_params(const Bits<D>* row, int c, int h, float (&a)[E]) {
+    if constexpr (!ODD) {
+        load_f<D, E>(row + c, a);
+    } else {
+        constexpr int W = Vec<D>::E;
+#pragma unroll
+        for (int i = 0; i < E / W; ++i) {
+            float t[W];
+            unpack<D, W>(get_row<true, D>(row, c + i * W, h), t);
+#pragma unroll
+            for (int e = 0; e < W; ++e) a[i * W + e] = t[e];
+        }
+    }
+}
+// Stores columns [c, c + E), those inside the row; row + c lies on a 16-byte boundary.
+template <bool ODD, int D, int E>
+__device__ __forceinline__ void put_row(Bits<D>* row, int c, int h, const float (&a)[E]) {
+    if (!ODD || (c >= 0 && c + E <= h)) {
+        store_f_cs<D, E>(row + c, a);
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (c + e >= 0 && c + e < h) row[c + e] = Ty<D>::store(a[e]);
+    }
+}
+template <bool ODD, int D>
+__device__ __forceinline__ void put_raw(Bits<D>* row, int c, int h, const Raw<D, Vec<D>::E>& r) {
+    if (!ODD || (c >= 0 && c + Vec<D>::E <= h)) {
+        store_raw_cs<D, Vec<D>::E>(row + c, r);
+    } else {
+        dev::V16<D> v;
+        v.u = r.v;
+#pragma unroll
+        for (int e = 0; e < Vec<D>::E; ++e)
+            if (c + e >= 0 && c + e < h) row[c + e] = v.b[e];
+    }
+}
+// Accesses that cover a row of h elements at any shift.
+template <bool ODD> __host__ __device__ __forceinline__ long long accesses(long long h, int e) {
+    return ODD ? (h + 2 * e - 2) / e : (h + e - 1) / e;
 }
 
 // Two floats in one register pair: sm_100 multiplies and adds both in one instruction.
@@ -216,6 +312,16 @@ inline int round32(long long v) { return static_cast<int>((v + 31) / 32 * 32); }
 
 // SMs of the current device (148 on a B200); looked up once per device.
 int sm_count();
+
+// Threads along a row and rows per block (at most `most` threads in all) for kernels without barriers:
+// short rows share a block.
+struct BlockShape {
+    int x, y;
+};
+inline BlockShape block_shape(long long accesses, int most) {
+    const int x = static_cast<int>(std::min<long long>(accesses, most));
+    return {x, most / x};
+}
 
 // f(integral_constant<D>) for a floating-point type code.
 template <int V> struct Int { static constexpr int value = V; };
