@@ -24,15 +24,17 @@ constexpr int kThreads = 256;
 // A thread copies its columns of TOKENS rows, all in flight at once: a row cannot be asked for before
 // its id is there, so one row at a time leaves the memory idle (32768 rows of 8 KiB: 97 us, with four 63).
 // blockDim (x, y): columns, groups of TOKENS rows.
-template <int D, bool ODD, int TOKENS>
-__global__ void __launch_bounds__(kThreads, ODD ? 3 : 6) lookup_kernel(const KeySource key, long long n, const Bits<D>* __restrict__ table,
+template <int D, typename Form, int TOKENS>
+__global__ void __launch_bounds__(kThreads) lookup_kernel(const KeySource key, long long n, const Bits<D>* __restrict__ table,
                                                           long long table_stride, int h, float scale,
                                                           Bits<D>* __restrict__ out, long long out_stride) {
     constexpr int E = Vec<D>::E;
+    constexpr bool ODD = Form::odd;
     const int j = blockIdx.y * blockDim.x + threadIdx.x;
     if (!ODD && j * E >= h) return;
-    const long long step = static_cast<long long>(gridDim.x) * blockDim.y * TOKENS;
-    for (long long i0 = (static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y) * TOKENS; i0 < n; i0 += step) {
+    const long long step = static_cast<long long>(gridDim.x) * rows_per_block<Form>() * TOKENS;
+    for (long long i0 = (static_cast<long long>(blockIdx.x) * rows_per_block<Form>() + row_in_block<Form>()) * TOKENS; i0 < n;
+         i0 += step) {
         unsigned int row[TOKENS];
         Raw<D, E> r[TOKENS];
 #pragma unroll
@@ -180,19 +182,21 @@ __device__ __forceinline__ void clear_absent(const WindowArgs& a, int j, Bits<OD
 
 // blockDim (x, y): columns, windows. blockIdx.x < window_blocks: windows of sorted positions; beyond:
 // rows to clear. blockIdx.y: columns.
-template <int D, int OD, bool ODD>
-__global__ void __launch_bounds__(kThreads, ODD ? 3 : 4) window_kernel(const WindowArgs a, const Bits<D>* __restrict__ dy,
+template <int D, int OD, typename Form>
+__global__ void __launch_bounds__(kThreads) window_kernel(const WindowArgs a, const Bits<D>* __restrict__ dy,
                                                           long long dy_stride, Bits<OD>* __restrict__ dtable) {
     constexpr int E = Vec<D>::E;
+    constexpr bool ODD = Form::odd;
     extern __shared__ uint2 items[];  // [blockDim.y][window + 2]: the windows and their neighbours on either side
     const int j = blockIdx.y * blockDim.x + threadIdx.x, h = a.h;
     if (static_cast<int>(blockIdx.x) >= a.window_blocks) {
         clear_absent<OD, E, ODD>(a, j, dtable);
         return;
     }
-    const long long w = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y, w0 = w * a.window;
+    const long long w = static_cast<long long>(blockIdx.x) * rows_per_block<Form>() + row_in_block<Form>();
+    const long long w0 = w * a.window;
     const int count = static_cast<int>(max(0ll, min(a.n - w0, static_cast<long long>(a.window))));
-    uint2* it = items + threadIdx.y * (a.window + 2) + 1;
+    uint2* it = items + row_in_block<Form>() * (a.window + 2) + 1;
     for (int i = threadIdx.x; i < count + 2; i += blockDim.x) {
         const long long k = w0 + i - 1;
         it[i - 1] = k >= 0 && k < a.n ? __ldg(a.sorted + k) : make_uint2(0xffffffffu, 0);
@@ -311,22 +315,19 @@ cudaError_t LaunchEmbeddingForward(const EmbeddingArgs& a, const void* table, lo
     const KeySource key{a.ids, a.ids64, a.first, a.rows, 0, 0};
     return with_type(dtype, [&](auto D) {
         constexpr int kD = decltype(D)::value;
-        auto go = [&](auto O, auto TT) {
-            constexpr bool ODD = decltype(O)::value != 0;
-            constexpr int T = decltype(TT)::value;
-            const long long wide = accesses<ODD>(a.h, Vec<kD>::E);
-            const BlockShape b = block_shape(wide, kThreads);
-            const dim3 grid(static_cast<unsigned>(std::min<long long>(ceil_div(a.n, T * b.y), 1 << 20)),
-                            static_cast<unsigned>(ceil_div(wide, b.x)));
-            lookup_kernel<kD, ODD, T><<<grid, dim3(b.x, b.y), 0, stream>>>(
-                key, a.n, static_cast<const Bits<kD>*>(table), table_stride, static_cast<int>(a.h), scale,
-                static_cast<Bits<kD>*>(out), out_stride);
-            return cudaGetLastError();
-        };
-        // Few accesses: one row each, on as many SMs as there are.
-        if (a.n * ceil_div(a.h, Vec<kD>::E) < 16ll * kThreads * sm_count())
-            return odd ? go(Int<1>{}, Int<1>{}) : go(Int<0>{}, Int<1>{});
-        return odd ? go(Int<1>{}, Int<4>{}) : go(Int<0>{}, Int<4>{});
+        return with_form(odd, a.h, Vec<kD>::E, kThreads, [&](auto form, long long wide, BlockShape b) {
+            auto go = [&](auto TT) {
+                constexpr int T = decltype(TT)::value;
+                const dim3 grid(static_cast<unsigned>(std::min<long long>(ceil_div(a.n, T * b.y), 1 << 20)),
+                                static_cast<unsigned>(ceil_div(wide, b.x)));
+                lookup_kernel<kD, decltype(form), T><<<grid, dim3(b.x, b.y), 0, stream>>>(
+                    key, a.n, static_cast<const Bits<kD>*>(table), table_stride, static_cast<int>(a.h), scale,
+                    static_cast<Bits<kD>*>(out), out_stride);
+                return cudaGetLastError();
+            };
+            // Few accesses: one row each, on as many SMs as there are.
+            return a.n * wide < 16ll * kThreads * sm_count() ? go(Int<1>{}) : go(Int<4>{});
+        });
     });
 }
 
@@ -391,10 +392,8 @@ cudaError_t LaunchEmbeddingBackward(const EmbeddingArgs& a, const void* dy, long
     const bool odd = !rows16(dy, dy_stride, a.h, size_of(dtype)) || !rows16(dtable, a.h, a.h, size_of(out_dtype));
     return with_types(dtype, out_dtype, [&](auto D, auto O) {
         constexpr int kD = decltype(D)::value, kO = decltype(O)::value, E = Vec<kD>::E;
-        auto go = [&](auto OO) {
-            constexpr bool ODD = decltype(OO)::value != 0;
-            const long long wide = accesses<ODD>(a.h, E);
-            BlockShape b = block_shape(wide, kThreads);
+        return with_form(odd, a.h, E, kThreads, [&](auto form, long long wide, BlockShape b) {
+            using Form = decltype(form);
             b.y = std::min<int>(b.y, 40 * 1024 / (sizeof(uint2) * (args.window + 2)));  // windows in shared memory
             const unsigned cols = static_cast<unsigned>(ceil_div(wide, b.x));
             // Tiles of about 128 KiB, a block each, so that blocks whose rows mostly occur make room
@@ -408,16 +407,15 @@ cudaError_t LaunchEmbeddingBackward(const EmbeddingArgs& a, const void* dy, long
             const long long clear = accumulate ? 0 : std::min(1ll << 20, ceil_div(a.rows, w.tile));
             w.window_blocks = static_cast<int>(ceil_div(w.windows, b.y));
             const size_t smem = sizeof(uint2) * b.y * (w.window + 2);
-            window_kernel<kD, kO, ODD>
+            window_kernel<kD, kO, Form>
                 <<<dim3(static_cast<unsigned>(w.window_blocks + clear), cols), dim3(b.x, b.y), smem, stream>>>(
                     w, static_cast<const Bits<kD>*>(dy), dy_stride, static_cast<Bits<kO>*>(dtable));
             cudaError_t err = cudaGetLastError();
             if (err != cudaSuccess || w.windows == 1) return err;
-            join_kernel<kO, E, ODD><<<dim3(static_cast<unsigned>(w.window_blocks), cols), dim3(b.x, b.y), 0, stream>>>(
+            join_kernel<kO, E, Form::odd><<<dim3(static_cast<unsigned>(w.window_blocks), cols), dim3(b.x, b.y), 0, stream>>>(
                 w, static_cast<Bits<kO>*>(dtable));
             return cudaGetLastError();
-        };
-        return odd ? go(Int<1>{}) : go(Int<0>{});
+        });
     });
 }
 

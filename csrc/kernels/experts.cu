@@ -53,15 +53,16 @@ __device__ __forceinline__ void clear_tail(Bits<D>* rows, long long kept, long l
 }
 
 // blockDim (x, y): columns, tokens. blockIdx.x walks tokens, blockIdx.y columns.
-template <int D, bool ODD>
+template <int D, typename Form>
 __global__ void __launch_bounds__(kTokenThreads) dispatch_kernel(const Bits<D>* __restrict__ x, long long x_stride,
                                                                  const int* __restrict__ slots,
                                                                  const int* __restrict__ kept, long long tokens, int top,
                                                                  int h, Bits<D>* __restrict__ rows) {
     constexpr int E = Vec<D>::E;
+    constexpr bool ODD = Form::odd;
     const int j = blockIdx.y * blockDim.x + threadIdx.x;
-    const long long first = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y;
-    const long long step = static_cast<long long>(gridDim.x) * blockDim.y, n = tokens * top;
+    const long long first = static_cast<long long>(blockIdx.x) * rows_per_block<Form>() + row_in_block<Form>();
+    const long long step = static_cast<long long>(gridDim.x) * rows_per_block<Form>(), n = tokens * top;
     if (!ODD && j * E >= h) return;
     for (long long t = first; t < tokens; t += step) {
         const Bits<D>* from = x + t * x_stride;
@@ -81,17 +82,18 @@ __global__ void __launch_bounds__(kTokenThreads) dispatch_kernel(const Bits<D>* 
 }
 
 // U rows are in flight per thread; each token's sum runs over its assignments in order.
-template <int D, int WD, bool ODD, int U>
+template <int D, int WD, typename Form, int U>
 __global__ void __launch_bounds__(kTokenThreads) combine_kernel(const Bits<D>* __restrict__ rows,
                                                                 const int* __restrict__ slots,
                                                                 const Bits<WD>* __restrict__ weights, long long tokens,
                                                                 int top, int h, Bits<D>* __restrict__ y,
                                                                 long long y_stride) {
     constexpr int E = Vec<D>::E;
+    constexpr bool ODD = Form::odd;
     const int j = blockIdx.y * blockDim.x + threadIdx.x;
     const long long n = tokens * top;
-    for (long long t = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y; t < tokens;
-         t += static_cast<long long>(gridDim.x) * blockDim.y) {
+    for (long long t = static_cast<long long>(blockIdx.x) * rows_per_block<Form>() + row_in_block<Form>(); t < tokens;
+         t += static_cast<long long>(gridDim.x) * rows_per_block<Form>()) {
         Bits<D>* to = y + t * y_stride;
         const int c = j * E - shift_of<ODD, D>(to);
         if (c >= h) continue;
@@ -213,18 +215,14 @@ cudaError_t LaunchExpertDispatch(const void* x, long long x_stride, const int* s
     const bool odd = !rows16(x, x_stride, h, size) || !on16(rows);
     return with_type(dtype, [&](auto D) {
         constexpr int kD = decltype(D)::value;
-        auto go = [&](auto O) {
-            constexpr bool ODD = decltype(O)::value != 0;
-            const long long wide = accesses<ODD>(h, Vec<kD>::E);
-            const BlockShape b = block_shape(wide, kTokenThreads);
+        return with_form(odd, h, Vec<kD>::E, kTokenThreads, [&](auto form, long long wide, BlockShape b) {
             const dim3 grid(static_cast<unsigned>(std::min(ceil_div(tokens, b.y), kMaxBlocks)),
                             static_cast<unsigned>(ceil_div(wide, b.x)));
-            dispatch_kernel<kD, ODD><<<grid, dim3(b.x, b.y), 0, stream>>>(
+            dispatch_kernel<kD, decltype(form)><<<grid, dim3(b.x, b.y), 0, stream>>>(
                 static_cast<const Bits<kD>*>(x), x_stride, slots, offsets + experts, tokens, top, static_cast<int>(h),
                 static_cast<Bits<kD>*>(rows));
             return cudaGetLastError();
-        };
-        return odd ? go(Int<1>{}) : go(Int<0>{});
+        });
     });
 }
 
@@ -236,20 +234,18 @@ cudaError_t LaunchExpertCombine(const void* rows, const int* slots, const void* 
     const bool odd = !rows16(y, y_stride, h, size) || !on16(rows);
     return with_types(dtype, wdtype, [&](auto D, auto W) {
         constexpr int kD = decltype(D)::value, kW = decltype(W)::value;
-        auto go = [&](auto O, auto UU) {
-            constexpr bool ODD = decltype(O)::value != 0;
-            constexpr int U = decltype(UU)::value;
-            const long long wide = accesses<ODD>(h, Vec<kD>::E);
-            const BlockShape b = block_shape(wide, kTokenThreads);
+        return with_form(odd, h, Vec<kD>::E, kTokenThreads, [&](auto form, long long wide, BlockShape b) {
             const dim3 grid(static_cast<unsigned>(std::min(ceil_div(tokens, b.y), kMaxBlocks)),
                             static_cast<unsigned>(ceil_div(wide, b.x)));
-            combine_kernel<kD, kW, ODD, U><<<grid, dim3(b.x, b.y), 0, stream>>>(
-                static_cast<const Bits<kD>*>(rows), slots, static_cast<const Bits<kW>*>(weights), tokens, top,
-                static_cast<int>(h), static_cast<Bits<kD>*>(y), y_stride);
-            return cudaGetLastError();
-        };
-        if (top <= 2) return odd ? go(Int<1>{}, Int<2>{}) : go(Int<0>{}, Int<2>{});
-        return odd ? go(Int<1>{}, Int<4>{}) : go(Int<0>{}, Int<8>{});
+            auto go = [&](auto UU) {
+                combine_kernel<kD, kW, decltype(form), decltype(UU)::value><<<grid, dim3(b.x, b.y), 0, stream>>>(
+                    static_cast<const Bits<kD>*>(rows), slots, static_cast<const Bits<kW>*>(weights), tokens, top,
+                    static_cast<int>(h), static_cast<Bits<kD>*>(y), y_stride);
+                return cudaGetLastError();
+            };
+            // Rows in flight; putting ODD rows together takes registers too.
+            return top <= 2 ? go(Int<2>{}) : go(Int<decltype(form)::odd ? 4 : 8>{});
+        });
     });
 }
 
