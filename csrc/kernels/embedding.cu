@@ -131,6 +131,7 @@ struct WindowArgs {
     int accumulate;
     int tile;            // rows that a block clears at a time
     int window_blocks;   // blocks of windows, the others clear
+    int join_windows;    // windows that a block of the join looks at
 };
 
 constexpr int kMaxTile = 4096;
@@ -249,47 +250,82 @@ __global__ void __launch_bounds__(kThreads) window_kernel(const WindowArgs a, co
     }
 }
 
-// The window in which a token begins that runs over its right edge adds the token's partial rows.
+// The window in which a token begins that runs over its right edge adds the token's partial rows. A
+// block looks at up to kJoinWindows windows at once (fewer where that leaves SMs idle), most of which have
+// nothing to join, for kJoinColumns accesses of columns; its kJoinParts rows of threads add consecutive shares of the partial rows and
+// are then added in order. (With one row of threads a token in 737 windows took 52 us.)
+constexpr int kJoinColumns = 32, kJoinParts = 8, kJoinWindows = 8, kJoinFlight = 4;
+
 template <int OD, int E, bool ODD>
-__global__ void __launch_bounds__(kThreads) join_kernel(const WindowArgs a, Bits<OD>* __restrict__ dtable) {
-    const long long w = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y;
-    const long long end = (w + 1) * a.window;  // windows but the last are full
-    if (end >= a.n) return;
-    const unsigned int row = __ldg(&a.sorted[end - 1].x);
-    if (row >= a.rows || __ldg(&a.sorted[end].x) != row) return;
-    const long long begin = w * a.window;
-    if (begin > 0 && __ldg(&a.sorted[begin - 1].x) == row) return;  // it began in an earlier window
-    const int j = blockIdx.y * blockDim.x + threadIdx.x;
-    Bits<OD>* to = dtable + static_cast<long long>(row) * a.h;
-    const int c = j * E - shift_of<ODD, OD>(to);
-    if (c >= a.h) return;
-    // The last window that holds the token, which is the last whose first position has it: mostly the
-    // next one, so search in growing steps.
-    long long lo = w + 1, step = 1;
-    while (lo + step < a.windows && __ldg(&a.sorted[(lo + step) * a.window].x) == row) {
-        lo += step;
-        step *= 2;
-    }
-    for (; step > 1; step /= 2) {
-        const long long mid = lo + step / 2;
-        if (mid < a.windows && __ldg(&a.sorted[mid * a.window].x) == row) lo = mid;
-    }
-    float sum[E];
-    load_f<kF32, E>(reinterpret_cast<const Bits<kF32>*>(a.partial + (w * 2 + 1) * a.width + j * E), sum);
-    for (long long k0 = w + 1; k0 <= lo; k0 += kFlight) {
-        float f[kFlight][E];
-#pragma unroll
-        for (int u = 0; u < kFlight; ++u)
-            if (k0 + u <= lo)
-                load_f<kF32, E>(reinterpret_cast<const Bits<kF32>*>(a.partial + (k0 + u) * 2 * a.width + j * E), f[u]);
-#pragma unroll
-        for (int u = 0; u < kFlight; ++u) {
-            if (k0 + u > lo) break;
-#pragma unroll
-            for (int e = 0; e < E; ++e) sum[e] += f[u][e];
+__global__ void __launch_bounds__(kJoinColumns * kJoinParts) join_kernel(const WindowArgs a, Bits<OD>* __restrict__ dtable) {
+    __shared__ float parts[kJoinParts][kJoinColumns][E + 1];
+    __shared__ long long last_of[kJoinWindows];  // last window of the token that begins in each and goes on, or -1
+    const long long w0 = static_cast<long long>(blockIdx.x) * a.join_windows;
+    if (threadIdx.y == 0 && threadIdx.x < a.join_windows) {
+        const long long w = w0 + threadIdx.x, begin = w * a.window, end = begin + a.window;
+        long long last = -1;
+        if (end < a.n) {  // windows but the last are full
+            const unsigned int row = __ldg(&a.sorted[end - 1].x), right = __ldg(&a.sorted[end].x);
+            const unsigned int left = begin > 0 ? __ldg(&a.sorted[begin - 1].x) : 0xffffffffu;
+            if (row < a.rows && right == row && left != row) {  // left == row: it began in an earlier window
+                // The last window whose first position has the token: mostly the next one, so search
+                // in growing steps.
+                long long step = 1;
+                last = w + 1;
+                while (last + step < a.windows && __ldg(&a.sorted[(last + step) * a.window].x) == row) {
+                    last += step;
+                    step *= 2;
+                }
+                for (; step > 1; step /= 2) {
+                    const long long mid = last + step / 2;
+                    if (mid < a.windows && __ldg(&a.sorted[mid * a.window].x) == row) last = mid;
+                }
+            }
         }
+        last_of[threadIdx.x] = last;
     }
-    write_row<OD, E, ODD>(to, c, a.h, sum, a.scale, a.accumulate != 0);
+    __syncthreads();
+    const int j = blockIdx.y * kJoinColumns + threadIdx.x;
+    for (int i = 0; i < a.join_windows; ++i) {
+        const long long w = w0 + i, last = last_of[i];
+        if (last < 0) continue;
+        float sum[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum[e] = 0.0f;
+        const long long share = (last - w + kJoinParts) / kJoinParts;  // of last - w + 1 partial rows
+        const long long k1 = min(last + 1, w + (threadIdx.y + 1) * share);
+        if (j * E < a.width) {
+            for (long long k0 = w + threadIdx.y * share; k0 < k1; k0 += kJoinFlight) {
+                float f[kJoinFlight][E];
+#pragma unroll
+                for (int u = 0; u < kJoinFlight; ++u)
+                    if (k0 + u < k1)
+                        load_f<kF32, E>(reinterpret_cast<const Bits<kF32>*>(
+                                            a.partial + ((k0 + u) * 2 + (k0 + u == w ? 1 : 0)) * a.width + j * E),
+                                        f[u]);
+#pragma unroll
+                for (int u = 0; u < kJoinFlight; ++u) {
+                    if (k0 + u >= k1) break;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) sum[e] += f[u][e];
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) parts[threadIdx.y][threadIdx.x][e] = sum[e];
+        __syncthreads();
+        const unsigned int row = __ldg(&a.sorted[(w + 1) * a.window].x);
+        Bits<OD>* to = dtable + static_cast<long long>(row) * a.h;
+        const int c = j * E - shift_of<ODD, OD>(to);
+        if (threadIdx.y == 0 && c < a.h) {
+            for (int p = 1; p < kJoinParts; ++p) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) sum[e] += parts[p][threadIdx.x][e];
+            }
+            write_row<OD, E, ODD>(to, c, a.h, sum, a.scale, a.accumulate != 0);
+        }
+        __syncthreads();
+    }
 }
 
 // Positions per window: long ones make fewer partial rows, short ones more threads (150000 fill the
@@ -406,14 +442,17 @@ cudaError_t LaunchEmbeddingBackward(const EmbeddingArgs& a, const void* dy, long
             w.tile = static_cast<int>(std::min<long long>(kMaxTile, std::max(1ll, tile)));
             const long long clear = accumulate ? 0 : std::min(1ll << 20, ceil_div(a.rows, w.tile));
             w.window_blocks = static_cast<int>(ceil_div(w.windows, b.y));
+            w.join_windows = static_cast<int>(
+                std::min<long long>(kJoinWindows, std::max(1ll, w.windows * ceil_div(wide, kJoinColumns) / (8 * sm_count()))));
             const size_t smem = sizeof(uint2) * b.y * (w.window + 2);
             window_kernel<kD, kO, Form>
                 <<<dim3(static_cast<unsigned>(w.window_blocks + clear), cols), dim3(b.x, b.y), smem, stream>>>(
                     w, static_cast<const Bits<kD>*>(dy), dy_stride, static_cast<Bits<kO>*>(dtable));
             cudaError_t err = cudaGetLastError();
             if (err != cudaSuccess || w.windows == 1) return err;
-            join_kernel<kO, E, Form::odd><<<dim3(static_cast<unsigned>(w.window_blocks), cols), dim3(b.x, b.y), 0, stream>>>(
-                w, static_cast<Bits<kO>*>(dtable));
+            const dim3 grid(static_cast<unsigned>(ceil_div(w.windows - 1, w.join_windows)),
+                            static_cast<unsigned>(ceil_div(wide, kJoinColumns)));
+            join_kernel<kO, E, Form::odd><<<grid, dim3(kJoinColumns, kJoinParts), 0, stream>>>(w, static_cast<Bits<kO>*>(dtable));
             return cudaGetLastError();
         });
     });
