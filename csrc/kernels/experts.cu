@@ -45,7 +45,7 @@ template <int D, bool ODD>
 __device__ __forceinline__ void clear_tail(Bits<D>* rows, long long kept, long long n, int h, int j0, int dj, long long first,
                                            long long step) {
     constexpr int E = Vec<D>::E;
-    for (long long i = kept + first; i < n; i += step) {
+    for (long long i = max(kept, 0ll) + first; i < n; i += step) {
         Bits<D>* row = rows + i * h;
         const int shift = shift_of<ODD, D>(row);
         for (int c = j0 * E - shift; c < h; c += dj * E) put_raw<ODD, D>(row, c, h, zero_raw<D, E>());

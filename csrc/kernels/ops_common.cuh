@@ -6,7 +6,7 @@
 // each kernel has an ODD form: accesses start on the 16-byte boundaries of the row that is written,
 // `shift` columns before multiples of E; a row read at another alignment is put together from two
 // 16-byte groups, and the first and last access of a row go element by element. (Element accesses
-// throughout were bound by issuing loads: norms over 16384 x 4097 bf16 took @ODD1@ us instead of @ODD8@.)
+// throughout were bound by issuing loads: RMS norm of 16384 x 4097 bf16 took 301 us instead of 59.)
 #pragma once
 
 #include "kernels/common.cuh"
@@ -28,91 +28,70 @@ using dev::Vec;
 template <int D> using Bits = typename Ty<D>::Bits;
 
 // What one access of E elements holds before conversion (kept in registers for prefetching).
-template <int D, int E> struct Raw { uint4 v; };
-template <int D> struct Raw<D, 1> { Bits<D> v; };
+template <int D, int E> struct Raw {
+    static_assert(E == Vec<D>::E, "16 bytes");
+    uint4 v;
+};
 
 template <int D, int E>
 __device__ __forceinline__ Raw<D, E> load_raw(const Bits<D>* p) {
-    Raw<D, E> r;
-    if constexpr (E == 1) r.v = __ldg(p);
-    else r.v = __ldg(reinterpret_cast<const uint4*>(p));
-    return r;
+    return {__ldg(reinterpret_cast<const uint4*>(p))};
 }
-// Streaming form for data that is read once: does not displace what other CTAs keep in L2.
+// Streaming form for data that is read once: does not displace what other blocks keep in L2.
 template <int D, int E>
 __device__ __forceinline__ Raw<D, E> load_raw_cs(const Bits<D>* p) {
-    Raw<D, E> r;
-    if constexpr (E == 1) r.v = __ldcs(p);
-    else r.v = __ldcs(reinterpret_cast<const uint4*>(p));
-    return r;
+    return {__ldcs(reinterpret_cast<const uint4*>(p))};
 }
 template <int D, int E>
 __device__ __forceinline__ void unpack(const Raw<D, E>& r, float (&a)[E]) {
-    if constexpr (E == 1) a[0] = Ty<D>::load(r.v);
-    else Vec<D>::unpack(r.v, a);
+    Vec<D>::unpack(r.v, a);
 }
 template <int D, int E>
 __device__ __forceinline__ Raw<D, E> zero_raw() {
-    Raw<D, E> r;
-    if constexpr (E == 1) r.v = 0;
-    else r.v = make_uint4(0, 0, 0, 0);
-    return r;
+    return {make_uint4(0, 0, 0, 0)};
 }
 
 // E elements of a (possibly wider) type: vectors of parameters next to 16-bit activations.
 template <int D, int E>
 __device__ __forceinline__ void load_f(const Bits<D>* p, float (&a)[E]) {
-    if constexpr (E == 1) {
-        a[0] = Ty<D>::load(__ldg(p));
-    } else {
-        constexpr int W = Vec<D>::E;
-        static_assert(E % W == 0, "whole 16-byte accesses");
+    constexpr int W = Vec<D>::E;
+    static_assert(E % W == 0, "whole 16-byte accesses");
 #pragma unroll
-        for (int i = 0; i < E / W; ++i) {
-            float t[W];
-            Vec<D>::unpack(__ldg(reinterpret_cast<const uint4*>(p) + i), t);
+    for (int i = 0; i < E / W; ++i) {
+        float t[W];
+        Vec<D>::unpack(__ldg(reinterpret_cast<const uint4*>(p) + i), t);
 #pragma unroll
-            for (int e = 0; e < W; ++e) a[i * W + e] = t[e];
-        }
+        for (int e = 0; e < W; ++e) a[i * W + e] = t[e];
     }
 }
 template <int D, int E>
 __device__ __forceinline__ void store_f(Bits<D>* p, const float (&a)[E]) {
-    if constexpr (E == 1) {
-        *p = Ty<D>::store(a[0]);
-    } else {
-        constexpr int W = Vec<D>::E;
-        static_assert(E % W == 0, "whole 16-byte accesses");
+    constexpr int W = Vec<D>::E;
+    static_assert(E % W == 0, "whole 16-byte accesses");
 #pragma unroll
-        for (int i = 0; i < E / W; ++i) {
-            float t[W];
+    for (int i = 0; i < E / W; ++i) {
+        float t[W];
 #pragma unroll
-            for (int e = 0; e < W; ++e) t[e] = a[i * W + e];
-            *(reinterpret_cast<uint4*>(p) + i) = Vec<D>::pack(t);
-        }
+        for (int e = 0; e < W; ++e) t[e] = a[i * W + e];
+        *(reinterpret_cast<uint4*>(p) + i) = Vec<D>::pack(t);
     }
 }
 // Streaming stores for outputs far larger than what is read again soon.
 template <int D, int E>
 __device__ __forceinline__ void store_f_cs(Bits<D>* p, const float (&a)[E]) {
-    if constexpr (E == 1) {
-        __stcs(p, Ty<D>::store(a[0]));
-    } else {
-        constexpr int W = Vec<D>::E;
-        static_assert(E % W == 0, "whole 16-byte accesses");
+    constexpr int W = Vec<D>::E;
+    static_assert(E % W == 0, "whole 16-byte accesses");
 #pragma unroll
-        for (int i = 0; i < E / W; ++i) {
-            float t[W];
+    for (int i = 0; i < E / W; ++i) {
+        float t[W];
 #pragma unroll
-            for (int e = 0; e < W; ++e) t[e] = a[i * W + e];
-            __stcs(reinterpret_cast<uint4*>(p) + i, Vec<D>::pack(t));
-        }
+        for (int e = 0; e < W; ++e) t[e] = a[i * W + e];
+        __stcs(reinterpret_cast<uint4*>(p) + i, Vec<D>::pack(t));
     }
 }
 template <int D, int E>
 __device__ __forceinline__ void store_raw_cs(Bits<D>* p, const Raw<D, E>& r) {
-    if constexpr (E == 1) __stcs(p, r.v);
-    else __stcs(reinterpret_cast<uint4*>(p), r.v);
+    __stcs(reinterpret_cast<uint4*>(p), r.v);
 }
 
 // ---------------------------------------------------------------- rows of any alignment
@@ -300,7 +279,6 @@ __device__ __forceinline__ float inv_sqrt(float v) {
     return fabsf(d) < 1.0f ? fmaf(0.5f * r, d, r) : r;
 }
 
-inline bool float_type(int d) { return d == kF32 || d == kBF16 || d == kF16; }
 inline int size_of(int d) { return d == kF32 || d == kI32 ? 4 : d == kI64 ? 8 : 2; }
 inline bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 // Rows of `h` elements, `stride` apart from `p`, that all start and end on 16-byte boundaries.

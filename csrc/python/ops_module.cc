@@ -144,6 +144,20 @@ int64_t out_rows(const char* op, const Tensor& out, at::IntArrayRef shape, at::S
     if (out.dim() == 2 && (h == 1 || out.stride(1) == 1) && out.stride(0) >= h) return out.stride(0);
     value_error(std::string(op) + ": out must have rows of adjacent elements, evenly spaced and apart");
 }
+// The bytes between a tensor's first and last element.
+std::pair<uint64_t, uint64_t> extent(const Tensor& t) {
+    if (t.numel() == 0) return {0, 0};
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    const auto from = reinterpret_cast<uint64_t>(t.data_ptr());
+    return {from, from + static_cast<uint64_t>(last + 1) * t.element_size()};
+}
+// An output must not lie in what is read while it is written.
+void apart(const char* op, const Tensor& out, const Tensor& in) {
+    const auto [a, b] = extent(out);
+    const auto [c, d] = extent(in);
+    if (a < d && c < b) value_error(std::string(op) + ": out must not overlap an input");
+}
 void* data(const Tensor& t) { return t.numel() == 0 ? nullptr : t.data_ptr(); }
 void* data(const Optional& t) { return t ? data(*t) : nullptr; }
 // A tensor of the caller's that a kernel writes: autograd must see that it changed.
@@ -231,6 +245,10 @@ PyObject* NormForward(PyObject* const* a) {
     if (!(eps >= 0.0)) value_error(std::string(op) + ": eps must not be negative or NaN");
     const int device = one_device(op, x, o.weight, o.bias, given);
     const Rows xr(x, o.h);
+    // In place is fine: a row is read before it is written.
+    if (given && !(given->data_ptr() == x.data_ptr() && given->strides() == x.strides())) apart(op, *given, x);
+    if (given && o.weight) apart(op, *given, *o.weight);
+    if (given && o.bias) apart(op, *given, *o.bias);
     const int64_t stride = given ? out_rows(op, *given, x.sizes(), x.scalar_type()) : o.h;
     const Tensor y = given ? written(*given) : at::empty(x.sizes(), x.options());
     const auto lead = x.sizes().slice(0, x.dim() - 1);
@@ -301,6 +319,8 @@ PyObject* EmbeddingForward(PyObject* const* a) {
     const int64_t h = weight.size(1);
     at::DimVector shape(ids.sizes().begin(), ids.sizes().end());
     shape.push_back(h);
+    if (given) apart(op, *given, weight);
+    if (given) apart(op, *given, ids);
     const int64_t stride = given ? out_rows(op, *given, shape, weight.scalar_type()) : h;
     const Tensor out = given ? written(*given) : at::empty(shape, weight.options()), i = ids.contiguous();
     const Rows w(weight, h);
@@ -331,6 +351,8 @@ PyObject* EmbeddingBackward(PyObject* const* a) {
     const int64_t h = dy.size(-1);
     if (given && (given->sizes() != at::IntArrayRef({rows, h}) || !given->is_contiguous()))
         value_error(std::string(op) + ": out must be a contiguous " + shape_of({rows, h}) + " tensor, got " + shape_of(*given));
+    if (given) apart(op, *given, dy);
+    if (given) apart(op, *given, ids);
     const int ocode = given ? like_or_f32(op, "out", *given, dy.scalar_type()) : code;
     const Tensor out = given ? written(*given) : at::empty({rows, h}, dy.options());
     const Tensor i = ids.contiguous();
@@ -416,6 +438,7 @@ PyObject* Dispatch(PyObject* const* a) {
                   !given->is_contiguous()))
         value_error(std::string(op) + ": out must be a contiguous " + type_of(x.scalar_type()) + " tensor of shape " +
                     shape_of({o.n, h}) + ", got " + type_of(given->scalar_type()) + " " + shape_of(*given));
+    if (given) apart(op, *given, x);
     const Tensor rows = given ? written(*given) : at::empty({o.n, h}, x.options());
     const Rows xr(x, h);
     launch(device, [&](void* s) {

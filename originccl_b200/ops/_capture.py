@@ -1,0 +1,26 @@
+"""A backward pass must not be captured into a CUDA graph while an eager graph of the same leaves lives.
+
+Autograd gives each leaf one accumulation node for as long as any graph refers to it, and runs it on the
+stream on which it was made. If an eager forward pass made it on another stream and its output is
+still held, a captured backward pass would wait for that stream, which a capture may not do; the
+error ends the process. :func:`guard` marks the nodes of an operator's leaves with the stream of their
+pass and refuses the capture's forward pass instead.
+"""
+from __future__ import annotations
+
+import torch
+
+_KEY = "bccl_stream"
+
+
+def guard(op: str, *inputs) -> None:
+    """Called first in the forward pass of a differentiable operator, with its tensor inputs."""
+    for t in inputs:
+        if t is None or not t.requires_grad or not t.is_leaf:
+            continue
+        stream = torch.cuda.current_stream(t.device).cuda_stream if t.is_cuda else 0
+        marks = torch.autograd.graph.get_gradient_edge(t).node.metadata
+        made = marks.setdefault(_KEY, stream)
+        if made != stream and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{op}: an eager graph of the same leaf tensors, made on another stream, is still alive; "
+                               "release its outputs (the loss) before the backward pass is captured")

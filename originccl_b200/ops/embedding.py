@@ -18,6 +18,7 @@ from typing import Optional
 import torch
 
 from .. import _native
+from ._capture import guard
 
 _ops = _native.ops()
 
@@ -39,6 +40,7 @@ def embedding_backward(dy, ids, num_rows: int, scale: float = 1.0, first_row: in
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, scale, padding_idx, first_row):
+        guard("embedding", weight)
         ctx.save_for_backward(ids)
         ctx.args = weight.shape[0], scale, first_row, padding_idx
         return embedding_forward(ids, weight, scale, first_row)

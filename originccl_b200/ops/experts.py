@@ -21,6 +21,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _native
+from ._capture import guard
 
 MAX_EXPERTS = 1023
 MAX_TOP = 64
@@ -90,6 +91,7 @@ def combine_backward(dy, rows, order: ExpertOrder, weights=None, *, weight_grad:
 class _Dispatch(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, order):
+        guard("dispatch", x)
         ctx.order = order
         return dispatch_forward(x, order)
 
@@ -102,6 +104,7 @@ class _Dispatch(torch.autograd.Function):
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, weights, order):
+        guard("combine", rows, weights)
         ctx.save_for_backward(rows, weights)
         ctx.order = order
         return combine_forward(rows, order, weights)

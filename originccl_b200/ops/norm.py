@@ -16,6 +16,7 @@ from typing import Tuple
 import torch
 
 from .. import _native
+from ._capture import guard
 
 _LAYER, _RMS = 0, 1
 _ops = _native.ops()
@@ -46,6 +47,7 @@ def rms_norm_backward(dy, x, rstd, weight=None, *, weight_grad: bool = True) -> 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
+        guard("layer_norm", x, weight, bias)
         y, mean, rstd = layer_norm_forward(x, weight, bias, eps)
         ctx.save_for_backward(x, weight, mean, rstd)
         return y
@@ -62,6 +64,7 @@ class _LayerNorm(torch.autograd.Function):
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, eps):
+        guard("rms_norm", x, weight)
         y, rstd = rms_norm_forward(x, weight, eps)
         ctx.save_for_backward(x, weight, rstd)
         return y

@@ -681,3 +681,117 @@ def test_tokens_go_to_their_experts_and_back():
         size += 2.0 ** -8 * term.abs() + (h + 8) * U * bound  # an answer is rounded to bf16 once
     check(y, exact, size)
     comm.destroy()
+
+
+# ---------------------------------------------------------------- refusals that need a GPU, large offsets
+def test_overlapping_tensors_are_not_clipped():
+    from originccl_b200.ops import gradients
+    flat = randn(1000, torch.float32, 1)
+    keep = flat.clone()
+    for grads, outs in (([flat[:600], flat[500:]], None),               # overlap in place
+                        ([flat, flat], None),                           # the same tensor twice
+                        ([flat[:400], flat[400:800]], [flat[100:500], flat[600:]]),
+                        ([flat[:100], flat[100:200]], [flat[100:200], flat[:100]]),  # each other's place
+                        ([flat[:100], flat[100:200]], [torch.empty(100, device="cuda")] * 2)):
+        if outs is not None and [o.numel() for o in outs] != [g.numel() for g in grads]:
+            outs = [o[:g.numel()] for o, g in zip(outs, grads)]
+        with pytest.raises(ValueError, match="overlap"):
+            gradients.clip_grad_norm(grads, 1e-3, outs=outs)
+    with pytest.raises(TypeError, match="float32"):
+        gradients.clip_grad_norm([flat], 1.0, outs=[torch.empty(1000, device="cuda", dtype=torch.float16)])
+    with pytest.raises(ValueError, match="shape"):
+        gradients.clip_grad_norm([flat], 1.0, outs=[torch.empty(10, 100, device="cuda")])
+    with pytest.raises(ValueError, match="dense"):
+        gradients.clip_grad_norm([flat[::2]], 1.0)
+    with pytest.raises(ValueError, match="one device"):
+        gradients.clip_grad_norm([flat, torch.zeros(3)], 1.0)
+    assert torch.equal(flat, keep)
+    gradients.clip_grad_norm([flat[:0], flat[:0], flat], 1e-3, outs=None)  # empty tensors share nothing
+    assert not torch.equal(flat, keep)
+
+
+def test_outputs_that_are_written_count_as_changed():
+    """Autograd notices that a tensor it saved was written by an operator."""
+    from originccl_b200.ops import gradients, norm
+    x = randn((4, 64), torch.float32, 1)
+    a = torch.ones(4, 64, device="cuda", requires_grad=True)
+    y = a * x
+    norm.rms_norm_forward(x, out=x)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+    before = x._version
+    gradients.clip_grad_norm([x], 1.0)
+    assert x._version > before
+
+
+def test_offsets_beyond_32_bits():
+    from originccl_b200.ops import embedding, experts as ex, gradients, norm
+    rows, h = 600_000, 4096  # 2.46e9 elements
+    big = torch.zeros(rows, h, device="cuda", dtype=torch.bfloat16)
+    ids = torch.tensor([0, rows - 1, rows - 1, rows - 7], device="cuda")
+    big[-8:] = randn((8, h), torch.bfloat16, 1)
+    assert torch.equal(embedding.embedding_forward(ids, big), big[ids])
+    y, rstd = norm.rms_norm_forward(big)
+    check(y[-8:], norm64("rms", big[-8:], None, None, 1e-5)[0], 64 * U * big[-8:].double().abs().amax() * 2)
+    assert y[:-8].abs().amax() == 0
+    dx, _ = norm.rms_norm_backward(big, big, rstd)
+    assert dx[:-8].abs().amax() == 0 and dx[-8:].abs().amax() > 0
+    total = gradients.clip_grad_norm([big], 1.0, outs=[y])
+    exact = big[-8:].double().norm()
+    check(total, exact, 34 * U * exact)
+    check(y[-8:], big[-8:].double() / (float(exact) + 1e-6), 40 * U * big[-8:].double().abs())
+    del y, dx
+    dy = randn((4, h), torch.bfloat16, 2)
+    grad = embedding.embedding_backward(dy, ids, rows, out=big)
+    assert torch.equal(grad[0], dy[0]) and torch.equal(grad[rows - 7], dy[3]) and grad[1:rows - 7].abs().amax() == 0
+    check(grad[rows - 1], dy[1].double() + dy[2].double(), 2 * U * (dy[1].double().abs() + dy[2].double().abs()))
+    order = ex.sort_by_expert(torch.arange(rows, device="cuda").remainder(2).reshape(-1, 2), 2)
+    x = torch.arange(rows // 2, device="cuda", dtype=torch.float32)[:, None].remainder(251).to(torch.bfloat16).expand(-1, h)
+    ex.dispatch_forward(x, order, out=big)
+    assert torch.equal(big[:, 0], x[order.sources.long() // 2, 0]) and torch.equal(big[:, 0], big[:, -1])
+    assert torch.equal(ex.combine_forward(big, order), x.contiguous() * 2)
+
+
+def test_a_backward_pass_is_captured():
+    from originccl_b200.ops import norm
+    from originccl_b200.utils.graphs import capture
+    x = randn((64, 256), torch.float32, 1).requires_grad_()
+    w = randn(256, torch.float32, 2).requires_grad_()
+    t = randn((64, 256), torch.float32, 3)
+    x.grad, w.grad = torch.zeros_like(x), torch.zeros_like(w)
+
+    def step():
+        x.grad.zero_()
+        w.grad.zero_()
+        (norm.rms_norm(x, w) * t).sum().backward()
+    step()
+    g = capture(step)
+    want = []
+    for seed in (4, 5):
+        with torch.no_grad():
+            x.copy_(randn((64, 256), torch.float32, seed))
+        g.replay()
+        torch.cuda.synchronize()
+        got = x.grad.clone(), w.grad.clone()
+        _, rstd = norm.rms_norm_forward(x.detach(), w.detach())
+        want = norm.rms_norm_backward(t, x.detach(), rstd, w.detach())
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_outputs_in_their_inputs_are_refused():
+    from originccl_b200.ops import embedding, experts as ex, norm
+    buf = randn(4096, torch.float32, 1)
+    x = buf[:1024].view(16, 64)
+    with pytest.raises(ValueError, match="overlap"):
+        norm.rms_norm_forward(x, out=buf[64:1088].view(16, 64))
+    with pytest.raises(ValueError, match="overlap"):
+        norm.rms_norm_forward(x, buf[1000:1064], out=buf[1024:2048].view(16, 64))
+    ids = torch.zeros(16, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        embedding.embedding_forward(ids, x, out=x)
+    with pytest.raises(ValueError, match="overlap"):
+        embedding.embedding_backward(x, ids, 16, out=x)
+    order = ex.sort_by_expert(ids, 2)
+    with pytest.raises(ValueError, match="overlap"):
+        ex.dispatch_forward(x, order, out=buf[960:1984].view(16, 64))
+    ex.dispatch_forward(x, order, out=buf[1024:2048].view(16, 64))

@@ -229,3 +229,32 @@ def test_the_c_interface_refuses():
     refused(lib.bcclExpertCombine(p(64), p(64), p(64), 4, 4, 2, 8, p(64), 8, 0, None), "dtypes")
     refused(lib.bcclExpertCombine(p(64), None, p(64), 0, 4, 2, 8, p(64), 8, 0, None), "null")
     refused(lib.bcclExpertCombineBackward(p(64), 8, p(0), p(64), p(64), p(64), 0, 4, 2, 8, 8, p(64), p(64), 0, None), "null")
+
+
+def test_a_capture_beside_an_eager_graph_of_the_same_leaves_is_refused(monkeypatch):
+    """The guard's rule with stand-ins for the stream and the capture: the leaf's accumulation node was
+    made on another stream and still lives."""
+    from originccl_b200.ops import _capture
+    leaf = torch.ones(3, requires_grad=True)
+
+    class Op(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            _capture.guard("op", x)
+            return x * 2
+
+        @staticmethod
+        def backward(ctx, g):
+            return g * 2
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    held = Op.apply(leaf)                          # an eager graph, stream 0
+    marks = torch.autograd.graph.get_gradient_edge(leaf).node.metadata
+    assert marks[_capture._KEY] == 0
+    marks[_capture._KEY] = 7                       # as if made on stream 7
+    Op.apply(leaf)                              # fine while nothing is captured
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="still alive"):
+        Op.apply(leaf)
+    del held, marks
+    Op.apply(leaf)                              # the eager graph is gone, and its node with it
