@@ -36,18 +36,18 @@ __global__ void __launch_bounds__(kThreads) lookup_kernel(const KeySource key, l
     for (long long i0 = (static_cast<long long>(blockIdx.x) * rows_per_block<Form>() + row_in_block<Form>()) * TOKENS; i0 < n;
          i0 += step) {
         unsigned int row[TOKENS];
-        Raw<D, E> r[TOKENS];
 #pragma unroll
         for (int t = 0; t < TOKENS; ++t)
             row[t] = i0 + t < n ? key(i0 + t) : static_cast<unsigned int>(key.bins);
+        Started<ODD> r[TOKENS];
 #pragma unroll
         for (int t = 0; t < TOKENS; ++t) {
-            if constexpr (!ODD) {
-                r[t] = row[t] < key.bins ? load_raw<D, E>(table + row[t] * table_stride + j * E) : zero_raw<D, E>();
+            const Bits<D>* from = table + row[t] * table_stride;
+            if constexpr (!ODD) {  // rows of frequent tokens stay in L1 and L2
+                r[t].lo = row[t] < key.bins ? __ldg(reinterpret_cast<const uint4*>(from + j * E)) : make_uint4(0, 0, 0, 0);
             } else {
                 const int c = j * E - shift_of<ODD, D>(out + (i0 + t) * out_stride);
-                r[t] = zero_raw<D, E>();
-                if (row[t] < key.bins && c < h) r[t] = get_row<ODD, D>(table + row[t] * table_stride, c, h);
+                r[t] = start_row<ODD, D>(from, c, h, row[t] < key.bins && c < h);
             }
         }
 #pragma unroll
@@ -56,11 +56,12 @@ __global__ void __launch_bounds__(kThreads) lookup_kernel(const KeySource key, l
             const int c = j * E - shift_of<ODD, D>(to);
             if (i0 + t >= n) break;
             if (ODD && c >= h) continue;
+            const Raw<D, E> v = finish_row<ODD, D>(r[t], table + row[t] * table_stride, c, h, row[t] < key.bins);
             if (scale == 1.0f) {
-                put_raw<ODD, D>(to, c, h, r[t]);
+                put_raw<ODD, D>(to, c, h, v);
             } else {
                 float f[E];
-                unpack<D, E>(r[t], f);
+                unpack<D, E>(v, f);
 #pragma unroll
                 for (int e = 0; e < E; ++e) f[e] = row[t] < key.bins ? f[e] * scale : 0.0f;
                 put_row<ODD, D, E>(to, c, h, f);
@@ -208,33 +209,30 @@ __global__ void __launch_bounds__(kThreads) window_kernel(const WindowArgs a, co
 #pragma unroll
     for (int e = 0; e < E; ++e) sum[e] = 0.0f;
     bool from_left = count > 0 && it[-1].x == it[0].x;
-    for (int i0 = 0; i0 < count; i0 += kFlight) {
-        Raw<D, E> r[kFlight];
+    constexpr int U = ODD ? kFlight / 2 : kFlight;  // putting ODD rows together takes registers
+    for (int i0 = 0; i0 < count; i0 += U) {
+        Started<ODD> r[U];
 #pragma unroll
-        for (int u = 0; u < kFlight; ++u) {
-            const bool in = i0 + u < count && it[i0 + u].x < a.rows;
-            r[u] = zero_raw<D, E>();
-            if constexpr (!ODD) {
-                if (in) r[u] = load_raw_cs<D, E>(dy + static_cast<long long>(it[i0 + u].y) * dy_stride + j * E);
-            } else if (in) {
-                const int c = j * E - shift_of<ODD, OD>(dtable + static_cast<long long>(it[i0 + u].x) * h);
-                if (c < h) r[u] = get_row<ODD, D>(dy + static_cast<long long>(it[i0 + u].y) * dy_stride, c, h);
-            }
+        for (int u = 0; u < U; ++u) {
+            const uint2 item = i0 + u < count ? it[i0 + u] : make_uint2(0xffffffffu, 0);
+            const bool in = item.x < a.rows;
+            const int c = j * E - (in ? shift_of<ODD, OD>(dtable + static_cast<long long>(item.x) * h) : 0);
+            r[u] = start_row<ODD, D>(dy + static_cast<long long>(item.y) * dy_stride, c, h, in && (!ODD || c < h));
         }
 #pragma unroll
-        for (int u = 0; u < kFlight; ++u) {
+        for (int u = 0; u < U; ++u) {
             const int i = i0 + u;
             if (i >= count) break;
             const unsigned int row = it[i].x;
             if (row >= a.rows) return;  // sorted last: nothing but dropped positions follows
+            Bits<OD>* to = dtable + static_cast<long long>(row) * h;
+            const int c = j * E - shift_of<ODD, OD>(to);
             float f[E];
-            unpack<D, E>(r[u], f);
+            unpack<D, E>(finish_row<ODD, D>(r[u], dy + static_cast<long long>(it[i].y) * dy_stride, c, h, c < h), f);
 #pragma unroll
             for (int e = 0; e < E; ++e) sum[e] += f[e];
             if (it[i + 1].x == row && i + 1 < count) continue;
             const bool to_right = it[i + 1].x == row;
-            Bits<OD>* to = dtable + static_cast<long long>(row) * h;
-            const int c = j * E - shift_of<ODD, OD>(to);
             if (ODD && c >= h) {
                 // nothing of this row in this thread
             } else if (from_left || to_right) {
@@ -253,7 +251,7 @@ __global__ void __launch_bounds__(kThreads) window_kernel(const WindowArgs a, co
 // The window in which a token begins that runs over its right edge adds the token's partial rows. A
 // block looks at up to kJoinWindows windows at once (fewer where that leaves SMs idle), most of which have
 // nothing to join, for kJoinColumns accesses of columns; its kJoinParts rows of threads add consecutive shares of the partial rows and
-// are then added in order. (With one row of threads a token in 737 windows took 52 us.)
+// are then added in order. (With one row of threads a token in 737 windows took 52 us, so 24.)
 constexpr int kJoinColumns = 32, kJoinParts = 8, kJoinWindows = 8, kJoinFlight = 4;
 
 template <int OD, int E, bool ODD>
@@ -362,7 +360,7 @@ cudaError_t LaunchEmbeddingForward(const EmbeddingArgs& a, const void* table, lo
                 return cudaGetLastError();
             };
             // Few accesses: one row each, on as many SMs as there are.
-            return a.n * wide < 16ll * kThreads * sm_count() ? go(Int<1>{}) : go(Int<4>{});
+            return a.n * wide < 16ll * kThreads * sm_count() ? go(Int<1>{}) : go(Int<decltype(form)::odd ? 2 : 4>{});
         });
     });
 }

@@ -101,19 +101,20 @@ __global__ void __launch_bounds__(kTokenThreads) combine_kernel(const Bits<D>* _
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = 0.0f;
         for (int k0 = 0; k0 < top; k0 += U) {
-            Raw<D, E> r[U];
+            Started<ODD> r[U];
+            int slot[U];
             float w[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int slot = k0 + u < top ? __ldg(slots + t * top + k0 + u) : -1;
-                const bool kept = in_rows(slot, n);
-                r[u] = kept ? get_row<ODD, D>(rows + static_cast<long long>(slot) * h, c, h) : zero_raw<D, E>();
+                slot[u] = k0 + u < top ? __ldg(slots + t * top + k0 + u) : -1;
+                const bool kept = in_rows(slot[u], n);
+                r[u] = start_row<ODD, D>(rows + static_cast<long long>(slot[u]) * h, c, h, kept);
                 w[u] = !kept ? 0.0f : weights == nullptr ? 1.0f : Ty<WD>::load(__ldg(weights + t * top + k0 + u));
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 float f[E];
-                unpack<D, E>(r[u], f);
+                unpack<D, E>(finish_row<ODD, D>(r[u], rows + static_cast<long long>(slot[u]) * h, c, h, in_rows(slot[u], n)), f);
 #pragma unroll
                 for (int e = 0; e < E; ++e) acc[e] = fmaf(w[u], f[e], acc[e]);
             }
@@ -150,7 +151,7 @@ __global__ void __launch_bounds__(kTokenThreads) combine_backward_kernel(
             const long long at = static_cast<long long>(slot) * h;
             const int shift = drows != nullptr ? shift_of<ODD, D>(drows + at) : 0;
             for (int c0 = lane * E - shift; c0 < h; c0 += LANES * kFlight * E) {
-                Raw<D, E> r[kFlight], t[kFlight];
+                Raw<D, E> r[kFlight], t[kFlight];  // ODD rows put together at once: their groups take registers
 #pragma unroll
                 for (int u = 0; u < kFlight; ++u) {
                     const int c = c0 + u * LANES * E;

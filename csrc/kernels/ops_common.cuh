@@ -95,16 +95,11 @@ __device__ __forceinline__ void store_raw_cs(Bits<D>* p, const Raw<D, E>& r) {
 }
 
 // ---------------------------------------------------------------- rows of any alignment
-// 16 bytes from any element boundary, by 16-byte groups that each hold some of them (so they lie in the
-// allocation that holds the row, whatever comes before and behind it).
+// 16 bytes from any element boundary are put together from the one or two 16-byte groups that hold them
+// (and so lie in the allocation that holds the row, whatever comes before and behind it).
 template <int D>
-__device__ __forceinline__ uint4 load_unaligned(const Bits<D>* p) {
-    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
-    const unsigned int k = a & 15;
-    const uint4* group = reinterpret_cast<const uint4*>(a - k);
-    const uint4 lo = __ldg(group);
-    if (k == 0) return lo;
-    const uint4 hi = __ldg(group + 1);
+__device__ __forceinline__ uint4 join_groups(const Bits<D>* p, const uint4& lo, const uint4& hi) {
+    const unsigned int k = reinterpret_cast<uintptr_t>(p) & 15;
     unsigned int w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
     if (k & 4) {
 #pragma unroll
@@ -123,24 +118,48 @@ template <bool ODD, int D>
 __device__ __forceinline__ int shift_of(const Bits<D>* row) {
     return ODD ? static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(Bits<D>)) : 0;
 }
-// Columns [c, c + E) of a row of h; zeros outside it. Not ODD: c is a multiple of E below h.
+// Columns [c, c + E) of a row of h; zeros outside it, and everywhere unless `in`. Not ODD: c is a multiple of
+// E, below h where `in`. Started and finished apart, so that a thread has the loads of several rows in
+// flight: finishing waits for them and, at the ends of an ODD row, loads element by element.
+template <bool ODD> struct Started {
+    uint4 lo;
+};
+template <> struct Started<true> {
+    uint4 lo, hi;
+};
+template <bool ODD, int D>
+__device__ __forceinline__ Started<ODD> start_row(const Bits<D>* row, int c, int h, bool in) {
+    Started<ODD> s;
+    if constexpr (!ODD) {
+        s.lo = in ? __ldcs(reinterpret_cast<const uint4*>(row + c)) : make_uint4(0, 0, 0, 0);
+    } else {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(row + c);
+        const uint4* group = reinterpret_cast<const uint4*>(a & ~static_cast<uintptr_t>(15));
+        in = in && c >= 0 && c + Vec<D>::E <= h;
+        s.lo = in ? __ldg(group) : make_uint4(0, 0, 0, 0);
+        s.hi = in ? __ldg(group + ((a & 15) != 0 ? 1 : 0)) : make_uint4(0, 0, 0, 0);
+    }
+    return s;
+}
+template <bool ODD, int D>
+__device__ __forceinline__ Raw<D, Vec<D>::E> finish_row(const Started<ODD>& s, const Bits<D>* row, int c, int h, bool in) {
+    constexpr int E = Vec<D>::E;
+    Raw<D, E> r;
+    if constexpr (!ODD) {
+        r.v = s.lo;
+    } else if (!in || (c >= 0 && c + E <= h)) {
+        r.v = join_groups<D>(row + c, s.lo, s.hi);
+    } else {
+        dev::V16<D> v;
+#pragma unroll
+        for (int e = 0; e < E; ++e) v.b[e] = c + e >= 0 && c + e < h ? __ldg(row + c + e) : 0;
+        r.v = v.u;
+    }
+    return r;
+}
 template <bool ODD, int D>
 __device__ __forceinline__ Raw<D, Vec<D>::E> get_row(const Bits<D>* row, int c, int h) {
-    constexpr int E = Vec<D>::E;
-    if constexpr (!ODD) {
-        return load_raw_cs<D, E>(row + c);
-    } else {
-        Raw<D, E> r;
-        if (c >= 0 && c + E <= h) {
-            r.v = load_unaligned<D>(row + c);
-        } else {
-            dev::V16<D> v;
-#pragma unroll
-            for (int e = 0; e < E; ++e) v.b[e] = c + e >= 0 && c + e < h ? __ldg(row + c + e) : 0;
-            r.v = v.u;
-        }
-        return r;
-    }
+    return finish_row<ODD, D>(start_row<ODD, D>(row, c, h, true), row, c, h, true);
 }
 // The same as floats, of a type that may be wider (parameters next to 16-bit rows).
 template <bool ODD, int D, int E>
