@@ -56,6 +56,7 @@ const Tensor& tensor(const char* op, const char* what, PyObject* o) {
     if (!THPVariable_Check(o)) type_error(std::string(op) + ": " + what + " must be a tensor");
     const Tensor& t = THPVariable_Unpack(o);
     if (t.layout() != at::kStrided) type_error(std::string(op) + ": " + what + " must be a strided tensor");
+    if (t.is_neg()) type_error(std::string(op) + ": " + what + " must not be a view of negated values");
     return t;
 }
 Optional optional_tensor(const char* op, const char* what, PyObject* o) {

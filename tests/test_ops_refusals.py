@@ -44,6 +44,15 @@ def test_norms_refuse():
         norm.layer_norm_backward(x, x, torch.zeros(4, dtype=bf), torch.zeros(4), w)
 
 
+def test_negated_views_are_refused():
+    x = torch._neg_view(torch.zeros(4, 8))
+    for call in (lambda: norm.rms_norm_forward(x), lambda: embedding.embedding_forward(torch.zeros(2, dtype=torch.long), x),
+                 lambda: experts.dispatch_forward(x, experts.ExpertOrder(
+                     *(torch.zeros(n, dtype=torch.int32) for n in ((4, 1), (4,), (3,)))))):
+        with pytest.raises(TypeError, match="negated"):
+            call()
+
+
 def test_embedding_refuses():
     ids, w = torch.zeros(5, dtype=torch.int64), torch.zeros(6, 8, dtype=bf)
     with pytest.raises(TypeError, match="ids"):
