@@ -2,8 +2,8 @@
 
 ``y = (x - mean) * rstd * weight + bias`` with ``rstd = 1 / sqrt(var + eps)``; RMS norm has no mean and
 no bias. Types: float32, bfloat16, float16; weight and bias have x's type or are float32.
-Statistics are float32, sums are kept in 32 bits, outputs are rounded once. Rows may be of any
-length; a 2-D input may have any row stride. The weights' gradients are summed in a fixed order.
+Statistics are float32, sums are kept in 32 bits, outputs are rounded once. Rows may have up
+to 2^23 elements; a 2-D input may have any row stride. The weights' gradients are summed in a fixed order.
 
 :func:`layer_norm` and :func:`rms_norm` are differentiable; the ``_forward`` / ``_backward`` pairs are the
 same kernels for code that keeps its own activations (pipeline stages, captured steps). The
