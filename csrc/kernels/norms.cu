@@ -177,14 +177,14 @@ template <int D> constexpr int ring_max_threads() { return D == kF32 ? 1024 : 51
 template <int D, int WD, bool LAYER, bool ODD, int STAGES, int NV>
 __global__ void __launch_bounds__(ring_max_threads<D>(), NV == 2 && D != kF32 ? 2 : 1) norm_forward_ring_kernel(const NormForwardArgs a) {
     constexpr int E = Vec<D>::E, P = E / 2;
-    extern __shared__ uint4 ring[];  // [STAGES][NV][threads], then the parameters
+    extern __shared__ uint4 ring[];  // [STAGES][NV][threads], then the weights and biases that there are
     __shared__ float buf[2][32];
     const int tx = threadIdx.x, g = blockDim.x, warps = g >> 5, h = static_cast<int>(a.h);
     const float inv_h = 1.0f / static_cast<float>(h);
     const int shift = shift_of<ODD, D>(static_cast<const Bits<D>*>(a.y) + blockIdx.x * a.y_stride);
     const int c0 = tx * E - shift, dc = g * E;  // columns of access v: c0 + v * dc
     Bits<WD>* w_smem = reinterpret_cast<Bits<WD>*>(ring + STAGES * NV * g) + tx * E;
-    Bits<WD>* b_smem = w_smem + NV * dc;
+    Bits<WD>* b_smem = w_smem + (a.w != nullptr ? NV * dc : 0);
     const long long x_step = static_cast<long long>(gridDim.x) * a.x_stride, y_step = static_cast<long long>(gridDim.x) * a.y_stride;
     const Bits<D>* x = static_cast<const Bits<D>*>(a.x) + blockIdx.x * a.x_stride + c0;  // of the next row to copy
     Bits<D>* y = static_cast<Bits<D>*>(a.y) + blockIdx.x * a.y_stride;
@@ -267,6 +267,10 @@ __global__ void __launch_bounds__(ring_max_threads<D>(), NV == 2 && D != kF32 ? 
 #pragma unroll
                     for (int e = 0; e < P; ++e) f[v][e] = mul2(f[v][e], w[e]);
                 }
+            } else if (LAYER && a.b != nullptr) {
+                read_params<WD, E>(b_smem + v * dc, w);
+#pragma unroll
+                for (int e = 0; e < P; ++e) f[v][e] = add2(f[v][e], w[e]);
             }
             put_row2<ODD, D>(y, c, h, f[v]);
         }

@@ -795,3 +795,25 @@ def test_outputs_in_their_inputs_are_refused():
     with pytest.raises(ValueError, match="overlap"):
         ex.dispatch_forward(x, order, out=buf[960:1984].view(16, 64))
     ex.dispatch_forward(x, order, out=buf[1024:2048].view(16, 64))
+
+
+# ---------------------------------------------------------------- the C interface where Python takes a narrower road
+@pytest.mark.parametrize("dtype,wtype,rows,h", [
+    (torch.bfloat16, torch.float32, 3, 64), (torch.bfloat16, torch.bfloat16, 700, 4096), (torch.float16, torch.float32, 700, 4096),
+    (torch.float16, torch.float32, 3000, 1001), (torch.bfloat16, torch.float32, 400, 9000), (torch.float32, torch.float32, 700, 4096),
+    (torch.float32, torch.float32, 2, 40000)])
+def test_layer_norm_with_a_bias_and_no_weight(dtype, wtype, rows, h):
+    """Each of weight and bias may be missing, in every form of the kernel. m as in check_norm."""
+    from originccl_b200 import _native
+    code = {torch.float32: 0, torch.bfloat16: 4, torch.float16: 5}
+    x, b = randn((rows, h), dtype, 1, 2.0, 0.5), randn(h, wtype, 2, 0.3)
+    y, mean, rstd = torch.empty_like(x), torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+    rc = _native.lib().bcclNormForward(0, x.data_ptr(), h, None, b.data_ptr(), y.data_ptr(), h, mean.data_ptr(), rstd.data_ptr(),
+                                       rows, h, 1e-5, code[dtype], code[wtype], torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, _native.last_error()
+    y64, mean64, rstd64, xh = norm64("layer", x, None, b, 1e-5)
+    size = x.double().abs().mean(-1, keepdim=True) * rstd64[:, None]
+    m = 64 * U
+    check(y, y64, m * (xh.abs() + size) + 2 * U * b.double().abs(), "y")
+    check(mean, mean64, m * x.double().abs().mean(-1), "mean")
+    check(rstd, rstd64, m * rstd64 * (1 + size[:, 0] ** 2 * U), "rstd")
