@@ -57,6 +57,10 @@ const Tensor& tensor(const char* op, const char* what, PyObject* o) {
     const Tensor& t = THPVariable_Unpack(o);
     if (t.layout() != at::kStrided) type_error(std::string(op) + ": " + what + " must be a strided tensor");
     if (t.is_neg()) type_error(std::string(op) + ": " + what + " must not be a view of negated values");
+    // Wrappers (distributed tensors, say) have a shape, a type and a device but no storage of their own, and the
+    // C interface reads a null pointer as "not given": a weight would be left out without a word.
+    if (t.numel() != 0 && t.const_data_ptr() == nullptr)
+        type_error(std::string(op) + ": " + what + " must have memory of its own, got a tensor without storage");
     return t;
 }
 Optional optional_tensor(const char* op, const char* what, PyObject* o) {

@@ -267,3 +267,35 @@ def test_a_capture_beside_an_eager_graph_of_the_same_leaves_is_refused(monkeypat
         Op.apply(leaf)
     del held, marks
     Op.apply(leaf)                              # the eager graph is gone, and its node with it
+
+
+def test_tensors_without_storage_are_refused():
+    """A wrapper has shape, type, layout and device of its own but a null data pointer, which the C
+    interface reads as "not given": it must not take the place of a weight that is then left out."""
+    class Wrapper(torch.Tensor):
+        @staticmethod
+        def __new__(cls, inner):
+            return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device)
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            raise AssertionError(f"{func} must not run")
+
+    x, w = torch.zeros(4, 8), torch.ones(8)
+    ids = torch.zeros(4, 1, dtype=torch.int32)
+    order = experts.ExpertOrder(ids, ids.reshape(-1), torch.zeros(3, dtype=torch.int32))
+    bare = Wrapper(w)
+    assert bare.is_contiguous() and bare.data_ptr() == 0
+    for what, call in (("weight", lambda: norm.rms_norm_forward(x, bare)),
+                       ("weight", lambda: norm.layer_norm_forward(x, bare, w)),
+                       ("bias", lambda: norm.layer_norm_forward(x, w, bare)),
+                       ("weight", lambda: norm.rms_norm_backward(x, x, torch.zeros(4), bare)),
+                       ("out", lambda: norm.rms_norm_forward(x, w, out=Wrapper(x))),
+                       ("input", lambda: norm.rms_norm_forward(Wrapper(x), w)),
+                       ("weight", lambda: embedding.embedding_forward(ids, Wrapper(x))),
+                       ("weights", lambda: experts.combine_forward(x, order, Wrapper(torch.ones(4, 1)))),
+                       ("weights", lambda: experts.combine_backward(x, x, order, Wrapper(torch.ones(4, 1)))),
+                       ("rows", lambda: experts.combine_forward(Wrapper(x), order)),
+                       ("input", lambda: experts.dispatch_forward(Wrapper(x), order))):
+        with pytest.raises(TypeError, match=f"{what} must have memory"):
+            call()
