@@ -744,12 +744,18 @@ int ring_blocks(int threads, int nv) { return std::min(24, std::max(1, (nv == 2 
 
 // The deepest ring of 2 to 4 rows that leaves the SM room for `per_sm` blocks (228 KiB; a block takes
 // 1 KiB for the system and 512 bytes for its sums besides). Launches f(Int<stages>, bytes).
+constexpr size_t kMostRing = 227 * 1024 - 1024 - 512;
 template <typename F>
 cudaError_t with_ring(size_t row, size_t params, int per_sm, F&& f) {
-    const size_t room = std::min<size_t>(228 * 1024 / per_sm, 227 * 1024) - 1024 - 512;
+    const size_t room = std::min<size_t>(228 * 1024 / per_sm - 1024 - 512, kMostRing);
     if (params + 4 * row <= room) return f(Int<4>{}, params + 4 * row);
     if (params + 3 * row <= room) return f(Int<3>{}, params + 3 * row);
     return f(Int<2>{}, params + 2 * row);
+}
+// The limit belongs to the kernel on the device, not to a launch: every call sets the same one, so that calls
+// of other widths, in other threads or captured before, never find it below what they launch with.
+template <typename K> cudaError_t allow_ring(K* kernel) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMostRing));
 }
 
 // Backward blocks: what is resident at once, but 4 rows each where that still fills the SMs, since
@@ -796,8 +802,7 @@ cudaError_t forward_ring(const NormForwardArgs& a, cudaStream_t s) {
     return with_ring(static_cast<size_t>(NV) * 16 * threads,
                      static_cast<size_t>(vectors) * NV * threads * E * sizeof(Bits<WD>), per_sm, [&](auto S, size_t smem) {
                          auto* kernel = &norm_forward_ring_kernel<D, WD, LAYER, ODD, decltype(S)::value, NV>;
-                         const cudaError_t e = cudaFuncSetAttribute(
-                             kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+                         const cudaError_t e = allow_ring(kernel);
                          if (e != cudaSuccess) return e;
                          kernel<<<grid, threads, smem, s>>>(a);
                          return cudaGetLastError();
@@ -849,8 +854,7 @@ cudaError_t backward_ring(const NormBackwardArgs& a, int grid, cudaStream_t s) {
                      a.w != nullptr ? static_cast<size_t>(NV) * threads * E * sizeof(Bits<WD>) : 0, per_sm,
                      [&](auto S, size_t smem) {
                          auto* kernel = &norm_backward_ring_kernel<D, WD, LAYER, ODD, decltype(S)::value, NV>;
-                         const cudaError_t e = cudaFuncSetAttribute(
-                             kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+                         const cudaError_t e = allow_ring(kernel);
                          if (e != cudaSuccess) return e;
                          kernel<<<grid, threads, smem, s>>>(a);
                          return cudaGetLastError();

@@ -817,3 +817,55 @@ def test_layer_norm_with_a_bias_and_no_weight(dtype, wtype, rows, h):
     check(y, y64, m * (xh.abs() + size) + 2 * U * b.double().abs(), "y")
     check(mean, mean64, m * x.double().abs().mean(-1), "mean")
     check(rstd, rstd64, m * rstd64 * (1 + size[:, 0] ** 2 * U), "rstd")
+
+
+def ring_pair():
+    """Rows of two widths that one instance of the ring kernels takes, with different amounts of shared memory."""
+    return [(randn((rows, h), torch.bfloat16, h), randn(h, torch.bfloat16, h + 1), randn((rows, h), torch.bfloat16, h + 2))
+            for rows, h in ((400, 8192), (1500, 2048))]
+
+
+def both_ways(x, w, dy):
+    from originccl_b200.ops import norm
+    y, rstd = norm.rms_norm_forward(x, w)
+    return [y, rstd, *norm.rms_norm_backward(dy, x, rstd, w)]
+
+
+def test_norms_of_two_widths_in_two_threads():
+    """Calls on different streams may run at the same time: a narrow one takes nothing from a wide one
+    between its setup and its launch."""
+    import threading
+    data = ring_pair()
+    want = [both_ways(*d) for d in data]
+    torch.cuda.synchronize()
+    failed, start = [], threading.Barrier(4)
+
+    def work(i):
+        try:
+            start.wait(60)
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(400):
+                    got = both_ways(*data[i])
+                torch.cuda.current_stream().synchronize()
+            assert equal(got, want[i])
+        except BaseException as e:  # reported by the main thread
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(i % 2,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    assert not failed and not any(t.is_alive() for t in threads), failed
+
+
+def test_norms_of_two_widths_in_one_graph():
+    from originccl_b200.utils.graphs import capture
+    data, box = ring_pair(), {}
+
+    def fn():
+        box["out"] = [t for d in data for t in both_ways(*d)]
+    g = capture(fn)
+    both_ways(*(t[:, :1024].contiguous() if t.dim() == 2 else t[:1024] for t in data[1]))  # narrower still, before the replay
+    g.replay()
+    torch.cuda.synchronize()
+    assert equal(box["out"], [t for d in data for t in both_ways(*d)])
