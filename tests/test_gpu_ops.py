@@ -869,3 +869,36 @@ def test_norms_of_two_widths_in_one_graph():
     g.replay()
     torch.cuda.synchronize()
     assert equal(box["out"], [t for d in data for t in both_ways(*d)])
+
+
+def test_norm_launches_of_two_widths_in_threads_never_fail():
+    """The same through the C interface, whose calls run without the interpreter's lock, often enough for
+    the threads to meet: about 1 wide call in 400 failed where each call set a limit of its own."""
+    import sys
+    import threading
+    from originccl_b200 import _native
+    forward = _native.lib().bcclNormForward
+    failed = [0] * 4
+
+    def work(i, x, w):
+        (rows, h), s = x.shape, torch.cuda.Stream()
+        y, rstd = torch.empty_like(x), torch.empty(rows, device="cuda")
+        args = (1, x.data_ptr(), h, w.data_ptr(), None, y.data_ptr(), h, None, rstd.data_ptr(), rows, h, 1e-5, 4, 4, s.cuda_stream)
+        for k in range(10000):
+            failed[i] += forward(*args) != 0
+            if k % 200 == 199:
+                s.synchronize()
+    data = ring_pair()
+    torch.cuda.synchronize()
+    interval = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    try:
+        threads = [threading.Thread(target=work, args=(i, *data[i % 2][:2])) for i in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join(120)
+    finally:
+        sys.setswitchinterval(interval)
+    torch.cuda.synchronize()
+    assert not any(t.is_alive() for t in threads) and failed == [0] * 4
