@@ -13,10 +13,18 @@ import torch
 _KEY = "bccl_stream"
 
 
+def apply(op: str, function, *args):
+    """``function.apply(*args)``, behind :func:`guard` where a graph is recorded. Where none is (``no_grad``,
+    ``inference_mode``) no backward pass will wait for anything, and there is no node to mark."""
+    if torch.is_grad_enabled() and not torch.is_inference_mode_enabled():
+        guard(op, *args)
+    return function.apply(*args)
+
+
 def guard(op: str, *inputs) -> None:
-    """Called first in the forward pass of a differentiable operator, with its tensor inputs."""
+    """Called before the forward pass of a differentiable operator, with its inputs."""
     for t in inputs:
-        if t is None or not t.requires_grad or not t.is_leaf:
+        if not isinstance(t, torch.Tensor) or not t.requires_grad or not t.is_leaf:
             continue
         stream = torch.cuda.current_stream(t.device).cuda_stream if t.is_cuda else 0
         marks = torch.autograd.graph.get_gradient_edge(t).node.metadata

@@ -18,7 +18,7 @@ from typing import Optional
 import torch
 
 from .. import _native
-from ._capture import guard
+from ._capture import apply
 
 _ops = _native.ops()
 
@@ -40,7 +40,6 @@ def embedding_backward(dy, ids, num_rows: int, scale: float = 1.0, first_row: in
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, scale, padding_idx, first_row):
-        guard("embedding", weight)
         ctx.save_for_backward(ids)
         ctx.args = weight.shape[0], scale, first_row, padding_idx
         return embedding_forward(ids, weight, scale, first_row)
@@ -58,4 +57,4 @@ def embedding(ids, weight, scale: float = 1.0, padding_idx: Optional[int] = None
     positions are looked up but add nothing to the gradient."""
     if padding_idx is not None and padding_idx < 0:
         raise ValueError(f"embedding: padding_idx must not be negative, got {padding_idx}")
-    return _Embedding.apply(ids, weight, scale, padding_idx, first_row)
+    return apply("embedding", _Embedding, ids, weight, scale, padding_idx, first_row)

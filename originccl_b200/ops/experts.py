@@ -21,7 +21,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _native
-from ._capture import guard
+from ._capture import apply
 
 MAX_EXPERTS = 1023
 MAX_TOP = 64
@@ -91,7 +91,6 @@ def combine_backward(dy, rows, order: ExpertOrder, weights=None, *, weight_grad:
 class _Dispatch(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, order):
-        guard("dispatch", x)
         ctx.order = order
         return dispatch_forward(x, order)
 
@@ -104,7 +103,6 @@ class _Dispatch(torch.autograd.Function):
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, weights, order):
-        guard("combine", rows, weights)
         ctx.save_for_backward(rows, weights)
         ctx.order = order
         return combine_forward(rows, order, weights)
@@ -119,9 +117,9 @@ class _Combine(torch.autograd.Function):
 
 def dispatch(x, order: ExpertOrder):
     """Differentiable :func:`dispatch_forward`."""
-    return _Dispatch.apply(x, order)
+    return apply("dispatch", _Dispatch, x, order)
 
 
 def combine(rows, order: ExpertOrder, weights: Optional[torch.Tensor] = None):
     """Differentiable :func:`combine_forward` (gradients of rows and weights)."""
-    return _Combine.apply(rows, weights, order)
+    return apply("combine", _Combine, rows, weights, order)

@@ -16,7 +16,7 @@ from typing import Tuple
 import torch
 
 from .. import _native
-from ._capture import guard
+from ._capture import apply
 
 _LAYER, _RMS = 0, 1
 _ops = _native.ops()
@@ -47,7 +47,6 @@ def rms_norm_backward(dy, x, rstd, weight=None, *, weight_grad: bool = True) -> 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        guard("layer_norm", x, weight, bias)
         y, mean, rstd = layer_norm_forward(x, weight, bias, eps)
         ctx.save_for_backward(x, weight, mean, rstd)
         return y
@@ -64,7 +63,6 @@ class _LayerNorm(torch.autograd.Function):
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, eps):
-        guard("rms_norm", x, weight)
         y, rstd = rms_norm_forward(x, weight, eps)
         ctx.save_for_backward(x, weight, rstd)
         return y
@@ -80,9 +78,9 @@ class _RmsNorm(torch.autograd.Function):
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
     """Differentiable layer norm over the last dimension."""
-    return _LayerNorm.apply(x, weight, bias, eps)
+    return apply("layer_norm", _LayerNorm, x, weight, bias, eps)
 
 
 def rms_norm(x, weight=None, eps: float = 1e-5):
     """Differentiable RMS norm over the last dimension."""
-    return _RmsNorm.apply(x, weight, eps)
+    return apply("rms_norm", _RmsNorm, x, weight, eps)

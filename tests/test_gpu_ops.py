@@ -902,3 +902,38 @@ def test_norm_launches_of_two_widths_in_threads_never_fail():
         sys.setswitchinterval(interval)
     torch.cuda.synchronize()
     assert not any(t.is_alive() for t in threads) and failed == [0] * 4
+
+
+def test_a_model_serves_without_a_graph():
+    """The stack in inference mode and under no_grad, eager and captured, also while a training step's loss
+    is still held: the same bits as its recorded forward pass."""
+    from originccl_b200.models import TinyLlamaStack
+    from originccl_b200.ops import experts as ex, norm
+    from originccl_b200.utils.graphs import capture
+    m = TinyLlamaStack(hidden=256, ffn=768, layers=2, device="cuda", dtype=torch.bfloat16, seed=5, vocab=1024, native=True)
+    ids = some_ids(64, 1024, "skewed", 1)
+    want = m(ids)
+    loss = want.square().mean()  # held until the end
+    for mode in (torch.inference_mode, torch.no_grad):
+        with mode():
+            assert torch.equal(m(ids), want)
+    w = torch.ones(256, device="cuda", requires_grad=True)
+    b = torch.zeros(256, device="cuda", requires_grad=True)
+    order = ex.sort_by_expert(ids[:, None].remainder(4), 4)
+    share = torch.full((64, 1), 0.5, device="cuda", requires_grad=True)
+    held = norm.layer_norm(want, w, b), ex.combine(ex.dispatch(want, order), order, share)
+    for mode in (torch.inference_mode, torch.no_grad):
+        with mode():
+            assert torch.equal(norm.layer_norm(want, w, b), held[0])
+            assert torch.equal(ex.combine(ex.dispatch(want, order), order, share), held[1])
+    box = {}
+
+    @torch.no_grad()
+    def serve():
+        box["y"] = m(ids), norm.layer_norm(want, w, b)
+    g = capture(serve)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(box["y"][0], want) and torch.equal(box["y"][1], held[0])
+    loss.backward()
+    assert m.embed.grad.abs().amax() > 0

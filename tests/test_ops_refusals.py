@@ -299,3 +299,34 @@ def test_tensors_without_storage_are_refused():
                        ("input", lambda: experts.dispatch_forward(Wrapper(x), order))):
         with pytest.raises(TypeError, match=f"{what} must have memory"):
             call()
+
+
+def public_calls(leaf):
+    """Every differentiable entry point with `leaf` [4, 8] or a slice of it among its inputs. On host tensors each
+    ends at the check of the device, behind everything that is done before a kernel's call."""
+    ids = torch.zeros(4, 1, dtype=torch.int32)
+    order = experts.ExpertOrder(ids, ids.reshape(-1), torch.zeros(3, dtype=torch.int32))
+    return (lambda: norm.rms_norm(leaf, None), lambda: norm.layer_norm(leaf, torch.ones(8), torch.ones(8)),
+            lambda: embedding.embedding(ids, leaf), lambda: experts.dispatch(leaf, order), lambda: experts.combine(leaf, order),
+            lambda: experts.combine(leaf, order, torch.ones(4, 1)))
+
+
+@pytest.mark.parametrize("mode", [torch.inference_mode, torch.no_grad])
+def test_the_capture_rule_holds_only_where_a_graph_is_recorded(monkeypatch, mode):
+    """Serving: parameters that require gradients, and no graph. The calls get past the rule (host tensors
+    are refused behind it) in every mode, also while something is captured beside an eager graph."""
+    leaf = torch.ones(4, 8, requires_grad=True)
+    for call in public_calls(leaf):
+        with mode(), pytest.raises(ValueError, match="CUDA"):
+            call()
+    with torch.inference_mode(), torch.enable_grad(), pytest.raises(ValueError, match="CUDA"):
+        norm.rms_norm(leaf, None)
+    held = leaf * 2
+    torch.autograd.graph.get_gradient_edge(leaf).node.metadata["bccl_stream"] = 7  # as if made on stream 7
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    for call in public_calls(leaf):
+        with mode(), pytest.raises(ValueError, match="CUDA"):
+            call()
+        with pytest.raises(RuntimeError, match="still alive"):
+            call()
+    del held
