@@ -11,7 +11,9 @@
 #include <ATen/core/LegacyTypeDispatch.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <algorithm>
 #include <cstdint>
@@ -668,6 +670,17 @@ PyObject* GradClip(PyObject* const* a) {
     return wrap(g.clip(total, max_norm, eps));
 }
 
+// ---------------------------------------------------------------- captures
+// leaf_stream(leaf) -> the CUDA stream on which its accumulation node was made, as an integer; None without a
+// node that lives, or without a stream (host tensors)
+PyObject* LeafStream(PyObject* const* a) {
+    if (!THPVariable_Check(a[0])) type_error("leaf_stream: a tensor is needed");
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(THPVariable_Unpack(a[0]));
+    const auto stream = node ? node->stream() : std::nullopt;
+    if (!stream || stream->device_type() != c10::DeviceType::CUDA) return Py_NewRef(Py_None);
+    return PyLong_FromUnsignedLongLong(reinterpret_cast<uintptr_t>(c10::cuda::CUDAStream(*stream).stream()));
+}
+
 // ---------------------------------------------------------------- the module
 template <PyObject* (*F)(PyObject* const*), int N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -704,6 +717,7 @@ PyMethodDef methods[] = {method<NormForward, 6>("norm_forward"),
                          method<GradSquares, 1>("grad_squares"),
                          method<GradNormOf, 2>("grad_norm_of"),
                          method<GradClip, 5>("grad_clip"),
+                         method<LeafStream, 1>("leaf_stream"),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

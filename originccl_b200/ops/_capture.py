@@ -3,13 +3,16 @@
 Autograd gives each leaf one accumulation node for as long as any graph refers to it, and runs it on the
 stream on which it was made. If an eager forward pass made it on another stream and its output is
 still held, a captured backward pass would wait for that stream, which a capture may not do; the
-error ends the process. :func:`guard` marks the nodes of an operator's leaves with the stream of their
-pass and refuses the capture's forward pass instead.
+error ends the process. :func:`guard` marks the nodes of an operator's leaves with the stream on which they
+were made, by whichever operator, and refuses the capture's forward pass instead.
 """
 from __future__ import annotations
 
 import torch
 
+from .. import _native
+
+_ops = _native.ops()
 _KEY = "bccl_stream"
 
 
@@ -27,8 +30,9 @@ def guard(op: str, *inputs) -> None:
         if not isinstance(t, torch.Tensor) or not t.requires_grad or not t.is_leaf:
             continue
         stream = torch.cuda.current_stream(t.device).cuda_stream if t.is_cuda else 0
+        before = _ops.leaf_stream(t)  # of a node that lives already, perhaps from another operator's pass
         marks = torch.autograd.graph.get_gradient_edge(t).node.metadata
-        made = marks.setdefault(_KEY, stream)
+        made = marks.setdefault(_KEY, stream if before is None else before)
         if made != stream and torch.cuda.is_current_stream_capturing():
             raise RuntimeError(f"{op}: an eager graph of the same leaf tensors, made on another stream, is still alive; "
                                "release its outputs (the loss) before the backward pass is captured")

@@ -937,3 +937,31 @@ def test_a_model_serves_without_a_graph():
     assert torch.equal(box["y"][0], want) and torch.equal(box["y"][1], held[0])
     loss.backward()
     assert m.embed.grad.abs().amax() > 0
+
+
+def test_a_capture_beside_another_operators_graph_is_refused():
+    """torch's own operator made the weight's accumulation node on the default stream, and its result is
+    held: the captured forward pass is refused, before a backward pass could be captured."""
+    from originccl_b200.ops import norm
+    from originccl_b200.utils.graphs import capture
+    x, w = randn((64, 256), torch.float32, 1), randn(256, torch.float32, 2).requires_grad_()
+    held = (w * 2).sum()
+    with pytest.raises(RuntimeError, match="still alive"):
+        capture(lambda: norm.rms_norm(x, w), warmup=0)
+    del held
+    box = {}
+
+    def fn():
+        box["y"] = norm.rms_norm(x, w)
+    g = capture(fn, warmup=0)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(box["y"].detach(), norm.rms_norm_forward(x, w.detach())[0])
+    del box["y"]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        held = (w * 3).sum()
+    norm.rms_norm(x, w)  # marks that node, from the default stream: still the node's stream
+    with pytest.raises(RuntimeError, match="still alive"):
+        capture(lambda: norm.rms_norm(x, w), warmup=0)
+    del held

@@ -330,3 +330,22 @@ def test_the_capture_rule_holds_only_where_a_graph_is_recorded(monkeypatch, mode
         with pytest.raises(RuntimeError, match="still alive"):
             call()
     del held
+
+
+def test_the_capture_rule_knows_nodes_of_other_operators(monkeypatch):
+    """The leaf's node was made by an operator that leaves no mark: its own stream counts (a stand-in here,
+    host tensors have none)."""
+    from originccl_b200.ops import _capture
+    leaf = torch.ones(4, 8, requires_grad=True)
+    assert _capture._ops.leaf_stream(leaf) is None
+    held = leaf * 2
+    assert _capture._ops.leaf_stream(leaf) is None and _capture._ops.leaf_stream(held) is None
+
+    class Ops:
+        leaf_stream = staticmethod(lambda t: 7)
+    monkeypatch.setattr(_capture, "_ops", Ops)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    _capture.guard("op", leaf)  # fine while nothing is captured
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="still alive"):
+        _capture.guard("op", leaf)
