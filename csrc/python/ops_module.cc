@@ -513,19 +513,26 @@ struct Gradients {
     const char* op;
     int device = -1;
     Tensor like;
-    // By type of gradient and output: pointers and counts.
+    // By type of gradient and output, and by whether other ranks hold the same: pointers and counts.
     struct Group {
         int code, out_code;
+        bool replicated;
         uint64_t total = 0;
         std::vector<const void*> in;
         std::vector<void*> out;
         std::vector<size_t> count;
     };
     std::vector<Group> groups;
+    double world;
 
-    Gradients(const char* name, PyObject* grads, PyObject* outs, bool written) : op(name) {
+    // replicated: None, or a list that says for each gradient whether all of `ranks` ranks hold the same.
+    Gradients(const char* name, PyObject* grads, PyObject* outs, bool written, PyObject* replicated, int64_t ranks)
+        : op(name), world(static_cast<double>(ranks)) {
         const Py_ssize_t n = PyList_Check(grads) ? PyList_GET_SIZE(grads) : 0;
         if (n == 0) value_error(std::string(op) + ": no gradients");
+        const bool marked = replicated != Py_None;
+        if (marked && (!PyList_Check(replicated) || PyList_GET_SIZE(replicated) != n || ranks < 1))
+            value_error(std::string(op) + ": replicated must say yes or no for each gradient");
         const bool apart = outs != Py_None;
         if (apart && (!PyList_Check(outs) || PyList_GET_SIZE(outs) != n))
             value_error(std::string(op) + ": outs must be a tensor for each gradient");
@@ -560,12 +567,12 @@ struct Gradients {
                     value_error(std::string(op) + ": each out must have its gradient's shape and layout");
             }
             if (t.numel() == 0) continue;
-            if (groups.empty() || groups.back().code != code || groups.back().out_code != out_code) {
-                const auto found = std::find_if(groups.begin(), groups.end(), [&](const Group& g) {
-                    return g.code == code && g.out_code == out_code;
-                });
+            const bool same = marked && truth(PyList_GET_ITEM(replicated, i));
+            const auto fits = [&](const Group& g) { return g.code == code && g.out_code == out_code && g.replicated == same; };
+            if (groups.empty() || !fits(groups.back())) {
+                const auto found = std::find_if(groups.begin(), groups.end(), fits);
                 if (found == groups.end()) {
-                    groups.push_back({code, out_code, 0, {}, {}, {}});
+                    groups.push_back({code, out_code, same, 0, {}, {}, {}});
                     groups.back().in.reserve(static_cast<size_t>(n));
                     groups.back().out.reserve(static_cast<size_t>(n));
                     groups.back().count.reserve(static_cast<size_t>(n));
@@ -603,7 +610,14 @@ struct Gradients {
         }
     }
 
+    // What this rank adds to the sum over all ranks: where all hold the same, its share of the squares.
     Tensor squares() const {
+        const Tensor total = squares(false);
+        if (std::any_of(groups.begin(), groups.end(), [](const Group& g) { return g.replicated; }))
+            total.add_(squares(true), 1.0 / world);
+        return total;
+    }
+    Tensor squares(bool replicated) const {
         const Tensor total = at::empty({1}, like.options().dtype(at::kDouble));
         std::vector<Tensor> keep;
         bool accumulate = false;
@@ -616,8 +630,9 @@ struct Gradients {
             });
             accumulate = true;
         };
-        for (const Group& g : groups) run(g.in.data(), g.count.data(), static_cast<int>(g.in.size()), g.code, g.total);
-        if (groups.empty()) run(nullptr, nullptr, 0, 0, 0);
+        for (const Group& g : groups)
+            if (g.replicated == replicated) run(g.in.data(), g.count.data(), static_cast<int>(g.in.size()), g.code, g.total);
+        if (!accumulate) run(nullptr, nullptr, 0, 0, 0);
         return total;
     }
 
@@ -638,8 +653,10 @@ struct Gradients {
     }
 };
 
-// grad_squares(grads) -> the sum of squares, a float64 tensor of one element
-PyObject* GradSquares(PyObject* const* a) { return wrap(Gradients("grad_norm", a[0], Py_None, false).squares()); }
+// grad_squares(grads, replicated, ranks) -> this rank's part of the sum of squares, a float64 tensor of one element
+PyObject* GradSquares(PyObject* const* a) {
+    return wrap(Gradients("grad_norm", a[0], Py_None, false, a[1], integer(a[2])).squares());
+}
 
 // grad_norm_of(grads[0], total) -> the norm
 PyObject* GradNormOf(PyObject* const* a) {
@@ -653,16 +670,16 @@ PyObject* GradNormOf(PyObject* const* a) {
     return wrap(norm);
 }
 
-// grad_clip(grads, outs, max_norm, eps, reduce) -> the norm from before. reduce (None or a function) is
-// called on the sum of squares between the two passes.
+// grad_clip(grads, outs, max_norm, eps, replicated, ranks, reduce) -> the norm from before. reduce (None or a
+// function) is called on this rank's part of the sum of squares between the two passes.
 PyObject* GradClip(PyObject* const* a) {
-    const Gradients g("clip_grad_norm", a[0], a[1], true);
     const double max_norm = number(a[2]), eps = number(a[3]);
+    const Gradients g("clip_grad_norm", a[0], a[1], true, a[4], integer(a[5]));
     const Tensor total = g.squares();
-    if (a[4] != Py_None) {
+    if (a[6] != Py_None) {
         PyObject* t = wrap(total);
         if (t == nullptr) return nullptr;
-        PyObject* done = PyObject_CallOneArg(a[4], t);
+        PyObject* done = PyObject_CallOneArg(a[6], t);
         Py_DECREF(t);
         if (done == nullptr) return nullptr;
         Py_DECREF(done);
@@ -714,9 +731,9 @@ PyMethodDef methods[] = {method<NormForward, 6>("norm_forward"),
                          method<Dispatch, 4>("dispatch"),
                          method<Combine, 4>("combine"),
                          method<CombineBackward, 6>("combine_backward"),
-                         method<GradSquares, 1>("grad_squares"),
+                         method<GradSquares, 3>("grad_squares"),
                          method<GradNormOf, 2>("grad_norm_of"),
-                         method<GradClip, 5>("grad_clip"),
+                         method<GradClip, 7>("grad_clip"),
                          method<LeafStream, 1>("leaf_stream"),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

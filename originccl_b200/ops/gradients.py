@@ -8,7 +8,9 @@ for up to 1024 tensors of one type, no synchronisation with the host, the same s
 Gradients are float32, bfloat16 or float16, mixed if need be, each dense in memory (any order of
 dimensions). With ``comm`` the tensors are this rank's shards of the parameters (tensor
 parallelism) and the norm is that of all ranks' shards: one AllReduce of the sum of squares
-between the launches; every rank of ``comm`` calls it together. Host tensors (ranks of a host communicator)
+between the launches; every rank of ``comm`` calls it together. Parameters that every rank of ``comm`` holds whole, with
+the same gradient (norm weights, say), are named by ``replicated``, a truth value for each gradient: their
+squares count once, not once per rank. Host tensors (ranks of a host communicator)
 run on torch operations. The reference has no compute operators.
 """
 from __future__ import annotations
@@ -23,32 +25,45 @@ _ops = _native.ops()
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def _host(op, grads, comm, outs=()):
+def _replicated(op, grads, replicated, comm):
+    """The list of truth values, or None where no rank would count anything twice."""
+    if replicated is None:
+        return None
+    replicated = [bool(r) for r in replicated]
+    if len(replicated) != len(grads):
+        raise ValueError(f"{op}: {len(grads)} gradients but {len(replicated)} truth values in replicated")
+    return replicated if comm is not None and comm.world_size > 1 and any(replicated) else None
+
+
+def _host(op, grads, comm, replicated, outs=()):
     """The norm of host tensors."""
     for t in (*grads, *outs):
         if t.is_cuda or t.dtype not in _FLOATS:
             raise ValueError(f"{op}: gradients must be float32, bfloat16 or float16 tensors, all on one device")
     total = torch.zeros(1, dtype=torch.float64)
-    for t in grads:
-        total += t.double().square().sum()
+    for i, t in enumerate(grads):
+        share = comm.world_size if replicated is not None and replicated[i] else 1
+        total += t.double().square().sum() / share
     if comm is not None and comm.world_size > 1:
         comm.all_reduce(total)
     return total.sqrt().float()[0]
 
 
-def grad_norm(grads: Sequence[torch.Tensor], *, comm=None):
+def grad_norm(grads: Sequence[torch.Tensor], *, comm=None, replicated: Optional[Sequence[bool]] = None):
     """The global norm, a float32 tensor of no dimensions on the gradients' device."""
     grads = list(grads)
+    replicated = _replicated("grad_norm", grads, replicated, comm)
     if grads and not grads[0].is_cuda:
-        return _host("grad_norm", grads, comm)
-    total = _ops.grad_squares(grads)
+        return _host("grad_norm", grads, comm, replicated)
+    total = _ops.grad_squares(grads, replicated, 1 if replicated is None else comm.world_size)
     if comm is not None and comm.world_size > 1:
         comm.all_reduce(total)
     return _ops.grad_norm_of(grads[0], total)
 
 
 def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, *, eps: float = 1e-6,
-                   outs: Optional[Sequence[torch.Tensor]] = None, comm=None):
+                   outs: Optional[Sequence[torch.Tensor]] = None, comm=None,
+                   replicated: Optional[Sequence[bool]] = None):
     """Scales the gradients by ``min(1, max_norm / (norm + eps))`` in place, or into ``outs`` (same shapes; the
     gradients' type or float32; memory of their own), and returns the norm from before."""
     op = "clip_grad_norm"
@@ -58,10 +73,12 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, *, eps: float
     outs = None if outs is None else list(outs)
     if outs is not None and len(outs) != len(grads):
         raise ValueError(f"{op}: {len(grads)} gradients but {len(outs)} outs")
+    replicated = _replicated(op, grads, replicated, comm)
     if grads and not grads[0].is_cuda:
-        norm = _host(op, grads, comm, outs or ())
+        norm = _host(op, grads, comm, replicated, outs or ())
         coef = torch.clamp(max_norm / (norm + eps), max=1.0)
         for t, o in zip(grads, grads if outs is None else outs):
             o.copy_(t.float() * coef)
         return norm
-    return _ops.grad_clip(grads, outs, max_norm, eps, comm.all_reduce if comm is not None and comm.world_size > 1 else None)
+    ranks = 1 if comm is None else comm.world_size
+    return _ops.grad_clip(grads, outs, max_norm, eps, replicated, ranks, comm.all_reduce if ranks > 1 else None)

@@ -188,13 +188,22 @@ class DataParallelSync:
         self.comm.all_reduce_many(self._bucket_batch, ReduceOp.SUM, scale=self.scale, grouped=False, stream=s)
         self._sync_small(s)
 
-    def clip_grad_norm_(self, max_norm: float, *, eps: float = 1e-6, shards=None):
+    def clip_grad_norm_(self, max_norm: float, *, eps: float = 1e-6, shards=None, replicated: Iterable[str] = ()):
         """Scales the synced gradients by ``min(1, max_norm / (norm + eps))`` and returns their global
         norm (a float32 tensor of no dimensions; the host does not wait). Call it after :meth:`sync` or
         :meth:`finish`: every rank then holds the same gradients and computes the same norm. Where the
         parameters are also sharded, ``shards`` is the communicator of the ranks that hold the other
-        shards (``Mesh.tp``), and all of them call this together."""
+        shards (``Mesh.tp``), and all of them call this together. Every parameter then counts as a shard but
+        those named in ``replicated``: what all those ranks hold whole, with the same gradients (norm weights, biases of
+        row-parallel layers), would count once per rank otherwise."""
         from ..ops import gradients
+        names = set(replicated)
+        unknown = names.difference(self.grads.names)
+        if unknown:
+            raise ValueError(f"clip_grad_norm_: no parameter is named {', '.join(sorted(unknown))}")
+        if shards is not None and shards.world_size > 1 and names:
+            return gradients.clip_grad_norm(self.grads.views, max_norm, eps=eps, comm=shards,
+                                            replicated=[n in names for n in self.grads.names])
         flats = [t for t in (self.grads.flat, self.grads.small_flat) if t.numel()]
         return gradients.clip_grad_norm(flats, max_norm, eps=eps, comm=shards)
 

@@ -11,3 +11,9 @@ pytest.importorskip("torch")
 def test_clipping_on_ranks(ranks):
     res = _mp.run(ranks, clip_cases.run_clip, timeout=240)
     assert all(r == res[0] for r in res)
+
+
+@pytest.mark.parametrize("ranks", [2, 3])
+def test_replicated_parameters_count_once(ranks):
+    res = _mp.run(ranks, clip_cases.run_replicated, timeout=240)
+    assert all(r == res[0] for r in res)

@@ -965,3 +965,32 @@ def test_a_capture_beside_another_operators_graph_is_refused():
     with pytest.raises(RuntimeError, match="still alive"):
         capture(lambda: norm.rms_norm(x, w), warmup=0)
     del held
+
+
+@pytest.mark.parametrize("clip", [False, True])
+def test_replicated_gradients_count_once(clip):
+    """Mixed types, some of them held by both of two ranks (stood in for by a doubled sum)."""
+    import originccl_b200 as occl
+    from originccl_b200.ops import gradients
+    comm = occl.Communicator().init(0, 1, None, device=0)
+
+    class Twice:
+        world_size = 2
+
+        def all_reduce(self, t):
+            comm.all_reduce(t, scale=2.0)
+
+    grads = [randn(1000, torch.float32, 1), randn((30, 41), torch.bfloat16, 2), randn(7, torch.float32, 3), randn(5000, torch.bfloat16, 4),
+             torch.empty(0, device="cuda"), randn(33, torch.float16, 5)]
+    for flags in ([False, True, True, False, True, False], [True] * 6, [False] * 6, [0, 0, 0, 0, 1, 0]):
+        mine = [g.clone() for g in grads]
+        n64 = sum(g.double().square().sum() * (1 if r else 2) for g, r in zip(grads, flags)).sqrt()
+        if clip:
+            norm = gradients.clip_grad_norm(mine, 3.0, comm=Twice(), replicated=flags)
+            for m, g in zip(mine, grads):
+                exact = g.double() * (3.0 / (float(n64) + 1e-6))
+                check(m, exact, 40 * U * exact.abs())
+        else:
+            norm = gradients.grad_norm(mine, comm=Twice(), replicated=flags)
+        check(norm, n64, 34 * U * n64)
+    comm.destroy()
