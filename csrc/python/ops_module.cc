@@ -54,15 +54,21 @@ std::string type_of(at::ScalarType t) {
 }
 
 // ---------------------------------------------------------------- arguments
-const Tensor& tensor(const char* op, const char* what, PyObject* o) {
+[[noreturn]] void no_storage(const char* op, const char* what) {
+    // Wrappers (distributed tensors, say) have a shape, a type and a device but no storage of their own, and the
+    // C interface reads a null pointer as "not given": a weight would be left out without a word.
+    type_error(std::string(op) + ": " + what + " must have memory of its own, got a tensor without storage");
+}
+const Tensor& strided(const char* op, const char* what, PyObject* o) {
     if (!THPVariable_Check(o)) type_error(std::string(op) + ": " + what + " must be a tensor");
     const Tensor& t = THPVariable_Unpack(o);
     if (t.layout() != at::kStrided) type_error(std::string(op) + ": " + what + " must be a strided tensor");
     if (t.is_neg()) type_error(std::string(op) + ": " + what + " must not be a view of negated values");
-    // Wrappers (distributed tensors, say) have a shape, a type and a device but no storage of their own, and the
-    // C interface reads a null pointer as "not given": a weight would be left out without a word.
-    if (t.numel() != 0 && t.const_data_ptr() == nullptr)
-        type_error(std::string(op) + ": " + what + " must have memory of its own, got a tensor without storage");
+    return t;
+}
+const Tensor& tensor(const char* op, const char* what, PyObject* o) {
+    const Tensor& t = strided(op, what, o);
+    if (t.numel() != 0 && t.const_data_ptr() == nullptr) no_storage(op, what);
     return t;
 }
 Optional optional_tensor(const char* op, const char* what, PyObject* o) {
@@ -542,14 +548,14 @@ struct Gradients {
         };
         std::vector<Range> ranges;
         if (written) ranges.reserve(static_cast<size_t>(apart ? 2 * n : n));
-        const auto range = [&](const Tensor& t, int code, bool w) {
-            const auto p = reinterpret_cast<uint64_t>(t.data_ptr());
-            ranges.push_back({p, p + static_cast<uint64_t>(t.numel()) * static_cast<uint64_t>(size_of(code)), w});
+        const auto range = [&](const void* at, int64_t count, int code, bool w) {
+            const auto p = reinterpret_cast<uint64_t>(at);
+            ranges.push_back({p, p + static_cast<uint64_t>(count) * static_cast<uint64_t>(size_of(code)), w});
         };
         bool elsewhere = false;  // an output that is not its gradient
         for (Py_ssize_t i = 0; i < n; ++i) {
-            const Tensor& t = tensor(op, "each gradient", PyList_GET_ITEM(grads, i));
-            const Tensor& o = apart ? tensor(op, "each out", PyList_GET_ITEM(outs, i)) : t;
+            const Tensor& t = strided(op, "each gradient", PyList_GET_ITEM(grads, i));
+            const Tensor& o = apart ? strided(op, "each out", PyList_GET_ITEM(outs, i)) : t;
             const int code = float_code(op, "each gradient", t);
             if (i == 0) {
                 device = one_device(op, t);
@@ -566,7 +572,12 @@ struct Gradients {
                 if (o.sizes() != t.sizes() || (o.strides() != t.strides() && !(o.is_contiguous() && t.is_contiguous())))
                     value_error(std::string(op) + ": each out must have its gradient's shape and layout");
             }
-            if (t.numel() == 0) continue;
+            const int64_t count = t.numel();
+            if (count == 0) continue;
+            void* out = o.mutable_data_ptr();  // first: it may move a lazily copied gradient, in place
+            const void* in = t.const_data_ptr();
+            if (in == nullptr) no_storage(op, "each gradient");
+            if (out == nullptr) no_storage(op, "each out");
             const bool same = marked && truth(PyList_GET_ITEM(replicated, i));
             const auto fits = [&](const Group& g) { return g.code == code && g.out_code == out_code && g.replicated == same; };
             if (groups.empty() || !fits(groups.back())) {
@@ -581,14 +592,14 @@ struct Gradients {
                 }
             }
             Group& g = groups.back();
-            g.in.push_back(t.data_ptr());
-            g.out.push_back(o.data_ptr());
-            g.count.push_back(static_cast<size_t>(t.numel()));
-            g.total += static_cast<uint64_t>(t.numel());
+            g.in.push_back(in);
+            g.out.push_back(out);
+            g.count.push_back(static_cast<size_t>(count));
+            g.total += static_cast<uint64_t>(count);
             if (!written) continue;
-            range(o, out_code, true);
-            if (o.data_ptr() != t.data_ptr() || out_code != code) elsewhere = true;
-            if (apart) range(t, code, false);
+            range(out, count, out_code, true);
+            if (out != in || out_code != code) elsewhere = true;
+            if (apart) range(in, count, code, false);
         }
         if (!written) return;
         check_apart(ranges, elsewhere);

@@ -349,3 +349,19 @@ def test_the_capture_rule_knows_nodes_of_other_operators(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     with pytest.raises(RuntimeError, match="still alive"):
         _capture.guard("op", leaf)
+
+
+def test_gradients_without_storage_are_refused():
+    class Wrapper(torch.Tensor):
+        @staticmethod
+        def __new__(cls, n):
+            return torch.Tensor._make_wrapper_subclass(cls, (n,), dtype=torch.float32, device=torch.device("cuda", 0))
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            raise AssertionError(f"{func} must not run")
+
+    for call in (lambda: gradients.grad_norm([Wrapper(4)]), lambda: gradients.clip_grad_norm([Wrapper(4)], 1.0),
+                 lambda: gradients.clip_grad_norm([Wrapper(4)], 1.0, outs=[Wrapper(4)])):
+        with pytest.raises(TypeError, match="each gradient must have memory"):
+            call()
