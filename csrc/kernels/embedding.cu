@@ -133,6 +133,7 @@ struct WindowArgs {
     int tile;            // rows that a block clears at a time
     int window_blocks;   // blocks of windows, the others clear
     int join_windows;    // windows that a block of the join looks at
+    int join_columns;    // stretches of kJoinColumns accesses in a row
 };
 
 constexpr int kMaxTile = 4096;
@@ -283,46 +284,49 @@ __global__ void __launch_bounds__(kJoinColumns * kJoinParts) join_kernel(const W
         last_of[threadIdx.x] = last;
     }
     __syncthreads();
-    const int j = blockIdx.y * kJoinColumns + threadIdx.x;
     for (int i = 0; i < a.join_windows; ++i) {
         const long long w = w0 + i, last = last_of[i];
         if (last < 0) continue;
-        float sum[E];
+        // Rows near 2^23 elements have more stretches of columns than a grid has blocks in y.
+        for (int stretch = blockIdx.y; stretch < a.join_columns; stretch += gridDim.y) {
+            const int j = stretch * kJoinColumns + threadIdx.x;
+            float sum[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) sum[e] = 0.0f;
-        const long long share = (last - w + kJoinParts) / kJoinParts;  // of last - w + 1 partial rows
-        const long long k1 = min(last + 1, w + (threadIdx.y + 1) * share);
-        if (j * E < a.width) {
-            for (long long k0 = w + threadIdx.y * share; k0 < k1; k0 += kJoinFlight) {
-                float f[kJoinFlight][E];
+            for (int e = 0; e < E; ++e) sum[e] = 0.0f;
+            const long long share = (last - w + kJoinParts) / kJoinParts;  // of last - w + 1 partial rows
+            const long long k1 = min(last + 1, w + (threadIdx.y + 1) * share);
+            if (j * E < a.width) {
+                for (long long k0 = w + threadIdx.y * share; k0 < k1; k0 += kJoinFlight) {
+                    float f[kJoinFlight][E];
 #pragma unroll
-                for (int u = 0; u < kJoinFlight; ++u)
-                    if (k0 + u < k1)
-                        load_f<kF32, E>(reinterpret_cast<const Bits<kF32>*>(
-                                            a.partial + ((k0 + u) * 2 + (k0 + u == w ? 1 : 0)) * a.width + j * E),
-                                        f[u]);
+                    for (int u = 0; u < kJoinFlight; ++u)
+                        if (k0 + u < k1)
+                            load_f<kF32, E>(reinterpret_cast<const Bits<kF32>*>(
+                                                a.partial + ((k0 + u) * 2 + (k0 + u == w ? 1 : 0)) * a.width + j * E),
+                                            f[u]);
 #pragma unroll
-                for (int u = 0; u < kJoinFlight; ++u) {
-                    if (k0 + u >= k1) break;
+                    for (int u = 0; u < kJoinFlight; ++u) {
+                        if (k0 + u >= k1) break;
 #pragma unroll
-                    for (int e = 0; e < E; ++e) sum[e] += f[u][e];
+                        for (int e = 0; e < E; ++e) sum[e] += f[u][e];
+                    }
                 }
             }
-        }
 #pragma unroll
-        for (int e = 0; e < E; ++e) parts[threadIdx.y][threadIdx.x][e] = sum[e];
-        __syncthreads();
-        const unsigned int row = __ldg(&a.sorted[(w + 1) * a.window].x);
-        Bits<OD>* to = dtable + static_cast<long long>(row) * a.h;
-        const int c = j * E - shift_of<ODD, OD>(to);
-        if (threadIdx.y == 0 && c < a.h) {
-            for (int p = 1; p < kJoinParts; ++p) {
+            for (int e = 0; e < E; ++e) parts[threadIdx.y][threadIdx.x][e] = sum[e];
+            __syncthreads();
+            const unsigned int row = __ldg(&a.sorted[(w + 1) * a.window].x);
+            Bits<OD>* to = dtable + static_cast<long long>(row) * a.h;
+            const int c = j * E - shift_of<ODD, OD>(to);
+            if (threadIdx.y == 0 && c < a.h) {
+                for (int p = 1; p < kJoinParts; ++p) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) sum[e] += parts[p][threadIdx.x][e];
+                    for (int e = 0; e < E; ++e) sum[e] += parts[p][threadIdx.x][e];
+                }
+                write_row<OD, E, ODD>(to, c, a.h, sum, a.scale, a.accumulate != 0);
             }
-            write_row<OD, E, ODD>(to, c, a.h, sum, a.scale, a.accumulate != 0);
+            __syncthreads();
         }
-        __syncthreads();
     }
 }
 
@@ -440,8 +444,9 @@ cudaError_t LaunchEmbeddingBackward(const EmbeddingArgs& a, const void* dy, long
             w.tile = static_cast<int>(std::min<long long>(kMaxTile, std::max(1ll, tile)));
             const long long clear = accumulate ? 0 : std::min(1ll << 20, ceil_div(a.rows, w.tile));
             w.window_blocks = static_cast<int>(ceil_div(w.windows, b.y));
+            w.join_columns = static_cast<int>(ceil_div(wide, kJoinColumns));
             w.join_windows = static_cast<int>(
-                std::min<long long>(kJoinWindows, std::max(1ll, w.windows * ceil_div(wide, kJoinColumns) / (8 * sm_count()))));
+                std::min<long long>(kJoinWindows, std::max(1ll, w.windows * w.join_columns / (8 * sm_count()))));
             const size_t smem = sizeof(uint2) * b.y * (w.window + 2);
             window_kernel<kD, kO, Form>
                 <<<dim3(static_cast<unsigned>(w.window_blocks + clear), cols), dim3(b.x, b.y), smem, stream>>>(
@@ -449,7 +454,7 @@ cudaError_t LaunchEmbeddingBackward(const EmbeddingArgs& a, const void* dy, long
             cudaError_t err = cudaGetLastError();
             if (err != cudaSuccess || w.windows == 1) return err;
             const dim3 grid(static_cast<unsigned>(ceil_div(w.windows - 1, w.join_windows)),
-                            static_cast<unsigned>(ceil_div(wide, kJoinColumns)));
+                            static_cast<unsigned>(std::min(w.join_columns, 65535)));
             join_kernel<kO, E, Form::odd><<<grid, dim3(kJoinColumns, kJoinParts), 0, stream>>>(w, static_cast<Bits<kO>*>(dtable));
             return cudaGetLastError();
         });

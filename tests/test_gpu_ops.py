@@ -994,3 +994,17 @@ def test_replicated_gradients_count_once(clip):
             norm = gradients.grad_norm(mine, comm=Twice(), replicated=flags)
         check(norm, n64, 34 * U * n64)
     comm.destroy()
+
+
+@pytest.mark.parametrize("h", [2 ** 23, 2 ** 23 - 1])
+def test_embedding_of_the_longest_rows(h):
+    """A token over several windows, so that its partial rows are joined."""
+    from originccl_b200.ops import embedding
+    ids = torch.tensor([1] * 15 + [0, 1], device="cuda")
+    w = randn((2, h), torch.float32, 1)
+    assert torch.equal(embedding.embedding_forward(ids[-2:], w), w[ids[-2:]])
+    dy = randn((17, h), torch.float32, 2)
+    got = embedding.embedding_backward(dy, ids, 3)
+    for row in range(3):
+        terms = dy[ids == row].double()
+        check(got[row], terms.sum(0), (terms.shape[0] + 2) * U * terms.abs().sum(0))
