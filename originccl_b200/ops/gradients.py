@@ -11,7 +11,7 @@ parallelism) and the norm is that of all ranks' shards: one AllReduce of the sum
 between the launches; every rank of ``comm`` calls it together. Parameters that every rank of ``comm`` holds whole, with
 the same gradient (norm weights, say), are named by ``replicated``, a truth value for each gradient: their
 squares count once, not once per rank. Host tensors (ranks of a host communicator)
-run on torch operations. The reference has no compute operators.
+run on torch operations, without the package's extension. The reference has no compute operators.
 """
 from __future__ import annotations
 
@@ -21,8 +21,14 @@ import torch
 
 from .. import _native
 
-_ops = _native.ops()
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _list(op, grads):
+    grads = list(grads)
+    if not grads:
+        raise ValueError(f"{op}: no gradients")
+    return grads
 
 
 def _replicated(op, grads, replicated, comm):
@@ -51,14 +57,15 @@ def _host(op, grads, comm, replicated, outs=()):
 
 def grad_norm(grads: Sequence[torch.Tensor], *, comm=None, replicated: Optional[Sequence[bool]] = None):
     """The global norm, a float32 tensor of no dimensions on the gradients' device."""
-    grads = list(grads)
+    grads = _list("grad_norm", grads)
     replicated = _replicated("grad_norm", grads, replicated, comm)
-    if grads and not grads[0].is_cuda:
+    if not grads[0].is_cuda:
         return _host("grad_norm", grads, comm, replicated)
-    total = _ops.grad_squares(grads, replicated, 1 if replicated is None else comm.world_size)
+    ops = _native.ops()
+    total = ops.grad_squares(grads, replicated, 1 if replicated is None else comm.world_size)
     if comm is not None and comm.world_size > 1:
         comm.all_reduce(total)
-    return _ops.grad_norm_of(grads[0], total)
+    return ops.grad_norm_of(grads[0], total)
 
 
 def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, *, eps: float = 1e-6,
@@ -69,16 +76,16 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, *, eps: float
     op = "clip_grad_norm"
     if not max_norm >= 0.0 or not eps >= 0.0:
         raise ValueError(f"{op}: max_norm and eps must not be negative, got {max_norm} and {eps}")
-    grads = list(grads)
+    grads = _list(op, grads)
     outs = None if outs is None else list(outs)
     if outs is not None and len(outs) != len(grads):
         raise ValueError(f"{op}: {len(grads)} gradients but {len(outs)} outs")
     replicated = _replicated(op, grads, replicated, comm)
-    if grads and not grads[0].is_cuda:
+    if not grads[0].is_cuda:
         norm = _host(op, grads, comm, replicated, outs or ())
         coef = torch.clamp(max_norm / (norm + eps), max=1.0)
         for t, o in zip(grads, grads if outs is None else outs):
             o.copy_(t.float() * coef)
         return norm
     ranks = 1 if comm is None else comm.world_size
-    return _ops.grad_clip(grads, outs, max_norm, eps, replicated, ranks, comm.all_reduce if ranks > 1 else None)
+    return _native.ops().grad_clip(grads, outs, max_norm, eps, replicated, ranks, comm.all_reduce if ranks > 1 else None)

@@ -365,3 +365,23 @@ def test_gradients_without_storage_are_refused():
                  lambda: gradients.clip_grad_norm([Wrapper(4)], 1.0, outs=[Wrapper(4)])):
         with pytest.raises(TypeError, match="each gradient must have memory"):
             call()
+
+
+def test_host_gradients_need_no_extension(monkeypatch):
+    """Where the extension was not built (no CUDA headers of PyTorch), ranks with host tensors still clip."""
+    import importlib
+
+    def missing():
+        raise ImportError("not built")
+    monkeypatch.setattr(_native, "ops", missing)
+    try:
+        again = importlib.reload(gradients)
+        g = [torch.full((4,), 3.0), torch.full((9,), 1.0)]
+        assert abs(again.grad_norm(g).item() - 45.0 ** 0.5) <= 45.0 ** 0.5 * 2 ** -23
+        again.clip_grad_norm(g, 1.0)
+        assert abs(g[0][0].item() - 3.0 / 45.0 ** 0.5) <= 2 ** -20
+        with pytest.raises(ValueError, match="no gradients"):
+            again.grad_norm([])
+    finally:
+        monkeypatch.undo()
+        importlib.reload(gradients)
