@@ -165,11 +165,23 @@ std::pair<uint64_t, uint64_t> extent(const Tensor& t) {
     const auto from = reinterpret_cast<uint64_t>(t.data_ptr());
     return {from, from + static_cast<uint64_t>(last + 1) * t.element_size()};
 }
-// An output must not lie in what is read while it is written.
+// The bytes of a row and from row to row, where t is a matrix with rows of adjacent elements; else zeros.
+std::pair<uint64_t, uint64_t> row_bytes(const Tensor& t) {
+    if (t.dim() != 2 || (t.size(1) != 1 && t.stride(1) != 1)) return {0, 0};
+    return {t.size(1) * t.element_size(), t.stride(0) * t.element_size()};
+}
+// An output must not lie in what is read while it is written. Columns of one array may lie beside each other.
 void apart(const char* op, const Tensor& out, const Tensor& in) {
     const auto [a, b] = extent(out);
     const auto [c, d] = extent(in);
-    if (a < d && c < b) value_error(std::string(op) + ": out must not overlap an input");
+    if (a >= d || c >= b) return;
+    const auto [out_row, pitch] = row_bytes(out);
+    const auto [in_row, in_pitch] = row_bytes(in);
+    if (pitch != 0 && pitch == in_pitch) {
+        const uint64_t column = c >= a ? (c - a) % pitch : (pitch - (a - c) % pitch) % pitch;  // of in, counted from out's first
+        if (column >= out_row && column + in_row <= pitch) return;
+    }
+    value_error(std::string(op) + ": out must not overlap an input");
 }
 void* data(const Tensor& t) { return t.numel() == 0 ? nullptr : t.data_ptr(); }
 void* data(const Optional& t) { return t ? data(*t) : nullptr; }

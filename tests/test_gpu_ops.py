@@ -1008,3 +1008,26 @@ def test_embedding_of_the_longest_rows(h):
     for row in range(3):
         terms = dy[ids == row].double()
         check(got[row], terms.sum(0), (terms.shape[0] + 2) * U * terms.abs().sum(0))
+
+
+@pytest.mark.parametrize("rows,h,gap", [(40, 640, 0), (40, 651, 1), (3000, 1016, 8), (3000, 1001, 3)])
+def test_outputs_beside_their_inputs_in_one_array(rows, h, gap):
+    """Columns of one array, either of them first, at any alignment; but not a column of the input's. The same
+    bits as from and into arrays of their own with that alignment (which decides which thread adds what)."""
+    from originccl_b200.ops import embedding, norm
+    wide = randn((rows, 2 * h + 2 * gap), torch.bfloat16, 1)
+    w = randn(h, torch.bfloat16, 2)
+    ids = some_ids(rows, rows, "flat", 3)
+    for a, b in ((gap, h + gap), (h + gap, gap)):
+        for call in (lambda x, out: norm.rms_norm_forward(x, w, out=out)[0], lambda x, out: norm.layer_norm_forward(x, w, out=out)[0],
+                     lambda x, out: embedding.embedding_forward(ids, x, 0.5, out=out)):
+            buf = wide.clone()
+            x, out = buf[:, a:a + h], buf[:, b:b + h]
+            want = call(wide[:, a:a + h], torch.empty_like(wide)[:, b:b + h])
+            assert call(x, out) is not None and torch.equal(out, want)
+            out.copy_(wide[:, b:b + h])
+            assert torch.equal(buf, wide)  # nothing else was written
+            for off in (-1, 1):
+                if (off < 0) == (a < b):  # one column into the input
+                    with pytest.raises(ValueError, match="overlap"):
+                        call(x, buf[:, b + off:b + off + h])
