@@ -1031,3 +1031,49 @@ def test_outputs_beside_their_inputs_in_one_array(rows, h, gap):
                 if (off < 0) == (a < b):  # one column into the input
                     with pytest.raises(ValueError, match="overlap"):
                         call(x, buf[:, b + off:b + off + h])
+
+
+# Rows per block of the ring kernels: more than the ring is deep, at both accesses per thread, at rows that begin
+# on 16 bytes and at rows that do not.
+RINGS = [(torch.bfloat16, 9000, 1531), (torch.float16, 9000, 1528), (torch.float16, 3000, 4097), (torch.bfloat16, 1000, 8200),
+         (torch.float16, 1000, 8201), (torch.bfloat16, 1000, 16384), (torch.bfloat16, 1000, 16001), (torch.float32, 3000, 2049),
+         (torch.float32, 2500, 4096), (torch.float32, 1000, 8189), (torch.bfloat16, 20000, 140), (torch.float32, 20000, 71)]
+
+
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("dtype,rows,h", RINGS)
+def test_norms_of_many_rows(kind, dtype, rows, h):
+    x, dy = randn((rows, h), dtype, 3, 2.0, 0.5), randn((rows, h), dtype, 4, 0.1)
+    for wtype in {dtype, torch.float32}:
+        w, b = randn(h, wtype, 1, 0.2, 1.0), randn(h, wtype, 2, 0.3)
+        check_norm(kind, x, w, b if kind == "layer" else None, 1e-5, dy)
+    check_norm(kind, x, None, None, 1e-5, dy)
+
+
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("dtype,rows,h", RINGS[:6])
+def test_norms_of_many_rows_in_other_layouts(kind, dtype, rows, h):
+    """Rows of x, dy or both that begin elsewhere than those of y and dx; and all at the same odd distance."""
+    wide, other = randn((rows, h + 19), dtype, 3, 2.0, 0.5), randn((rows, h + 19), dtype, 4, 0.1)
+    w = randn(h, dtype, 1, 0.2, 1.0)
+    for x, dy in ((wide[:, 5:h + 5], other[:, :h]), (wide[:, :h].contiguous(), other[:, 1:h + 1]),
+                  (wide[:, 8:h + 8], other[:, 8:h + 8].contiguous()), (wide[:, :h].contiguous(), other[:1, :h].expand(rows, h))):
+        check_norm(kind, x, w, None, 1e-5, dy)
+
+
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("dtype,rows,h", RINGS + [(torch.bfloat16, 37, 1531), (torch.float16, 3, 40001), (torch.float32, 500, 33)])
+def test_norms_in_place(kind, dtype, rows, h):
+    """The same bits as into an array of its own, whatever a block's neighbours write meanwhile."""
+    from originccl_b200.ops import norm
+    w, b = randn(h, dtype, 1, 0.2, 1.0), randn(h, dtype, 2, 0.3)
+    run = (lambda x, out: norm.layer_norm_forward(x, w, b, out=out)) if kind == "layer" else \
+        (lambda x, out: norm.rms_norm_forward(x, w, out=out))
+    for off in (0, 3):  # rows that begin anywhere
+        store = randn(rows * h + off, dtype, 3, 2.0, 0.5)
+        x = store[off:].view(rows, h)
+        want = run(x, torch.empty_like(store)[off:].view(rows, h))
+        for _ in range(3):
+            again = store.clone()
+            got = run(again[off:].view(rows, h), again[off:].view(rows, h))
+            assert equal(got, want) and torch.equal(again[:off], store[:off])
