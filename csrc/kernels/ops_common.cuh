@@ -20,8 +20,6 @@ namespace ops {
 using dev::kBF16;
 using dev::kF16;
 using dev::kF32;
-using dev::kI32;
-using dev::kI64;
 using dev::Ty;
 using dev::Vec;
 
@@ -36,11 +34,6 @@ template <int D, int E> struct Raw {
 template <int D, int E>
 __device__ __forceinline__ Raw<D, E> load_raw(const Bits<D>* p) {
     return {__ldg(reinterpret_cast<const uint4*>(p))};
-}
-// Streaming form for data that is read once: does not displace what other blocks keep in L2.
-template <int D, int E>
-__device__ __forceinline__ Raw<D, E> load_raw_cs(const Bits<D>* p) {
-    return {__ldcs(reinterpret_cast<const uint4*>(p))};
 }
 template <int D, int E>
 __device__ __forceinline__ void unpack(const Raw<D, E>& r, float (&a)[E]) {
@@ -298,7 +291,7 @@ __device__ __forceinline__ float inv_sqrt(float v) {
     return fabsf(d) < 1.0f ? fmaf(0.5f * r, d, r) : r;
 }
 
-inline int size_of(int d) { return d == kF32 || d == kI32 ? 4 : d == kI64 ? 8 : 2; }
+inline int size_of(int d) { return d == kF32 ? 4 : 2; }
 inline bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 // Rows of `h` elements, `stride` apart from `p`, that all start and end on 16-byte boundaries.
 inline bool rows16(const void* p, long long stride, long long h, int size) {
