@@ -1077,3 +1077,27 @@ def test_norms_in_place(kind, dtype, rows, h):
             again = store.clone()
             got = run(again[off:].view(rows, h), again[off:].view(rows, h))
             assert equal(got, want) and torch.equal(again[:off], store[:off])
+
+
+def test_a_capture_beside_an_eager_graph_of_the_operator_is_refused():
+    """The operator's own eager pass on the default stream, whose output is held, and then released."""
+    from originccl_b200.models import TinyLlamaStack
+    from originccl_b200.ops import embedding, experts as ex, norm
+    from originccl_b200.utils.graphs import capture
+    x = randn((64, 256), torch.float32, 1).requires_grad_()
+    w, b = (randn(256, torch.float32, s).requires_grad_() for s in (2, 3))
+    ids = some_ids(64, 64, "flat", 4)
+    order = ex.sort_by_expert(ids[:, None], 64)
+    for call in (lambda: norm.rms_norm(x, w), lambda: norm.layer_norm(x, w, b), lambda: embedding.embedding(ids, x),
+                 lambda: ex.dispatch(x, order), lambda: ex.combine(x, order)):
+        held = call()
+        with pytest.raises(RuntimeError, match="still alive"):
+            capture(call, warmup=0)
+        del held
+        capture(call, warmup=0).replay()
+    torch.cuda.synchronize()
+    m = TinyLlamaStack(hidden=64, ffn=128, layers=1, device="cuda", seed=5, vocab=64, native=True)
+    loss = m(ids).square().mean()
+    with pytest.raises(RuntimeError, match="still alive"):
+        capture(lambda: m(ids), warmup=0)
+    loss.backward()

@@ -323,6 +323,7 @@ def test_the_capture_rule_holds_only_where_a_graph_is_recorded(monkeypatch, mode
         norm.rms_norm(leaf, None)
     held = leaf * 2
     torch.autograd.graph.get_gradient_edge(leaf).node.metadata["bccl_stream"] = 7  # as if made on stream 7
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     for call in public_calls(leaf):
         with mode(), pytest.raises(ValueError, match="CUDA"):
@@ -385,3 +386,19 @@ def test_host_gradients_need_no_extension(monkeypatch):
     finally:
         monkeypatch.undo()
         importlib.reload(gradients)
+
+
+def test_the_capture_rule_looks_at_nothing_without_a_capture(monkeypatch):
+    """Eager training calls pay for no look-up of nodes."""
+    from originccl_b200.ops import _capture
+
+    def never(*_):
+        raise AssertionError("looked up")
+    monkeypatch.setattr(_capture, "guard", never)
+    leaf = torch.ones(4, 8, requires_grad=True)
+    for initialized in (False, True):
+        monkeypatch.setattr(torch.cuda, "is_initialized", lambda: initialized)
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+        for call in public_calls(leaf):
+            with pytest.raises(ValueError, match="CUDA"):
+                call()
