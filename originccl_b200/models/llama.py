@@ -125,7 +125,8 @@ class TinyLlamaStack(nn.Module):
         if not self.native:
             return norm(x)
         from ..ops import norm as native_norm
-        return native_norm.rms_norm(x, norm.weight, torch.finfo(x.dtype).eps if norm.eps is None else norm.eps)
+        # Where none is set torch takes the epsilon of its 32-bit arithmetic for the 16-bit types too.
+        return native_norm.rms_norm(x, norm.weight, torch.finfo(torch.float32).eps if norm.eps is None else norm.eps)
 
     def _lookup(self, ids):
         scale = self.embed.shape[1] ** 0.5

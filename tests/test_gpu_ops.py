@@ -1101,3 +1101,17 @@ def test_a_capture_beside_an_eager_graph_of_the_operator_is_refused():
     with pytest.raises(RuntimeError, match="still alive"):
         capture(lambda: m(ids), warmup=0)
     loss.backward()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+def test_a_native_stack_answers_as_torchs(dtype):
+    """Small activations, where the epsilon decides: torch takes that of its 32-bit arithmetic for every type.
+    Each side rounds twice at most (torch before the weights, which are ones): a step apart, and m as in check_norm twice."""
+    from originccl_b200.models import TinyLlamaStack
+    m = TinyLlamaStack(hidden=256, ffn=256, layers=1, device="cuda", dtype=dtype, native=True)
+    x = randn((40, 256), dtype, 1, 0.01)
+    n = m.blocks[0]["norm"]
+    for eps in (None, 1e-4):
+        n.eps = eps
+        got, want = m._norm(n, x).double(), n(x).double()
+        assert ((got - want).abs() <= (torch.finfo(dtype).eps + 128 * U) * want.abs() + 2 * TINY[dtype]).all()

@@ -402,3 +402,23 @@ def test_the_capture_rule_looks_at_nothing_without_a_capture(monkeypatch):
         for call in public_calls(leaf):
             with pytest.raises(ValueError, match="CUDA"):
                 call()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, bf, torch.float16])
+def test_a_native_stack_has_the_norms_of_torch(monkeypatch, dtype):
+    """Small activations, where the epsilon that a norm without one of its own takes decides. The kernel's place
+    is taken by the formula in 64 bits. The weights are ones, so each side rounds once: a step apart at most
+    (float32 sums of 64 squares and the root: 70 more)."""
+    from originccl_b200.models import TinyLlamaStack
+
+    def rms_norm(x, weight, eps):
+        d = x.double()
+        return (d * (d.square().mean(-1, keepdim=True) + eps).rsqrt() * weight.double()).to(x.dtype)
+    monkeypatch.setattr(norm, "rms_norm", rms_norm)
+    x = (torch.randn(5, 64, generator=torch.Generator().manual_seed(1)) * 0.01).to(dtype)
+    m = TinyLlamaStack(hidden=64, ffn=64, layers=1, dtype=dtype, native=True)
+    for eps in (None, 1e-4):
+        n = m.blocks[0]["norm"]
+        n.eps = eps
+        want = n(x).double()
+        assert ((m._norm(n, x).double() - want).abs() <= (torch.finfo(dtype).eps + 70 * 2 ** -24) * want.abs() + 1e-7).all()
