@@ -11,12 +11,14 @@
 #include <ATen/core/LegacyTypeDispatch.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
 
 #include <algorithm>
 #include <cstdint>
+#include <exception>
 #include <optional>
 #include <string>
 #include <utility>
@@ -733,10 +735,8 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
         return F(args);
     } catch (const Refusal& r) {
         if (r.type != nullptr) PyErr_SetString(r.type, r.what.c_str());
-    } catch (const std::bad_alloc&) {
-        PyErr_NoMemory();
-    } catch (const std::exception& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
+    } catch (...) {  // torch's own: an allocation that fails is a torch.OutOfMemoryError, as from torch's operators
+        torch::translate_exception_to_python(std::current_exception());
     }
     return nullptr;
 }

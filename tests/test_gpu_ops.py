@@ -1115,3 +1115,23 @@ def test_a_native_stack_answers_as_torchs(dtype):
         n.eps = eps
         got, want = m._norm(n, x).double(), n(x).double()
         assert ((got - want).abs() <= (torch.finfo(dtype).eps + 128 * U) * want.abs() + 2 * TINY[dtype]).all()
+
+
+def test_an_allocation_that_fails_is_torchs_error():
+    """What a program that looks for its largest batch catches. torch's allocator refuses by itself (the process'
+    share of the memory is set to less than the output), so the device is asked for nothing."""
+    from originccl_b200.ops import experts as ex, norm
+    row = torch.zeros(1, 1 << 20, device="cuda")
+    order = ex.sort_by_expert(torch.zeros(1 << 12, 1, dtype=torch.int32, device="cuda"), 1)
+    torch.cuda.synchronize()
+    torch.cuda.set_per_process_memory_fraction(0.02)
+    try:
+        for call in (lambda: norm.rms_norm_forward(row.expand(1 << 12, -1)),  # 16 GB
+                     lambda: ex.dispatch_forward(row.expand(1 << 12, -1), order)):
+            with pytest.raises(torch.OutOfMemoryError):
+                call()
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    y, _ = norm.rms_norm_forward(row.expand(2, -1))
+    torch.cuda.synchronize()
+    assert not y.any()
