@@ -46,6 +46,10 @@ def _host(op, grads, comm, replicated, outs=()):
     for t in (*grads, *outs):
         if t.is_cuda or t.dtype not in _FLOATS:
             raise ValueError(f"{op}: gradients must be float32, bfloat16 or float16 tensors, all on one device")
+    for t, o in zip(grads, outs):
+        if o.shape != t.shape or o.dtype not in (t.dtype, torch.float32):
+            raise ValueError(f"{op}: each out must have its gradient's shape, and its type or float32, got "
+                             f"{o.dtype} {tuple(o.shape)} for {t.dtype} {tuple(t.shape)}")
     total = torch.zeros(1, dtype=torch.float64)
     for i, t in enumerate(grads):
         share = comm.world_size if replicated is not None and replicated[i] else 1

@@ -422,3 +422,18 @@ def test_a_native_stack_has_the_norms_of_torch(monkeypatch, dtype):
         n.eps = eps
         want = n(x).double()
         assert ((m._norm(n, x).double() - want).abs() <= (torch.finfo(dtype).eps + 70 * 2 ** -24) * want.abs() + 1e-7).all()
+
+
+def test_host_clipping_refuses_outs_of_another_shape_or_type():
+    """As on a GPU: a larger out took the clipped values broadcast, and a narrower type lost them."""
+    g = [torch.ones(4), torch.ones(2, 3, dtype=bf)]
+    fine = [torch.full((4,), 7.0), torch.full((2, 3), 7.0)]
+    for i, out in ((0, torch.full((3, 4), 7.0)), (0, torch.full((4,), 7.0, dtype=bf)), (1, torch.full((2, 3), 7.0).half()),
+                   (1, torch.full((5, 2, 3), 7.0)), (0, torch.full((4,), 7.0, dtype=torch.float64))):
+        outs = list(fine)
+        outs[i] = out
+        with pytest.raises(ValueError, match="out|float32"):
+            gradients.clip_grad_norm(g, 1.0, outs=outs)
+        assert all((t == 7).all() for t in outs)
+    gradients.clip_grad_norm(g, 10.0, outs=fine)
+    assert all((t == 1).all() for t in fine)
